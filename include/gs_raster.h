@@ -91,7 +91,8 @@ const char* gs_last_error(void);
  * and gs_composite_bwd_l1 take a gs_clear_list_t; gs_preprocess_bwd and
  * gs_preprocess_bwd_w2c take zeroed.  Added since, with every call of 14 as it was:
  * gs_composite_segments_size, gs_composite_segments_size_for, gs_composite_fwd_seg,
- * gs_composite_bwd_seg; gs_l1_ssim_loss, gs_l1_ssim_loss_bwd. */
+ * gs_composite_bwd_seg; gs_l1_ssim_loss, gs_l1_ssim_loss_bwd; gs_grad_norms_workspace_size, gs_grad_norms,
+ * gs_adamw_step, gs_moments_encode, gs_moments_decode. */
 int gs_abi_version(void);
 
 /* Projection + covariance + SH colour for every Gaussian.
@@ -519,6 +520,61 @@ int gs_adam_step(void* stream, int num_arrays, float* const* params, const float
                  float* const* mus, float* const* nus, const int64_t* counts, const int* row_lens,
                  const double* lrs, const uint8_t* active, int64_t rows, int step, double b1,
                  double b2, double eps);
+
+/* Element types of the many-tensor operators below. */
+#define GS_TYPE_F32 0
+#define GS_TYPE_BF16 1
+#define GS_TYPE_F16 2
+/* Elements per block of 8-bit moments, and the multiple at which each tensor's moments begin. */
+#define GS_MOMENT_BLOCK 256
+
+/* Workspace bytes of gs_grad_norms for num tensors of counts[i] elements (0 for a bad size). */
+size_t gs_grad_norms_workspace_size(int num, const int64_t* counts);
+
+/* The 2-norm of each of num gradients (norms[num], may be NULL) and out[2] = {the norm of them
+ * all, the factor that clips}: s min(1, max_norm / (norm + 1e-6)) with s = grad_scale[0] (device
+ * scalar, NULL for 1; the norms are those of s times the gradients), s itself when max_norm <= 0,
+ * NaN when the norm is not finite.  grads, grad_types (GS_TYPE_*), counts and row_lens are host
+ * arrays, grads of device pointers aligned to their type.  With active (device, rows bytes) every
+ * tensor has rows x row_lens[i] elements, and rows whose byte is 0 are left out whatever they
+ * hold.  Sums are float64 in a fixed order.  workspace: 8-byte aligned. */
+int gs_grad_norms(void* stream, int num, const void* const* grads, const int* grad_types, const int64_t* counts,
+                  const int64_t* row_lens, const uint8_t* active, int64_t rows, double max_norm,
+                  const float* grad_scale, void* workspace, size_t workspace_bytes, float* norms, float* out);
+
+/* One AdamW step, in place, of num tensors of any sizes and of types GS_TYPE_* (gradients of
+ * types of their own).  Per element, g = s * gradient (0 in rows whose mask is 0),
+ *   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,
+ *   w -= lr_i ((m / (1 - b1^t)) / (sqrt(v) / sqrt(1 - b2^t) + eps) + decay_i w)
+ * in float32 with t = updates made, this one included; rows whose mask is 0 keep w.  s =
+ * grad_scale[0] (device scalar, NULL for 1); when it is not finite nothing changes and t stays.
+ * The moments are flat arrays of state_size elements, tensor i's from offsets[i] (a multiple of
+ * GS_MOMENT_BLOCK) on, each tensor in blocks of its own.  moment_bits 32: mu, nu are float32 (m
+ * and v), fields NULL.  moment_bits 8: mu, nu are bytes and fields holds two bytes per block
+ * (see gs_moments_encode), rounded stochastically by a hash of the element's place and key,
+ * which the caller changes from step to step.  Elements between tensors are left alone or
+ * written as zero.  master (may be NULL): float32 weights of half-typed tensors, flat as the
+ * moments; they are updated and the tensor gets their rounded value.
+ * powers (device, four doubles): b1^(t-1), b2^(t-1), 1 / (1 - b1^t), 1 / sqrt(1 - b2^t);
+ * powers_next, another four, receives those of the next step.
+ * Host arrays: params, grads (device pointers; a NULL gradient leaves tensor i alone),
+ * param_types, grad_types, offsets, counts, row_lens (NULL without active), lrs, decays. */
+int gs_adamw_step(void* stream, int num, void* const* params, const int* param_types, const void* const* grads,
+                  const int* grad_types, const int64_t* offsets, const int64_t* counts, const int64_t* row_lens,
+                  const double* lrs, const double* decays, int moment_bits, int64_t state_size, void* mu, void* nu,
+                  uint8_t* fields, float* master, const uint8_t* active, int64_t rows, const float* grad_scale,
+                  const double* powers, double* powers_next, double b1, double b2, double eps, uint32_t key);
+
+/* Moments m and v (float32, state_size elements, a multiple of GS_MOMENT_BLOCK) to 8 bits and
+ * back.  Per block, byte 0 of fields is the exponent field e_m + 127 of m, byte 1 e_r + 127 of
+ * r = sqrt(v); mu8 holds sign, 4 exponent and 3 mantissa bits, nu8 4 exponent and 4 mantissa
+ * bits of r: (1 + M / 2^k) 2^(E - 15 + e), for E = 0 (M / 2^k) 2^(-14 + e).  The largest magnitude
+ * code (127, 255) is "not finite" and decodes to NaN.  Encoding rounds to nearest even; a root
+ * above zero becomes at least code 1. */
+int gs_moments_encode(void* stream, int64_t state_size, const float* mu, const float* nu, uint8_t* mu8,
+                      uint8_t* nu8, uint8_t* fields);
+int gs_moments_decode(void* stream, int64_t state_size, const uint8_t* mu8, const uint8_t* nu8,
+                      const uint8_t* fields, float* mu, float* nu);
 
 /* Workspace bytes of gs_densify_and_prune for a capacity of M Gaussians. */
 size_t gs_densify_workspace_size(int64_t capacity);

@@ -1,0 +1,371 @@
+// AdamW over many tensors at once on gfx950, with moments in 32 or in 8 bits, and the
+// conversion of moments between the two.
+//
+// Per element, with g = scale * grad (0 in masked rows), t = updates made, this one included:
+//   m = b1 m + (1 - b1) g,   v = b2 v + (1 - b2) g^2,
+//   u = (m / (1 - b1^t)) / (sqrt(v) / sqrt(1 - b2^t) + eps),
+//   w = w - lr (u + decay w)                       (masked rows keep w).
+// Moments, weights and every operation are float32; half parameters are rounded once to
+// nearest even from the float32 result, which a master copy keeps when there is one.  A scale
+// that is not finite leaves everything as it is and does not count as an update.
+//
+// The state is flat: tensor i's moments begin at offsets[i], a multiple of 256, so that blocks
+// of the 8-bit form, whole quads and their alignment do not depend on the tensors' sizes.
+// A workgroup takes 1024 consecutive elements of one tensor, a wave one block, a lane four
+// elements.  The tensor is found by one comparison per lane and a ballot.
+#include "gs_moments.h"
+
+namespace gs {
+namespace {
+
+constexpr int kStepTensors = 56;   // per launch: the argument block stays below 4 KiB
+constexpr int kStepChunk = 1024;   // elements per workgroup
+
+struct StepTensor {
+  void* param;
+  const void* grad;
+  int64_t at;          // first element in the state
+  int64_t count;
+  uint64_t row_magic;  // floor(2^64 / row_len) + 1 (0: row_len 1)
+  int32_t row_len;
+  float lr, decay;
+  int32_t kind;        // parameter type * 6 + gradient type * 2 + master
+};
+
+struct StepArgs {
+  StepTensor t[kStepTensors];
+  uint32_t begin[64];  // first workgroup of each tensor, ~0 after the last
+  void* mu;
+  void* nu;
+  uint8_t* fields;
+  float* master;
+  const uint8_t* active;
+  const float* scale;
+  const double* powers;  // b1^(t-1), b2^(t-1), 1 / (1 - b1^t), 1 / sqrt(1 - b2^t)
+  double* powers_next;   // NULL in all launches of a step but the first
+  double b1d, b2d;
+  float b1, b2, omb1, omb2, eps;
+  uint32_t key;
+};
+static_assert(sizeof(StepArgs) <= 4096, "kernel arguments");
+
+template <class T>
+__device__ inline void load4(const T* p, int n, float (&x)[4]) {
+  // the vector is only as aligned as its element: a tensor may begin anywhere
+  typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  if (n >= 4) {
+    const vec v = *reinterpret_cast<const vec*>(p);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = (float)v[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = j < n ? (float)p[j] : 0.0f;
+  }
+}
+template <class T>
+__device__ inline void store4(T* p, int n, const float (&x)[4]) {
+  typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  if (n >= 4) {
+    vec v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = (T)x[j];
+    *reinterpret_cast<vec*>(p) = v;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) p[j] = (T)x[j];
+  }
+}
+
+// Mask of four consecutive elements from `tid` * 4 within the workgroup's chunk.
+__device__ inline void rows_on(const StepArgs& A, const StepTensor& t, int64_t base, int n, bool (&on)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) on[j] = true;
+  if (A.active == nullptr) return;
+  // row of the chunk's first element by a 64-bit reciprocal (exact for base * row_len < 2^64),
+  // of the lane's by a 32-bit one: rem + 1024 elements hold few rows
+  const uint64_t row0 = t.row_magic ? __umul64hi((uint64_t)base, t.row_magic) : (uint64_t)base;
+  const uint32_t L = (uint32_t)t.row_len;
+  uint32_t e = (uint32_t)((uint64_t)base - row0 * L) + threadIdx.x * 4u;
+  uint32_t q;
+  if (L > 4096u) {
+    q = e >= L ? 1u : 0u;
+  } else {
+    q = t.row_magic ? __umulhi(e, (uint32_t)(t.row_magic >> 32) + 1u) : e;
+  }
+  e -= q * L;
+  const uint8_t* a = A.active + row0 + q;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (j < n) on[j] = *a != 0;
+    if (++e == L) {
+      e = 0;
+      ++a;
+    }
+  }
+}
+
+template <bool k8, class P, class G, bool kMaster>
+__device__ inline void step_chunk(const StepArgs& A, const StepTensor& t, int64_t base, float scale, float r1,
+                                  float r2) {
+  const int64_t e = base + (int64_t)threadIdx.x * 4;
+  if (base + (int64_t)(threadIdx.x & ~63u) * 4 >= t.count) return;  // the wave's block is past the end
+  const int64_t left = t.count - e;
+  const int n = left >= 4 ? 4 : left > 0 ? (int)left : 0;
+  const int64_t at = t.at + e;
+  float w[4], g[4], m[4], r[4], v[4];
+  load4((const G*)t.grad + e, n, g);
+  if (kMaster) load4(A.master + at, 4, w);
+  else load4((const P*)t.param + e, n, w);
+  const int64_t block = at >> 8;
+  if (k8) {
+    const uint32_t m8 = *(const uint32_t*)((const uint8_t*)A.mu + at);
+    const uint32_t r8 = *(const uint32_t*)((const uint8_t*)A.nu + at);
+    const uint32_t f = *(const uint16_t*)(A.fields + 2 * block);
+    decode_m4(m8, (int)(f & 255u), m);
+    decode_r4(r8, (int)(f >> 8), r);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = r[j] * r[j];
+  } else {
+    load4((const float*)A.mu + at, 4, m);
+    load4((const float*)A.nu + at, 4, v);
+  }
+  bool on[4];
+  rows_on(A, t, base, n, on);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float x = on[j] ? g[j] * scale : 0.0f;
+    m[j] = m[j] * A.b1 + x * A.omb1;
+    v[j] = v[j] * A.b2 + (x * x) * A.omb2;
+    r[j] = sqrtf(v[j]);
+    const float u = (m[j] * r1) / (r[j] * r2 + A.eps);
+    const float y = w[j] - t.lr * (u + t.decay * w[j]);
+    w[j] = on[j] ? y : w[j];
+  }
+  if (n > 0) {
+    store4((P*)t.param + e, n, w);
+    if (kMaster) store4(A.master + at, n, w);
+  }
+  if (k8) {
+    uint32_t h[4], m8, r8, f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[j] = place_hash(at + j, A.key);
+    encode_block<true>(m, r, h, m8, r8, f);
+    *(uint32_t*)((uint8_t*)A.mu + at) = m8;
+    *(uint32_t*)((uint8_t*)A.nu + at) = r8;
+    if ((threadIdx.x & 63u) == 0) *(uint16_t*)(A.fields + 2 * block) = (uint16_t)f;
+  } else {
+    store4((float*)A.mu + at, 4, m);
+    store4((float*)A.nu + at, 4, v);
+  }
+}
+
+template <bool k8>
+__global__ __launch_bounds__(256) void adamw_kernel(StepArgs A) {
+  const float scale = A.scale ? *A.scale : 1.0f;
+  const bool ok = fabsf(scale) < __builtin_huge_valf();
+  if (A.powers_next != nullptr && blockIdx.x == 0 && threadIdx.x == 0) {
+    if (ok) {
+      const double p1 = A.powers[0] * A.b1d, p2 = A.powers[1] * A.b2d;
+      A.powers_next[0] = p1;
+      A.powers_next[1] = p2;
+      A.powers_next[2] = 1.0 / (1.0 - p1 * A.b1d);
+      A.powers_next[3] = 1.0 / sqrt(1.0 - p2 * A.b2d);
+    } else {
+      for (int j = 0; j < 4; ++j) A.powers_next[j] = A.powers[j];
+    }
+  }
+  if (!ok) return;
+  const uint32_t b = blockIdx.x;
+  const int k = __popcll(__ballot(b >= A.begin[threadIdx.x & 63u])) - 1;
+  if (k < 0) return;
+  const StepTensor t = A.t[k];
+  const int64_t base = (int64_t)(b - A.begin[k]) * kStepChunk;
+  const float r1 = (float)A.powers[2], r2 = (float)A.powers[3];
+  switch (t.kind) {
+#define GS_STEP(i, P, G, M)                                \
+  case i:                                                  \
+    step_chunk<k8, P, G, M>(A, t, base, scale, r1, r2);    \
+    break;
+    GS_STEP(0, float, float, false)
+    GS_STEP(2, float, __bf16, false)
+    GS_STEP(4, float, _Float16, false)
+    GS_STEP(6, __bf16, float, false)
+    GS_STEP(7, __bf16, float, true)
+    GS_STEP(8, __bf16, __bf16, false)
+    GS_STEP(9, __bf16, __bf16, true)
+    GS_STEP(10, __bf16, _Float16, false)
+    GS_STEP(11, __bf16, _Float16, true)
+    GS_STEP(12, _Float16, float, false)
+    GS_STEP(13, _Float16, float, true)
+    GS_STEP(14, _Float16, __bf16, false)
+    GS_STEP(15, _Float16, __bf16, true)
+    GS_STEP(16, _Float16, _Float16, false)
+    GS_STEP(17, _Float16, _Float16, true)
+#undef GS_STEP
+  }
+}
+
+__global__ __launch_bounds__(256) void moments_encode_kernel(int64_t blocks, const float* __restrict__ mu,
+                                                             const float* __restrict__ nu, uint8_t* __restrict__ m8,
+                                                             uint8_t* __restrict__ r8, uint8_t* __restrict__ fields) {
+  const int64_t block = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (block >= blocks) return;
+  const int64_t at = block * kMomBlock + (threadIdx.x & 63u) * 4;
+  float m[4], r[4];
+  load4(mu + at, 4, m);
+  load4(nu + at, 4, r);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) r[j] = sqrtf(r[j]);
+  const uint32_t none[4] = {0, 0, 0, 0};
+  uint32_t cm, cr, f;
+  encode_block<false>(m, r, none, cm, cr, f);
+  *(uint32_t*)(m8 + at) = cm;
+  *(uint32_t*)(r8 + at) = cr;
+  if ((threadIdx.x & 63u) == 0) *(uint16_t*)(fields + 2 * block) = (uint16_t)f;
+}
+
+__global__ __launch_bounds__(256) void moments_decode_kernel(int64_t blocks, const uint8_t* __restrict__ m8,
+                                                             const uint8_t* __restrict__ r8,
+                                                             const uint8_t* __restrict__ fields,
+                                                             float* __restrict__ mu, float* __restrict__ nu) {
+  const int64_t block = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (block >= blocks) return;
+  const int64_t at = block * kMomBlock + (threadIdx.x & 63u) * 4;
+  const uint32_t f = *(const uint16_t*)(fields + 2 * block);
+  float m[4], r[4];
+  decode_m4(*(const uint32_t*)(m8 + at), (int)(f & 255u), m);
+  decode_r4(*(const uint32_t*)(r8 + at), (int)(f >> 8), r);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) r[j] = r[j] * r[j];
+  store4(mu + at, 4, m);
+  store4(nu + at, 4, r);
+}
+
+bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+size_t size_of(int type) { return type == GS_TYPE_F32 ? 4 : 2; }
+
+}  // namespace
+}  // namespace gs
+
+using namespace gs;
+
+extern "C" int gs_adamw_step(void* stream, int num, void* const* params, const int* param_types,
+                             const void* const* grads, const int* grad_types, const int64_t* offsets,
+                             const int64_t* counts, const int64_t* row_lens, const double* lrs,
+                             const double* decays, int moment_bits, int64_t state_size, void* mu, void* nu,
+                             uint8_t* fields, float* master, const uint8_t* active, int64_t rows,
+                             const float* grad_scale, const double* powers, double* powers_next, double b1,
+                             double b2, double eps, uint32_t key) {
+  GS_REQUIRE(num >= 0, "gs_adamw_step: %d tensors", num);
+  GS_REQUIRE(num == 0 || (params && param_types && grads && grad_types && offsets && counts && lrs && decays),
+             "gs_adamw_step: NULL argument");
+  GS_REQUIRE(moment_bits == 32 || moment_bits == 8, "gs_adamw_step: moments in 32 or 8 bits, not %d", moment_bits);
+  GS_REQUIRE(state_size >= 0 && state_size % kMomBlock == 0, "gs_adamw_step: state of %lld elements",
+             (long long)state_size);
+  GS_REQUIRE(state_size == 0 || (mu && nu && (moment_bits == 32 || fields)), "gs_adamw_step: NULL state");
+  GS_REQUIRE(aligned(mu, 16) && aligned(nu, 16) && aligned(fields, 2) && aligned(master, 16),
+             "gs_adamw_step: the state's arrays must be 16-byte aligned");
+  GS_REQUIRE(powers && powers_next && powers != powers_next, "gs_adamw_step: two arrays of powers are needed");
+  GS_REQUIRE(b1 >= 0.0 && b1 < 1.0 && b2 >= 0.0 && b2 < 1.0, "gs_adamw_step: b1 and b2 must be in [0, 1)");
+  GS_REQUIRE(eps >= 0.0, "gs_adamw_step: eps must not be negative");
+  GS_REQUIRE(!active || row_lens, "gs_adamw_step: a mask needs row lengths");
+  for (int i = 0; i < num; ++i) {
+    if (!grads[i] || counts[i] == 0) continue;
+    const int pt = param_types[i], gt = grad_types[i];
+    GS_REQUIRE(pt >= GS_TYPE_F32 && pt <= GS_TYPE_F16 && gt >= GS_TYPE_F32 && gt <= GS_TYPE_F16,
+               "gs_adamw_step: type of tensor %d", i);
+    GS_REQUIRE(counts[i] > 0 && counts[i] < ((int64_t)1 << 40), "gs_adamw_step: tensor %d has %lld elements", i,
+               (long long)counts[i]);
+    GS_REQUIRE(params[i], "gs_adamw_step: NULL tensor %d", i);
+    GS_REQUIRE(aligned(params[i], size_of(pt)) && aligned(grads[i], size_of(gt)),
+               "gs_adamw_step: tensor %d is not aligned to its type", i);
+    GS_REQUIRE(offsets[i] >= 0 && offsets[i] % kMomBlock == 0 && offsets[i] <= state_size &&
+                   counts[i] <= state_size - offsets[i],
+               "gs_adamw_step: tensor %d lies outside the state", i);
+    if (active)
+      GS_REQUIRE(row_lens[i] >= 1 && row_lens[i] < ((int64_t)1 << 24) && rows >= 0 &&
+                     counts[i] % row_lens[i] == 0 && counts[i] / row_lens[i] == rows,
+                 "gs_adamw_step: tensor %d has %lld elements, not rows x row length", i, (long long)counts[i]);
+  }
+  StepArgs A{};
+  A.mu = mu;
+  A.nu = nu;
+  A.fields = fields;
+  A.master = master;
+  A.active = active;
+  A.scale = grad_scale;
+  A.powers = powers;
+  A.powers_next = powers_next;
+  A.b1d = b1;
+  A.b2d = b2;
+  A.b1 = (float)b1;
+  A.b2 = (float)b2;
+  A.omb1 = (float)(1.0 - b1);
+  A.omb2 = (float)(1.0 - b2);
+  A.eps = (float)eps;
+  A.key = key;
+  hipStream_t s = (hipStream_t)stream;
+  // always one launch, so that the powers move on; further ones take what does not fit it
+  int i = 0;
+  do {
+    int k = 0;
+    int64_t groups = 0;
+    for (; i < num && k < kStepTensors; ++i) {
+      if (!grads[i] || counts[i] == 0) continue;
+      const int64_t more = (counts[i] + kStepChunk - 1) / kStepChunk;
+      if (k > 0 && groups + more > 0x7fffffff) break;
+      StepTensor& t = A.t[k];
+      t.param = params[i];
+      t.grad = grads[i];
+      t.at = offsets[i];
+      t.count = counts[i];
+      t.row_len = active ? (int32_t)row_lens[i] : 1;
+      t.row_magic = t.row_len > 1 ? ~(uint64_t)0 / (uint64_t)t.row_len + 1 : 0;
+      t.lr = (float)lrs[i];
+      t.decay = (float)decays[i];
+      t.kind = param_types[i] * 6 + grad_types[i] * 2 + (param_types[i] != GS_TYPE_F32 && master ? 1 : 0);
+      A.begin[k++] = (uint32_t)groups;
+      groups += more;
+    }
+    for (; k < 64; ++k) A.begin[k] = 0xffffffffu;
+    const dim3 grid((unsigned)(groups > 0 ? groups : 1));
+    if (moment_bits == 8) hipLaunchKernelGGL(adamw_kernel<true>, grid, dim3(256), 0, s, A);
+    else hipLaunchKernelGGL(adamw_kernel<false>, grid, dim3(256), 0, s, A);
+    GS_LAUNCH_CHECK("adamw_kernel");
+    A.powers_next = nullptr;
+    while (i < num && (!grads[i] || counts[i] == 0)) ++i;
+  } while (i < num);
+  return GS_OK;
+}
+
+extern "C" int gs_moments_encode(void* stream, int64_t state_size, const float* mu, const float* nu, uint8_t* mu8,
+                                 uint8_t* nu8, uint8_t* fields) {
+  GS_REQUIRE(state_size >= 0 && state_size % kMomBlock == 0 && state_size < ((int64_t)1 << 40),
+             "gs_moments_encode: state of %lld elements", (long long)state_size);
+  if (state_size == 0) return GS_OK;
+  GS_REQUIRE(mu && nu && mu8 && nu8 && fields, "gs_moments_encode: NULL argument");
+  GS_REQUIRE(aligned(mu, 16) && aligned(nu, 16) && aligned(mu8, 16) && aligned(nu8, 16) && aligned(fields, 2),
+             "gs_moments_encode: the state's arrays must be 16-byte aligned");
+  const int64_t blocks = state_size / kMomBlock;
+  hipLaunchKernelGGL(moments_encode_kernel, dim3((unsigned)div_up(blocks, 4)), dim3(256), 0, (hipStream_t)stream,
+                     blocks, mu, nu, mu8, nu8, fields);
+  GS_LAUNCH_CHECK("moments_encode_kernel");
+  return GS_OK;
+}
+
+extern "C" int gs_moments_decode(void* stream, int64_t state_size, const uint8_t* mu8, const uint8_t* nu8,
+                                 const uint8_t* fields, float* mu, float* nu) {
+  GS_REQUIRE(state_size >= 0 && state_size % kMomBlock == 0 && state_size < ((int64_t)1 << 40),
+             "gs_moments_decode: state of %lld elements", (long long)state_size);
+  if (state_size == 0) return GS_OK;
+  GS_REQUIRE(mu && nu && mu8 && nu8 && fields, "gs_moments_decode: NULL argument");
+  GS_REQUIRE(aligned(mu, 16) && aligned(nu, 16) && aligned(mu8, 16) && aligned(nu8, 16) && aligned(fields, 2),
+             "gs_moments_decode: the state's arrays must be 16-byte aligned");
+  const int64_t blocks = state_size / kMomBlock;
+  hipLaunchKernelGGL(moments_decode_kernel, dim3((unsigned)div_up(blocks, 4)), dim3(256), 0, (hipStream_t)stream,
+                     blocks, mu8, nu8, fields, mu, nu);
+  GS_LAUNCH_CHECK("moments_decode_kernel");
+  return GS_OK;
+}

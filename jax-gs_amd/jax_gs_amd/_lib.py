@@ -109,6 +109,12 @@ _SIGS = {
     "gs_l1_ssim_loss_bwd": [_P, _I, _I, _I, _P, _P, ctypes.c_double, _P, _P, _P, _P, _P, _SZ, _P],
     "gs_adam_step": [_P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I, ctypes.c_double, ctypes.c_double,
                      ctypes.c_double],
+    "gs_grad_norms_workspace_size": [_I, _P],
+    "gs_grad_norms": [_P, _I, _P, _P, _P, _P, _P, _I64, ctypes.c_double, _P, _P, _SZ, _P, _P],
+    "gs_adamw_step": [_P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I64, _P, _P, _P, _P, _P, _I64, _P, _P, _P,
+                      ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_uint32],
+    "gs_moments_encode": [_P, _I64, _P, _P, _P, _P, _P],
+    "gs_moments_decode": [_P, _I64, _P, _P, _P, _P, _P],
     "gs_densify_accumulate": [_P, _I64, _P, _P, _P, _F, _F, _P, _P, _P, _P, _P, _P],
 }
 _RESTYPE = {"gs_last_error": ctypes.c_char_p, "gs_bin_workspace_size": _SZ, "gs_l1_ssim_workspace_size": _SZ,
@@ -116,7 +122,7 @@ _RESTYPE = {"gs_last_error": ctypes.c_char_p, "gs_bin_workspace_size": _SZ, "gs_
             "gs_bin_reference_workspace_size": _SZ, "gs_preprocess_bwd_w2c_workspace_size": _SZ,
             "gs_l1_ssim_window_workspace_size": _SZ,
             "gs_densify_workspace_size": _SZ, "gs_composite_segments_size": _SZ,
-            "gs_composite_segments_size_for": _SZ, "gs_composite_l1_out_size": _I64}
+            "gs_composite_segments_size_for": _SZ, "gs_grad_norms_workspace_size": _SZ, "gs_composite_l1_out_size": _I64}
 
 _lib = None
 

@@ -1,0 +1,400 @@
+"""AdamW over many tensors at once, with moments in 32 or in 8 bits, and gradient norms with
+the factor that clips them.
+
+For models of any number of tensors of any sizes (the five Gaussian arrays, and whatever is
+trained next to them); ``optimizer.Adam`` stays the reference trainer's own step.  One launch
+updates up to 56 tensors, nothing waits for the host, and a step whose gradients are not finite
+changes nothing when its scale comes from ``grad_norms``:
+
+    optimizer = AdamW(1e-3, weight_decay=0.01, moment_bits=8, max_grad_norm=1.0)
+    state = optimizer.init(params)
+    optimizer.step(params, grads, state)
+
+``params`` and ``grads`` are ``Gaussians``, dicts, lists or tuples of tensors, or one tensor:
+float32, bfloat16 or float16, gradients of a type of their own (``None``: the tensor is left
+alone).  The arithmetic is float32; the kernels are ``gs_adamw_step``, ``gs_grad_norms``,
+``gs_moments_encode`` and ``gs_moments_decode``.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Callable, Dict, List, NamedTuple, Optional, Sequence, Union
+
+import torch
+
+from .. import _lib
+from ..core.gaussians import Gaussians
+from ..renderer._buffers import as_bytes
+from .optimizer import FIELDS, make_optimizer
+
+LearningRate = Union[float, Callable[[int], float]]
+BLOCK = 256  # elements that share an exponent in 8 bits; each tensor's moments begin at a multiple
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_MASK32 = 0xFFFFFFFF
+
+
+class GradNorms(NamedTuple):
+    """Device float32: the norm of all gradients, each tensor's, and the factor for the step."""
+    total: torch.Tensor
+    per_tensor: torch.Tensor
+    scale: torch.Tensor
+
+
+def _keys(x) -> Optional[list]:
+    if isinstance(x, Gaussians):
+        return list(FIELDS)
+    return list(x) if isinstance(x, dict) else None
+
+
+def _tensors(x, keys=None) -> list:
+    if isinstance(x, torch.Tensor):
+        return [x]
+    if isinstance(x, Gaussians):
+        return [getattr(x, f) for f in FIELDS]
+    if isinstance(x, dict):
+        return [x[k] for k in (x if keys is None else keys)]
+    return list(x)
+
+
+def _like(keys, values):
+    return list(values) if keys is None else dict(zip(keys, values))
+
+
+def _device(tensors, what: str) -> torch.device:
+    dev = tensors[0].device
+    if dev.type != "cuda":
+        raise ValueError(f"{what}: tensors must live on the GPU (there is no CPU path)")
+    return dev
+
+
+def _types(tensors, what: str) -> list:
+    try:
+        return [_TYPES[t.dtype] for t in tensors]
+    except KeyError as e:
+        raise TypeError(f"{what}: tensors must be float32, bfloat16 or float16, not {e.args[0]}") from None
+
+
+def _mask(active_mask, tensors, dev, what: str):
+    """(mask bytes, rows, elements per row of each tensor) for a mask over leading rows."""
+    act = as_bytes(torch.as_tensor(active_mask, device=dev))
+    rows = act.numel()
+    if act.dim() != 1:
+        raise ValueError(f"{what}: active_mask must have one dimension")
+    for i, t in enumerate(tensors):
+        if t is not None and (t.dim() == 0 or t.shape[0] != rows):
+            raise ValueError(f"{what}: active_mask has {rows} entries, tensor {i} has shape {tuple(t.shape)}")
+    lens = [1 if t is None or rows == 0 else max(t.numel() // rows, 1) for t in tensors]
+    return act, rows, (ctypes.c_int64 * len(lens))(*lens)
+
+
+def _scalar(grad_scale, dev, what: str):
+    if grad_scale is None:
+        return None
+    if not isinstance(grad_scale, torch.Tensor):
+        return torch.full((), float(grad_scale), device=dev)
+    if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != dev:
+        raise ValueError(f"{what}: grad_scale must be one float32 on {dev}")
+    return grad_scale
+
+
+def grad_norms(grads, max_norm: Optional[float] = None, active_mask=None, grad_scale=None) -> GradNorms:
+    """2-norms of grad_scale times the gradients, per tensor and of all, and the factor
+    ``grad_scale * min(1, max_norm / (total + 1e-6))`` (``grad_scale`` without ``max_norm``),
+    NaN when the total is not finite, all on the device.  Rows where ``active_mask`` is False
+    are left out, whatever they hold; ``None`` gradients count as empty."""
+    gs = _tensors(grads)
+    have = [g for g in gs if g is not None]
+    if not have:
+        raise ValueError("grad_norms: no gradients")
+    dev = _device(have, "grad_norms")
+    k = len(gs)
+    act, rows, lens = None, 0, None
+    if active_mask is not None:
+        act, rows, lens = _mask(active_mask, gs, dev, "grad_norms")
+    if len(have) < k or not all([g.is_contiguous() for g in gs]):
+        some = have[0].new_empty(0)
+        gs = [some if g is None else g.contiguous() for g in gs]
+        if act is not None:
+            # an empty tensor has no rows: pass the others, and put zeros in its place
+            at = [i for i, g in enumerate(gs) if g.numel() or rows == 0]
+            if len(at) < k:
+                got = grad_norms([gs[i] for i in at], max_norm, active_mask, grad_scale)
+                each = got.per_tensor.new_zeros(k)
+                each[at] = got.per_tensor
+                return GradNorms(got.total, each, got.scale)
+    types = _types(gs, "grad_norms")
+    if any([g.device != dev for g in gs]):
+        raise ValueError(f"grad_norms: tensors on different devices, the first on {dev}")
+    scale = _scalar(grad_scale, dev, "grad_norms")
+    I64 = ctypes.c_int64 * k
+    counts = I64(*[g.numel() for g in gs])
+    nbytes = _lib.lib().gs_grad_norms_workspace_size(k, counts)
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+    out = torch.empty((k + 2,), dtype=torch.float32, device=dev)
+    at = out.data_ptr()
+    _lib.call("gs_grad_norms", _lib.stream_handle(dev), k, (ctypes.c_void_p * k)(*[g.data_ptr() for g in gs]),
+              (ctypes.c_int * k)(*types), counts, lens, _lib.ptr(act), rows,
+              0.0 if max_norm is None else float(max_norm), _lib.ptr(scale), ctypes.c_void_p(ws.data_ptr()), nbytes,
+              ctypes.c_void_p(at + 8), ctypes.c_void_p(at))
+    return GradNorms(out[0], out[2:], out[1])
+
+
+class AdamWState:
+    """Moments and step count of one model's parameters.
+
+    ``mu_flat`` and ``nu_flat`` hold all moments: tensor i's from ``offsets[i]`` on, a multiple
+    of 256, zeros between.  With ``bits`` 32 they are float32 and ``mu``/``nu`` give them tensor
+    by tensor, as views.  With ``bits`` 8 they are bytes with two exponent bytes per 256 elements
+    in ``fields``: ``mu_flat`` a sign, four exponent and three mantissa bits, ``nu_flat`` four
+    exponent and four mantissa bits of the root of the second moment (``gs_moments_encode``).
+    ``master_flat`` holds float32 weights of half-typed tensors, if asked for.  ``count`` is the
+    number of steps asked for; ``powers`` (device float64) belongs to the updates made, which
+    are fewer if a scale was not finite."""
+
+    def __init__(self, keys, shapes, bits: int):
+        self.keys, self.shapes, self.bits = keys, [tuple(s) for s in shapes], bits
+        self.counts, self.offsets, at = [], [], 0
+        for s in self.shapes:
+            n = 1
+            for d in s:
+                n *= d
+            self.counts.append(n)
+            self.offsets.append(at)
+            at += -(-n // BLOCK) * BLOCK
+        self.size = at
+        k = len(self.shapes)
+        self._counts = (ctypes.c_int64 * k)(*self.counts)
+        self._offsets = (ctypes.c_int64 * k)(*self.offsets)
+        self.mu_flat = self.nu_flat = self.fields = self.master_flat = self.powers = None
+        self.count = 0
+        self.norms: Optional[GradNorms] = None
+
+    def _allocate(self, dev, zero: bool):
+        new = torch.zeros if zero else torch.empty
+        dtype = torch.float32 if self.bits == 32 else torch.uint8
+        self.mu_flat, self.nu_flat = (new((self.size,), dtype=dtype, device=dev) for _ in range(2))
+        self.fields = new((self.size // BLOCK, 2), dtype=torch.uint8, device=dev) if self.bits == 8 else None
+
+    def _views(self, flat):
+        return _like(self.keys, [flat[o:o + n].view(s) for o, n, s in zip(self.offsets, self.counts, self.shapes)])
+
+    @property
+    def mu(self):
+        """First moments, tensor by tensor: views of a 32-bit state."""
+        return self.moments()[0] if self._is32("mu") else None
+
+    @property
+    def nu(self):
+        """Second moments, tensor by tensor: views of a 32-bit state."""
+        return self.moments()[1] if self._is32("nu") else None
+
+    @property
+    def master(self):
+        """Float32 weights, tensor by tensor (those of float32 tensors are not kept up), or None."""
+        return None if self.master_flat is None else self._views(self.master_flat)
+
+    def _is32(self, name):
+        if self.bits != 32:
+            raise ValueError(f"AdamWState.{name}: this state is in 8 bits: moments() has its values")
+        return True
+
+    def moments(self):
+        """(first, second) moments in float32, tensor by tensor: views of a 32-bit state, the
+        values that an 8-bit state stands for."""
+        s = self if self.bits == 32 else self.convert(32)
+        return s._views(s.mu_flat), s._views(s.nu_flat)
+
+    def convert(self, bits: int) -> "AdamWState":
+        """A state of its own with the same moments in ``bits`` (32 or 8), to nearest."""
+        if bits not in (32, 8):
+            raise ValueError(f"AdamWState.convert: 32 or 8 bits, not {bits}")
+        to = AdamWState(self.keys, self.shapes, bits)
+        to.count, to.powers = self.count, self.powers  # never written in place
+        to.master_flat = None if self.master_flat is None else self.master_flat.clone()
+        to._allocate(self.mu_flat.device, zero=False)
+        to.set_moments(self)
+        return to
+
+    def set_moments(self, other: "AdamWState") -> None:
+        """Take over another state's moments (of the same tensors), to nearest."""
+        if other.shapes != self.shapes:
+            raise ValueError("AdamWState.set_moments: states of different tensors")
+        dev = self.mu_flat.device
+        if self.bits == other.bits:
+            for name in ("mu_flat", "nu_flat", "fields"):
+                if getattr(self, name) is not None:
+                    getattr(self, name).copy_(getattr(other, name))
+        elif self.bits == 8:
+            _lib.call("gs_moments_encode", _lib.stream_handle(dev), self.size, _lib.ptr(other.mu_flat),
+                      _lib.ptr(other.nu_flat), _lib.ptr(self.mu_flat), _lib.ptr(self.nu_flat), _lib.ptr(self.fields))
+        else:
+            _lib.call("gs_moments_decode", _lib.stream_handle(dev), self.size, _lib.ptr(other.mu_flat),
+                      _lib.ptr(other.nu_flat), _lib.ptr(other.fields), _lib.ptr(self.mu_flat), _lib.ptr(self.nu_flat))
+
+    def state_dict(self) -> dict:
+        """The state as a dict of tensors (the state's own) and plain values, for a checkpoint."""
+        return {"bits": self.bits, "shapes": list(self.shapes), "count": self.count, "mu_flat": self.mu_flat,
+                "nu_flat": self.nu_flat, "fields": self.fields, "master_flat": self.master_flat,
+                "powers": self.powers}
+
+
+class AdamW:
+    """w -= lr ((m / (1 - b1^t)) / (sqrt(v) / sqrt(1 - b2^t) + eps) + weight_decay w).
+
+    ``learning_rates`` and ``weight_decay`` are one value for all tensors, or a list or dict
+    like the parameters; a rate may be a schedule of the step count (``exponential_decay``).
+    ``moment_bits`` 8 holds the moments in 8 bits, rounded stochastically with random bits that
+    follow from ``seed``, the step and the element.  ``master_weights`` keeps float32 weights of
+    half-typed parameters in the state.  With ``max_grad_norm`` every step takes the gradients'
+    norm first (``state.norms``), scales them down to it, and leaves everything as it is when
+    it is not finite."""
+
+    def __init__(self, learning_rates, b1: float = 0.9, b2: float = 0.999, eps: float = 1e-8, weight_decay=0.0,
+                 moment_bits: int = 32, master_weights: bool = False, max_grad_norm: Optional[float] = None,
+                 seed: int = 0):
+        if moment_bits not in (32, 8):
+            raise ValueError(f"AdamW: moments in 32 or 8 bits, not {moment_bits}")
+        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+            raise ValueError(f"AdamW: b1 and b2 must be in [0, 1), not {b1}, {b2}")
+        if not eps >= 0.0:
+            raise ValueError(f"AdamW: eps must not be negative, not {eps}")
+        if max_grad_norm is not None and not max_grad_norm > 0.0:
+            raise ValueError(f"AdamW: max_grad_norm must be positive, not {max_grad_norm}")
+        self.lrs, self.decay = learning_rates, weight_decay
+        self.b1, self.b2, self.eps = float(b1), float(b2), float(eps)
+        self.moment_bits, self.master_weights = moment_bits, bool(master_weights)
+        self.max_grad_norm, self.seed = max_grad_norm, int(seed)
+
+    def _powers(self, t: int, dev) -> torch.Tensor:
+        p1, p2 = self.b1 ** t, self.b2 ** t
+        return torch.tensor([p1, p2, 1.0 / (1.0 - p1 * self.b1), (1.0 - p2 * self.b2) ** -0.5], dtype=torch.float64,
+                            device=dev)
+
+    @staticmethod
+    def _each(values, state: AdamWState, what: str) -> list:
+        k = len(state.shapes)
+        if isinstance(values, dict):
+            missing = [x for x in (state.keys or ()) if x not in values]
+            if state.keys is None or missing:
+                raise ValueError(f"AdamW: {what} for {missing or 'parameters without names'} missing")
+            return [values[x] for x in state.keys]
+        if isinstance(values, (list, tuple)):
+            if len(values) != k:
+                raise ValueError(f"AdamW: {len(values)} values of {what} for {k} tensors")
+            return list(values)
+        return [values] * k
+
+    def _state(self, params, bits) -> AdamWState:
+        ps = _tensors(params)
+        if not ps:
+            raise ValueError("AdamW: no parameters")
+        _device(ps, "AdamW")
+        _types(ps, "AdamW")
+        state = AdamWState(_keys(params), [p.shape for p in ps], bits)
+        self._each(self.lrs, state, "the learning rate")
+        self._each(self.decay, state, "weight_decay")
+        return state
+
+    def _masters(self, state: AdamWState, ps, master) -> None:
+        if not self.master_weights or all([p.dtype == torch.float32 for p in ps]):
+            return
+        state.master_flat = torch.zeros((state.size,), dtype=torch.float32, device=ps[0].device)
+        for o, n, x in zip(state.offsets, state.counts, ps if master is None else _tensors(master, state.keys)):
+            state.master_flat[o:o + n].copy_(x.detach().reshape(-1))
+
+    def init(self, params) -> AdamWState:
+        """Zero moments for these parameters, no step made."""
+        state = self._state(params, self.moment_bits)
+        ps = _tensors(params)
+        state._allocate(ps[0].device, zero=True)
+        state.powers = self._powers(0, ps[0].device)
+        self._masters(state, ps, None)
+        return state
+
+    def restore(self, params, mu, nu, count: int, master=None) -> AdamWState:
+        """The state after ``count`` updates from first and second moments in 32 bits given
+        tensor by tensor (an ``AdamState``'s ``mu`` and ``nu``, for one)."""
+        full = self._state(params, 32)
+        ps = _tensors(params)
+        full._allocate(ps[0].device, zero=True)
+        for flat, given in ((full.mu_flat, mu), (full.nu_flat, nu)):
+            given = _tensors(given, full.keys)
+            if [x.numel() for x in given] != full.counts:
+                raise ValueError("AdamW.restore: the moments are not those of the parameters")
+            for o, n, x in zip(full.offsets, full.counts, given):
+                flat[o:o + n].copy_(x.detach().reshape(-1))
+        full.count, full.powers = int(count), self._powers(int(count), ps[0].device)
+        state = full if self.moment_bits == 32 else full.convert(8)
+        self._masters(state, ps, master)
+        return state
+
+    def load_state_dict(self, params, d: dict) -> AdamWState:
+        """The state of a checkpoint (``AdamWState.state_dict``) for these parameters."""
+        state = self._state(params, int(d["bits"]))
+        dev = _tensors(params)[0].device
+        if [tuple(s) for s in d["shapes"]] != state.shapes:
+            raise ValueError("AdamW.load_state_dict: the checkpoint is of other tensors")
+        state._allocate(dev, zero=True)
+        for name in ("mu_flat", "nu_flat", "fields"):
+            if getattr(state, name) is not None:
+                getattr(state, name).copy_(d[name])
+        state.count, state.powers = int(d["count"]), d["powers"].to(device=dev, dtype=torch.float64, copy=True)
+        if d["master_flat"] is not None:
+            state.master_flat = d["master_flat"].to(device=dev, dtype=torch.float32, copy=True)
+        return state
+
+    def lr_at(self, lr: LearningRate, count: int) -> float:
+        return float(lr(count)) if callable(lr) else float(lr)
+
+    def step(self, params, grads, state: AdamWState, active_mask=None, grad_scale=None) -> AdamWState:
+        """Update the parameters, the moments and the count in place; returns the state.
+
+        ``grad_scale`` (one float32 on the device, or a number) multiplies the gradients; when it
+        is not finite nothing changes.  Rows whose ``active_mask`` entry is False keep their
+        parameters and take a zero gradient, whatever theirs holds."""
+        ps = _tensors(params, state.keys)
+        gs = _tensors(grads, state.keys)
+        k = len(ps)
+        if [tuple(p.shape) for p in ps] != state.shapes:
+            raise ValueError("AdamW: the parameters are not those of the state")
+        if len(gs) != k:
+            raise ValueError(f"AdamW: {len(gs)} gradients for {k} tensors")
+        dev = state.mu_flat.device
+        for i, (p, g) in enumerate(zip(ps, gs)):
+            if not p.is_contiguous() or p.device != dev:
+                raise ValueError(f"AdamW: parameter {i} must be a contiguous tensor on {dev}")
+            if g is not None:
+                if g.shape != p.shape or g.device != dev:
+                    raise ValueError(f"AdamW: gradient {i} must be shaped like its parameter on {dev}")
+                if not g.is_contiguous():
+                    gs[i] = g.contiguous()
+        at = [p.data_ptr() for p in ps]
+        if len(set(at)) < k and len({a for a, n in zip(at, state.counts) if n}) < sum(n > 0 for n in state.counts):
+            raise ValueError("AdamW: a parameter is given twice")
+        scale = _scalar(grad_scale, dev, "AdamW")
+        if self.max_grad_norm is not None:
+            state.norms = grad_norms(gs, self.max_grad_norm, active_mask, scale)
+            scale = state.norms.scale
+        act, rows, lens = None, 0, None
+        if active_mask is not None:
+            act, rows, lens = _mask(active_mask, ps, dev, "AdamW")
+        P, I, D = ctypes.c_void_p * k, ctypes.c_int * k, ctypes.c_double * k
+        rates = [self.lr_at(x, state.count) for x in self._each(self.lrs, state, "the learning rate")]
+        nxt = torch.empty_like(state.powers)
+        key = (self.seed * 0x85EBCA6B + (state.count + 1) * 0xC2B2AE3D + 0x27D4EB2F) & _MASK32
+        _lib.call("gs_adamw_step", _lib.stream_handle(dev), k, P(*at), I(*_types(ps, "AdamW")),
+                  P(*[0 if g is None else g.data_ptr() for g in gs]),
+                  I(*_types([p if g is None else g for p, g in zip(ps, gs)], "AdamW")), state._offsets, state._counts,
+                  lens, D(*rates), D(*[float(x) for x in self._each(self.decay, state, "weight_decay")]), state.bits,
+                  state.size, _lib.ptr(state.mu_flat), _lib.ptr(state.nu_flat), _lib.ptr(state.fields),
+                  _lib.ptr(state.master_flat), _lib.ptr(act), rows, _lib.ptr(scale), _lib.ptr(state.powers),
+                  _lib.ptr(nxt), self.b1, self.b2, self.eps, key)
+        state.powers = nxt
+        state.count += 1
+        return state
+
+
+def make_adamw(extent: float, num_iterations: int, **options) -> AdamW:
+    """AdamW with the trainer's learning rates (``make_optimizer``) for the five Gaussian arrays."""
+    return AdamW(dict(make_optimizer(extent, num_iterations).lrs), **options)

@@ -12,19 +12,20 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
-from typing import Optional
+from typing import Optional, Union
 
 import torch
 
 from .. import _lib
 from ..core.gaussians import Gaussians
+from .adamw import AdamW, AdamWState
 from .optimizer import FIELDS, Adam, AdamState
 
 
 @dataclass
 class DensityState:
     gaussians: Gaussians
-    opt_state: Optional[AdamState]
+    opt_state: Union[AdamState, AdamWState, None]
     active_mask: torch.Tensor  # uint8 [M] (0/1)
     num_active: int
     grad_accum: torch.Tensor   # float32 [M]
@@ -32,7 +33,7 @@ class DensityState:
     max_radii: torch.Tensor    # float32 [M]
 
 
-def init_density_state(gaussians: Gaussians, optimizer: Optional[Adam], max_gaussians: int) -> DensityState:
+def init_density_state(gaussians: Gaussians, optimizer: Union[Adam, AdamW, None], max_gaussians: int) -> DensityState:
     """density.py:19-61: pad every array to max_gaussians (padded quaternions are
     (1, 0, 0, 0)), the first N active, zero statistics, the optimizer initialised on the
     padded arrays."""
@@ -74,8 +75,13 @@ def densify_and_prune(state: DensityState, generator: Optional[torch.Generator] 
     if tuple(noise.shape) != (M, 3):
         raise ValueError(f"densify_and_prune: noise must be [{M}, 3]")
     moments = []
-    if state.opt_state is not None:
-        moments = [state.opt_state.mu[f] for f in FIELDS] + [state.opt_state.nu[f] for f in FIELDS]
+    opt = state.opt_state
+    if opt is not None:
+        # 8-bit moments are moved in 32 bits: what they stand for comes back unchanged, but where a
+        # row that moved in has raised the exponent of its block
+        wide = opt.convert(32) if getattr(opt, "bits", 32) == 8 else opt
+        mu, nu = wide.mu, wide.nu
+        moments = [mu[f] for f in FIELDS] + [nu[f] for f in FIELDS]
     for t in [getattr(g, f) for f in FIELDS] + moments:
         if t.dtype != torch.float32 or not t.is_contiguous() or t.shape[0] != M:
             raise ValueError("densify_and_prune: every array must be contiguous float32 with the capacity rows")
@@ -89,6 +95,8 @@ def densify_and_prune(state: DensityState, generator: Optional[torch.Generator] 
               len(moments), mptr, _lib.ptr(state.active_mask), _lib.ptr(state.grad_accum), _lib.ptr(state.denom),
               _lib.ptr(state.max_radii), _lib.ptr(noise), int(bool(densify_enabled)), float(grad_threshold),
               float(min_opacity), float(extent), float(max_screen_size), _lib.ptr(ws), nbytes, _lib.ptr(counts))
+    if opt is not None and wide is not opt:
+        opt.set_moments(wide)
     state.last_counts = counts
     return state
 

@@ -18,6 +18,7 @@ from .. import _lib
 from ..core.camera import Camera
 from ..core.gaussians import Gaussians
 from ..renderer._buffers import as_bytes
+from .adamw import AdamW
 
 
 def accumulate_from_extras(state: dict, grad_means: torch.Tensor, means: torch.Tensor, camera, extras: dict,
@@ -63,13 +64,15 @@ def train_step(state, target_image, w2c, camera_static, optimizer, fast_tpu_rast
     fused=True runs the step without autograd: forward kernels, the loss pair, the
     rasterizer's VJP, then one kernel for the preprocessing VJP, the statistics and the
     Adam update (no parameter gradient reaches memory).  fused=False builds the same
-    step from ``render``'s autograd, ``accumulate_from_extras`` and ``Adam.step``."""
+    step from ``render``'s autograd, ``accumulate_from_extras`` and ``Adam.step``.  An
+    ``AdamW`` optimizer needs the gradients whole (their norm comes before the update) and
+    always takes that form; metrics["grad_norm"] is the norm it clipped."""
     W, H, fx, fy, cx, cy = camera_static
     params = state.gaussians
     dev = params.means.device
     camera = Camera(int(W), int(H), float(fx), float(fy), float(cx), float(cy),
                     torch.as_tensor(w2c, dtype=torch.float32, device=dev), None)
-    if not fused:
+    if not fused or isinstance(optimizer, AdamW):
         return _train_step_autograd(state, target_image, camera, optimizer, fast_tpu_rasterizer, sh_degree)
     return _train_step_fused(state, target_image, camera, optimizer, sh_degree, fast_tpu_rasterizer)
 
@@ -92,6 +95,8 @@ def _train_step_autograd(state, target_image, camera, optimizer, fast_tpu_raster
     accumulate_from_extras({"grad_accum": state.grad_accum, "denom": state.denom, "max_radii": state.max_radii},
                            grads.means, params.means, camera, extras, active=state.active_mask)
     optimizer.step(params, grads, state.opt_state, state.active_mask)
+    if getattr(state.opt_state, "norms", None) is not None:
+        metrics["grad_norm"] = state.opt_state.norms.total
     return state, total.detach(), metrics
 
 
