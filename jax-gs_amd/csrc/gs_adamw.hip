@@ -14,6 +14,7 @@
 // A workgroup takes 1024 consecutive elements of one tensor, a wave one block, a lane four
 // elements.  The tensor is found by one comparison per lane and a ballot.
 #include "gs_moments.h"
+#include "gs_rows.h"
 
 namespace gs {
 namespace {
@@ -26,7 +27,7 @@ struct StepTensor {
   const void* grad;
   int64_t at;          // first element in the state
   int64_t count;
-  uint64_t row_magic;  // floor(2^64 / row_len) + 1 (0: row_len 1)
+  uint64_t row_magic;
   int32_t row_len;
   float lr, decay;
   int32_t kind;        // parameter type * 6 + gradient type * 2 + master
@@ -49,11 +50,12 @@ struct StepArgs {
 };
 static_assert(sizeof(StepArgs) <= 4096, "kernel arguments");
 
+// Four consecutive elements of a lane; `whole`: all of the wave's 256 exist, else the first n.
 template <class T>
-__device__ inline void load4(const T* p, int n, float (&x)[4]) {
+__device__ inline void load4(const T* p, bool whole, int n, float (&x)[4]) {
   // the vector is only as aligned as its element: a tensor may begin anywhere
   typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-  if (n >= 4) {
+  if (whole) {
     const vec v = *reinterpret_cast<const vec*>(p);
 #pragma unroll
     for (int j = 0; j < 4; ++j) x[j] = (float)v[j];
@@ -63,9 +65,9 @@ __device__ inline void load4(const T* p, int n, float (&x)[4]) {
   }
 }
 template <class T>
-__device__ inline void store4(T* p, int n, const float (&x)[4]) {
+__device__ inline void store4(T* p, bool whole, int n, const float (&x)[4]) {
   typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-  if (n >= 4) {
+  if (whole) {
     vec v;
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = (T)x[j];
@@ -77,90 +79,75 @@ __device__ inline void store4(T* p, int n, const float (&x)[4]) {
   }
 }
 
-// Mask of four consecutive elements from `tid` * 4 within the workgroup's chunk.
-__device__ inline void rows_on(const StepArgs& A, const StepTensor& t, int64_t base, int n, bool (&on)[4]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) on[j] = true;
-  if (A.active == nullptr) return;
-  // row of the chunk's first element by a 64-bit reciprocal (exact for base * row_len < 2^64),
-  // of the lane's by a 32-bit one: rem + 1024 elements hold few rows
-  const uint64_t row0 = t.row_magic ? __umul64hi((uint64_t)base, t.row_magic) : (uint64_t)base;
-  const uint32_t L = (uint32_t)t.row_len;
-  uint32_t e = (uint32_t)((uint64_t)base - row0 * L) + threadIdx.x * 4u;
-  uint32_t q;
-  if (L > 4096u) {
-    q = e >= L ? 1u : 0u;
-  } else {
-    q = t.row_magic ? __umulhi(e, (uint32_t)(t.row_magic >> 32) + 1u) : e;
-  }
-  e -= q * L;
-  const uint8_t* a = A.active + row0 + q;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (j < n) on[j] = *a != 0;
-    if (++e == L) {
-      e = 0;
-      ++a;
-    }
-  }
-}
-
-template <bool k8, class P, class G, bool kMaster>
-__device__ inline void step_chunk(const StepArgs& A, const StepTensor& t, int64_t base, float scale, float r1,
+template <bool k8, bool kMask, class P, class G, bool kMaster>
+__device__ inline void step_chunk(const StepArgs& A, const StepTensor& t, int64_t chunk, float scale, float r1,
                                   float r2) {
-  const int64_t e = base + (int64_t)threadIdx.x * 4;
-  if (base + (int64_t)(threadIdx.x & ~63u) * 4 >= t.count) return;  // the wave's block is past the end
-  const int64_t left = t.count - e;
-  const int n = left >= 4 ? 4 : left > 0 ? (int)left : 0;
-  const int64_t at = t.at + e;
-  float w[4], g[4], m[4], r[4], v[4];
-  load4((const G*)t.grad + e, n, g);
-  if (kMaster) load4(A.master + at, 4, w);
-  else load4((const P*)t.param + e, n, w);
-  const int64_t block = at >> 8;
+  const uint32_t l4 = (threadIdx.x & 63u) * 4u;
+  const int64_t base = chunk + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) * kMomBlock;
+  const int64_t left = t.count - base;
+  if (left <= 0) return;  // the wave's block is past the end
+  const bool whole = left >= kMomBlock;
+  const int n = whole ? 4 : min(max((int)left - (int)l4, 0), 4);
+  const int64_t at = t.at + base;
+  G* const grad = (G*)t.grad + base;
+  P* const param = (P*)t.param + base;
+  float* const master = A.master + at;
+  float w[4] = {0.0f, 0.0f, 0.0f, 0.0f}, g[4] = {0.0f, 0.0f, 0.0f, 0.0f}, m[4], r[4], v[4];
+  uint32_t m8 = 0, r8 = 0, f = 0;
   if (k8) {
-    const uint32_t m8 = *(const uint32_t*)((const uint8_t*)A.mu + at);
-    const uint32_t r8 = *(const uint32_t*)((const uint8_t*)A.nu + at);
-    const uint32_t f = *(const uint16_t*)(A.fields + 2 * block);
+    m8 = *(const uint32_t*)((const uint8_t*)A.mu + at + l4);
+    r8 = *(const uint32_t*)((const uint8_t*)A.nu + at + l4);
+    f = *(const uint16_t*)(A.fields + (at >> 7));
+  } else {
+    load4((const float*)A.mu + at + l4, true, 4, m);
+    load4((const float*)A.nu + at + l4, true, 4, v);
+  }
+  // masked rows: neither gradient nor parameter is read or written
+  const uint32_t on = kMask ? rows_on<4>(A.active, t.row_magic, (uint32_t)t.row_len, base, l4, n) : 15u;
+  if (!kMask || on) {
+    load4(grad + l4, whole, n, g);
+    if (kMaster) load4(master + l4, whole, n, w);
+    else load4(param + l4, whole, n, w);
+  }
+  if (k8) {
     decode_m4(m8, (int)(f & 255u), m);
     decode_r4(r8, (int)(f >> 8), r);
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = r[j] * r[j];
-  } else {
-    load4((const float*)A.mu + at, 4, m);
-    load4((const float*)A.nu + at, 4, v);
   }
-  bool on[4];
-  rows_on(A, t, base, n, on);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float x = on[j] ? g[j] * scale : 0.0f;
+    const float x = !kMask || (on >> j & 1u) ? g[j] * scale : 0.0f;
     m[j] = m[j] * A.b1 + x * A.omb1;
     v[j] = v[j] * A.b2 + (x * x) * A.omb2;
-    r[j] = sqrtf(v[j]);
-    const float u = (m[j] * r1) / (r[j] * r2 + A.eps);
-    const float y = w[j] - t.lr * (u + t.decay * w[j]);
-    w[j] = on[j] ? y : w[j];
   }
-  if (n > 0) {
-    store4((P*)t.param + e, n, w);
-    if (kMaster) store4(A.master + at, n, w);
+  roots4(v, r);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    // the divisor's reciprocal to within one step: 2^-23 of a step of the weight
+    const float u = (m[j] * r1) * __builtin_amdgcn_rcpf(r[j] * r2 + A.eps);
+    const float y = w[j] - t.lr * (u + t.decay * w[j]);
+    w[j] = !kMask || (on >> j & 1u) ? y : w[j];
+  }
+  if (!kMask || on) {
+    store4(param + l4, whole, n, w);
+    if (kMaster) store4(master + l4, whole, n, w);
   }
   if (k8) {
-    uint32_t h[4], m8, r8, f;
+    uint32_t h[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) h[j] = place_hash(at + j, A.key);
+    for (int j = 0; j < 4; ++j) h[j] = place_hash(at, l4 + j, A.key);
     encode_block<true>(m, r, h, m8, r8, f);
-    *(uint32_t*)((uint8_t*)A.mu + at) = m8;
-    *(uint32_t*)((uint8_t*)A.nu + at) = r8;
-    if ((threadIdx.x & 63u) == 0) *(uint16_t*)(A.fields + 2 * block) = (uint16_t)f;
+    *(uint32_t*)((uint8_t*)A.mu + at + l4) = m8;
+    *(uint32_t*)((uint8_t*)A.nu + at + l4) = r8;
+    if (l4 == 0) *(uint16_t*)(A.fields + (at >> 7)) = (uint16_t)f;
   } else {
-    store4((float*)A.mu + at, 4, m);
-    store4((float*)A.nu + at, 4, v);
+    store4((float*)A.mu + at + l4, true, 4, m);
+    store4((float*)A.nu + at + l4, true, 4, v);
   }
 }
 
-template <bool k8>
+template <bool k8, bool kMask>
 __global__ __launch_bounds__(256) void adamw_kernel(StepArgs A) {
   const float scale = A.scale ? *A.scale : 1.0f;
   const bool ok = fabsf(scale) < __builtin_huge_valf();
@@ -180,12 +167,12 @@ __global__ __launch_bounds__(256) void adamw_kernel(StepArgs A) {
   const int k = __popcll(__ballot(b >= A.begin[threadIdx.x & 63u])) - 1;
   if (k < 0) return;
   const StepTensor t = A.t[k];
-  const int64_t base = (int64_t)(b - A.begin[k]) * kStepChunk;
+  const int64_t chunk = (int64_t)(b - A.begin[k]) * kStepChunk;
   const float r1 = (float)A.powers[2], r2 = (float)A.powers[3];
   switch (t.kind) {
-#define GS_STEP(i, P, G, M)                                \
-  case i:                                                  \
-    step_chunk<k8, P, G, M>(A, t, base, scale, r1, r2);    \
+#define GS_STEP(i, P, G, M)                                       \
+  case i:                                                         \
+    step_chunk<k8, kMask, P, G, M>(A, t, chunk, scale, r1, r2);   \
     break;
     GS_STEP(0, float, float, false)
     GS_STEP(2, float, __bf16, false)
@@ -212,11 +199,10 @@ __global__ __launch_bounds__(256) void moments_encode_kernel(int64_t blocks, con
   const int64_t block = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (block >= blocks) return;
   const int64_t at = block * kMomBlock + (threadIdx.x & 63u) * 4;
-  float m[4], r[4];
-  load4(mu + at, 4, m);
-  load4(nu + at, 4, r);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) r[j] = sqrtf(r[j]);
+  float m[4], r[4], v[4];
+  load4(mu + at, true, 4, m);
+  load4(nu + at, true, 4, v);
+  roots4(v, r);
   const uint32_t none[4] = {0, 0, 0, 0};
   uint32_t cm, cr, f;
   encode_block<false>(m, r, none, cm, cr, f);
@@ -238,8 +224,8 @@ __global__ __launch_bounds__(256) void moments_decode_kernel(int64_t blocks, con
   decode_r4(*(const uint32_t*)(r8 + at), (int)(f >> 8), r);
 #pragma unroll
   for (int j = 0; j < 4; ++j) r[j] = r[j] * r[j];
-  store4(mu + at, 4, m);
-  store4(nu + at, 4, r);
+  store4(mu + at, true, 4, m);
+  store4(nu + at, true, 4, r);
 }
 
 bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
@@ -285,7 +271,7 @@ extern "C" int gs_adamw_step(void* stream, int num, void* const* params, const i
                    counts[i] <= state_size - offsets[i],
                "gs_adamw_step: tensor %d lies outside the state", i);
     if (active)
-      GS_REQUIRE(row_lens[i] >= 1 && row_lens[i] < ((int64_t)1 << 24) && rows >= 0 &&
+      GS_REQUIRE(row_lens[i] >= 1 && row_lens[i] < kMaxRowLen && rows >= 0 &&
                      counts[i] % row_lens[i] == 0 && counts[i] / row_lens[i] == rows,
                  "gs_adamw_step: tensor %d has %lld elements, not rows x row length", i, (long long)counts[i]);
   }
@@ -322,7 +308,7 @@ extern "C" int gs_adamw_step(void* stream, int num, void* const* params, const i
       t.at = offsets[i];
       t.count = counts[i];
       t.row_len = active ? (int32_t)row_lens[i] : 1;
-      t.row_magic = t.row_len > 1 ? ~(uint64_t)0 / (uint64_t)t.row_len + 1 : 0;
+      t.row_magic = row_magic(t.row_len);
       t.lr = (float)lrs[i];
       t.decay = (float)decays[i];
       t.kind = param_types[i] * 6 + grad_types[i] * 2 + (param_types[i] != GS_TYPE_F32 && master ? 1 : 0);
@@ -331,8 +317,9 @@ extern "C" int gs_adamw_step(void* stream, int num, void* const* params, const i
     }
     for (; k < 64; ++k) A.begin[k] = 0xffffffffu;
     const dim3 grid((unsigned)(groups > 0 ? groups : 1));
-    if (moment_bits == 8) hipLaunchKernelGGL(adamw_kernel<true>, grid, dim3(256), 0, s, A);
-    else hipLaunchKernelGGL(adamw_kernel<false>, grid, dim3(256), 0, s, A);
+    auto* kernel = moment_bits == 8 ? (active ? adamw_kernel<true, true> : adamw_kernel<true, false>)
+                                    : (active ? adamw_kernel<false, true> : adamw_kernel<false, false>);
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, A);
     GS_LAUNCH_CHECK("adamw_kernel");
     A.powers_next = nullptr;
     while (i < num && (!grads[i] || counts[i] == 0)) ++i;

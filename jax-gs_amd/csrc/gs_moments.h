@@ -28,12 +28,16 @@ constexpr int kMomBlock = 256;  // elements per block: one wave, four elements a
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
-// Maximum over the wave, in every lane (unsigned order is that of non-negative floats).
-__device__ inline uint32_t wave_max_u32(uint32_t x) {
-#define GS_DPP_MAX(ctrl)                                                                            \
-  {                                                                                                 \
-    const uint32_t y = (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, ctrl, 0xf, 0xf, false); \
-    x = x > y ? x : y;                                                                              \
+// Maxima of x and of y over the wave, in every lane (unsigned order is that of non-negative
+// floats).  A lane without a source reads 0, so that each step is one instruction; the two
+// chains fill each other's wait states.
+__device__ inline void wave_max2_u32(uint32_t& x, uint32_t& y) {
+#define GS_DPP_MAX(ctrl)                                                                          \
+  {                                                                                               \
+    const uint32_t a = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, 0xf, 0xf, true);    \
+    const uint32_t b = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)y, ctrl, 0xf, 0xf, true);    \
+    x = x > a ? x : a;                                                                            \
+    y = y > b ? y : b;                                                                            \
   }
   GS_DPP_MAX(0xB1);   // quad_perm [1, 0, 3, 2]
   GS_DPP_MAX(0x4E);   // quad_perm [2, 3, 0, 1]
@@ -42,7 +46,8 @@ __device__ inline uint32_t wave_max_u32(uint32_t x) {
   GS_DPP_MAX(0x142);  // row_bcast15: rows 1 and 3 hold pairs of rows
   GS_DPP_MAX(0x143);  // row_bcast31: row 3 holds all
 #undef GS_DPP_MAX
-  return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+  x = (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+  y = (uint32_t)__builtin_amdgcn_readlane((int)y, 63);
 }
 
 // Exponent field of a block whose largest finite magnitude has the given bits.
@@ -52,44 +57,84 @@ __device__ inline uint32_t moment_field(uint32_t most) {
   return f < 254u ? f : 254u;
 }
 
-// The code's magnitude of a finite value x >= 0; `low` is what is added below the code's
-// bits: a random number of 23 - kMant bits, or kNearest for round to nearest even.
+// A finite value x >= 0 scaled so that its code is the top of the bits (from bit 23 - kMant on),
+// with what rounds it added: a random number of 23 - kMant bits, or kNearest for round to nearest
+// even.  A root (kMant 4) above zero gets at least code 1; its bits are at least those of the
+// least normal float, as the root of any float32 is.
 constexpr uint32_t kNearest = 0xffffffffu;
 template <int kMant>
-__device__ inline uint32_t moment_code(float x, int field, uint32_t low) {
+__device__ inline uint32_t moment_bits(uint32_t x, int field, uint32_t low) {
   constexpr int drop = 23 - kMant;
-  constexpr uint32_t top = (16u << kMant) - 2u;
-  const uint32_t b = float_to_bits(ldexpf(x, 15 - field));
+  uint32_t b = float_to_bits(ldexpf(bits_to_float(x), 15 - field));
   if (low == kNearest) low = (1u << (drop - 1)) - 1u + ((b >> drop) & 1u);
-  uint32_t c = (b + low) >> drop;
-  if (kMant == 4) c = c > 0 || x == 0.0f ? c : 1u;
-  return c < top ? c : top;
+  b += low;
+  if (kMant == 4) {
+    const uint32_t least = x < (1u << drop) ? x : 1u << drop;
+    b = b > least ? b : least;
+  }
+  return b;
 }
 
-// Four decoded values of the packed codes w of one lane; field as stored.
+// Four decoded values of the packed codes w of one lane; field as stored.  The signed code is the
+// machine's own 8-bit float (bias 7, the same "not finite" code).
 __device__ inline void decode_m4(uint32_t w, int field, float (&m)[4]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    m[j] = ldexpf(bits_to_float((uint32_t)((int32_t)(w << (24 - 8 * j)) >> 4) & 0x87f00000u), field - 15);
-  if (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (((w >> (8 * j)) & 127u) == 127u) m[j] = bits_to_float(0x7fc00000u);
-  }
+  const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+  m[0] = ldexpf(a[0], field - 135);
+  m[1] = ldexpf(a[1], field - 135);
+  m[2] = ldexpf(b[0], field - 135);
+  m[3] = ldexpf(b[1], field - 135);
 }
 __device__ inline void decode_r4(uint32_t w, int field, float (&r)[4]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) r[j] = ldexpf(bits_to_float(((w >> (8 * j)) & 255u) << 19), field - 15);
-  if ((~w - 0x01010101u) & w & 0x80808080u) {
+  constexpr uint32_t mask = 255u << 19;
+  r[0] = ldexpf(bits_to_float((w << 19) & mask), field - 15);
+  r[1] = ldexpf(bits_to_float((w << 11) & mask), field - 15);
+  r[2] = ldexpf(bits_to_float((w << 3) & mask), field - 15);
+  r[3] = ldexpf(bits_to_float((w >> 5) & mask), field - 15);
+  if ((~w - 0x01010101u) & w & 0x80808080u) {  // some code is 255
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (((w >> (8 * j)) & 255u) == 255u) r[j] = bits_to_float(0x7fc00000u);
   }
 }
 
+// The top bytes of four words.
+__device__ inline uint32_t pack_top(const uint32_t (&x)[4]) {
+  const uint32_t lo = __builtin_amdgcn_perm(x[1], x[0], 0x0c0c0703u), hi = __builtin_amdgcn_perm(x[3], x[2], 0x0c0c0703u);
+  return (hi << 16) | lo;
+}
+
+// encode_block where the block holds values that are not finite or the largest exponents.
+template <bool kStochastic>
+__device__ inline void encode_block_odd(const float (&m)[4], const float (&r)[4], const uint32_t (&h)[4],
+                                        uint32_t& m8, uint32_t& r8, uint32_t& fields) {
+  constexpr uint32_t kInf = 0x7f800000u;
+  uint32_t mb[4], rb[4], mm = 0, rr = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    mb[j] = float_to_bits(m[j]) & 0x7fffffffu;
+    rb[j] = float_to_bits(r[j]) & 0x7fffffffu;
+    if (mb[j] < kInf && mb[j] > mm) mm = mb[j];
+    if (rb[j] < kInf && rb[j] > rr) rr = rb[j];
+  }
+  wave_max2_u32(mm, rr);
+  const uint32_t fm = moment_field<3>(mm), fr = moment_field<4>(rr);
+  fields = fm | (fr << 8);
+  m8 = r8 = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t cm = moment_bits<3>(mb[j], (int)fm, kStochastic ? (h[j] >> 16) << 4 : kNearest) >> 20;
+    uint32_t cr = moment_bits<4>(rb[j], (int)fr, kStochastic ? (h[j] & 0xffffu) << 3 : kNearest) >> 19;
+    cm = mb[j] >= kInf ? 127u : cm < 126u ? cm : 126u;
+    cr = rb[j] >= kInf ? 255u : cr < 254u ? cr : 254u;
+    cm |= (float_to_bits(m[j]) >> 24) & 128u;
+    m8 |= cm << (8 * j);
+    r8 |= cr << (8 * j);
+  }
+}
+
 // Codes and exponent fields of one block, four values a lane (the whole wave calls).
-// h: 32 random bits per value (the upper half rounds m, the lower half r), or NULL for
-// round to nearest even.
+// h: 32 random bits per value (the upper half rounds m, the lower half r), unused for round to
+// nearest even.
 template <bool kStochastic>
 __device__ inline void encode_block(const float (&m)[4], const float (&r)[4], const uint32_t (&h)[4], uint32_t& m8,
                                     uint32_t& r8, uint32_t& fields) {
@@ -97,45 +142,57 @@ __device__ inline void encode_block(const float (&m)[4], const float (&r)[4], co
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     mb[j] = float_to_bits(m[j]) & 0x7fffffffu;
-    rb[j] = float_to_bits(r[j]) & 0x7fffffffu;
+    rb[j] = float_to_bits(r[j]);
     mm = mm > mb[j] ? mm : mb[j];
     rr = rr > rb[j] ? rr : rb[j];
   }
-  constexpr uint32_t kInf = 0x7f800000u;
-  uint32_t wm = wave_max_u32(mm), wr = wave_max_u32(rr);
-  const bool odd = wm >= kInf || wr >= kInf;  // uniform: something here is not finite
-  if (odd) {
-    mm = rr = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (mb[j] < kInf && mb[j] > mm) mm = mb[j];
-      if (rb[j] < kInf && rb[j] > rr) rr = rb[j];
-    }
-    wm = wave_max_u32(mm);
-    wr = wave_max_u32(rr);
+  wave_max2_u32(mm, rr);
+  // from 2^126 on (not finite, or a field that would pass 254): rare, and the same for the wave
+  if (mm >= 0x7e800000u || rr >= 0x7e800000u) {
+    encode_block_odd<kStochastic>(m, r, h, m8, r8, fields);
+    return;
   }
-  const uint32_t fm = moment_field<3>(wm), fr = moment_field<4>(wr);
+  const uint32_t fm = moment_field<3>(mm), fr = moment_field<4>(rr);
   fields = fm | (fr << 8);
-  m8 = r8 = 0;
+  uint32_t cm[4], cr[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    uint32_t cm = moment_code<3>(bits_to_float(mb[j]), (int)fm, kStochastic ? (h[j] >> 16) << 4 : kNearest);
-    uint32_t cr = moment_code<4>(bits_to_float(rb[j]), (int)fr, kStochastic ? (h[j] & 0xffffu) << 3 : kNearest);
-    if (odd) {
-      if (mb[j] >= kInf) cm = 127u;
-      if (rb[j] >= kInf) cr = 255u;
-    }
-    cm |= (float_to_bits(m[j]) >> 24) & 128u;
-    m8 |= cm << (8 * j);
-    r8 |= cr << (8 * j);
+    cm[j] = moment_bits<3>(mb[j], (int)fm, kStochastic ? (h[j] >> 16) << 4 : kNearest) << 4;
+    cm[j] |= float_to_bits(m[j]) & 0x80000000u;
+    cr[j] = moment_bits<4>(rb[j], (int)fr, kStochastic ? (h[j] & 0xffffu) << 3 : kNearest) << 5;
+  }
+  m8 = pack_top(cm);
+  r8 = pack_top(cr);
+}
+
+// Correctly rounded roots of four values v >= 0.  The hardware's reciprocal root and one
+// correction from the exact residual give the rounded root of every float from 2^-100 on (all
+// 1.9e9 of them compared with the compiler's sequence); a lane with smaller ones, whose residual
+// would underflow, or with one that is not finite takes that sequence.
+__device__ inline void roots4(const float (&v)[4], float (&r)[4]) {
+  constexpr float kLeast = 7.888609052210118e-31f;  // 2^-100
+  bool odd = false;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float up = fmaxf(v[j], kLeast);
+    const float y = __builtin_amdgcn_rsqf(up);
+    const float s = v[j] * y;
+    r[j] = fmaf(fmaf(-s, s, v[j]), 0.5f * y, s);
+    // between 0 and 2^-100, infinite or not a number
+    odd |= float_to_bits(v[j]) - 1u < float_to_bits(kLeast) - 1u || float_to_bits(v[j]) >= 0x7f800000u;
+  }
+  if (odd) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = sqrtf(v[j]);
   }
 }
 
 // 32 hashed bits of an element's place in the state: a Weyl step, one multiplication by an
-// odd constant between two shifts.  key holds the seed and the step.
-__device__ inline uint32_t place_hash(int64_t place, uint32_t key) {
-  const uint32_t x = (uint32_t)place + (uint32_t)((uint64_t)place >> 32) * 0x632be5abu;
-  uint32_t h = x * 0x9e3779b1u + key;
+// odd constant between two shifts.  key holds the seed and the step.  The element is block + j
+// with block a multiple of 256 that is the same for the wave and j < 256.
+__device__ inline uint32_t place_hash(int64_t block, uint32_t j, uint32_t key) {
+  const uint32_t x = (uint32_t)block + (uint32_t)((uint64_t)block >> 32) * 0x632be5abu;
+  uint32_t h = j * 0x9e3779b1u + (x * 0x9e3779b1u + key);
   h ^= h >> 15;
   h *= 0xd1b54a35u;
   return h ^ (h >> 13);

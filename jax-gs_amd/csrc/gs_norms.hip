@@ -9,30 +9,25 @@
 // Every workgroup sums one run of consecutive elements of one tensor (the runs' length is chosen
 // so that about 2048 of them cover all tensors) into one partial sum; a second launch of one
 // workgroup adds the partial sums of each tensor and the tensors' sums.
-#include "gs_common.h"
+#include "gs_rows.h"
 
 #include <algorithm>
 
 namespace gs {
 namespace {
 
-constexpr int kNormTensors = 64;  // per launch
-constexpr int kNormRuns = 2048;   // 8 workgroups of 4 waves on each of 256 CUs
-
-struct NormTensor {
-  const void* grad;
-  int64_t count;
-  uint64_t row_magic;  // floor(2^64 / row_len) + 1 (0: row_len 1)
-  int32_t row_len;
-  int32_t type;
-};
+constexpr int kNormTensors = 152;  // per launch: the argument block stays below 4 KiB
+constexpr int kNormRuns = 2048;    // 8 workgroups of 4 waves on each of 256 CUs
 
 struct NormArgs {
-  NormTensor t[kNormTensors];
-  uint32_t begin[64];  // first workgroup of each tensor, ~0 after the last
+  const void* grad[kNormTensors];
+  int64_t count[kNormTensors];
+  uint32_t begin[kNormTensors];  // first workgroup of each tensor
+  int32_t row_len[kNormTensors];
+  uint8_t type[kNormTensors];
   const uint8_t* active;
-  double* partial;     // of this launch's first workgroup
-  int32_t* first;      // this launch's tensors: their first partial sums
+  double* partial;  // of this launch's first workgroup
+  int32_t* first;   // this launch's tensors: their first partial sums
   int32_t first_partial;
   int32_t n;
   uint32_t groups;
@@ -49,7 +44,7 @@ NormLayout norm_layout(int num, const int64_t* counts) {
   NormLayout L;
   int64_t total = 0;
   for (int i = 0; i < num; ++i) total += counts[i];
-  L.run = std::max<int64_t>(4096, ((total + kNormRuns - 1) / kNormRuns + 2047) / 2048 * 2048);
+  L.run = std::max<int64_t>(8192, ((total + kNormRuns - 1) / kNormRuns + 8191) / 8192 * 8192);
   L.partials = 0;
   for (int i = 0; i < num; ++i) L.partials += (counts[i] + L.run - 1) / L.run;
   L.sums = (size_t)L.partials * sizeof(double);
@@ -65,38 +60,72 @@ __device__ inline double wave_sum(double x) {
 }
 
 template <class G>
-__device__ inline double run_sum(const NormArgs& A, const NormTensor& t, int64_t begin, int64_t end) {
+__device__ inline double run_sum(const G* __restrict__ g, const uint8_t* __restrict__ active, int32_t row_len,
+                                 int64_t begin, int64_t end) {
   constexpr int kVec = 16 / sizeof(G);  // 16 bytes a lane
+  constexpr int kStep = 256 * kVec;
+  constexpr int kAhead = 4;  // vectors in flight
   typedef G vec __attribute__((ext_vector_type(kVec), aligned(sizeof(G))));
-  const G* g = (const G*)t.grad;
   double acc[4] = {0.0, 0.0, 0.0, 0.0};
-  if (A.active == nullptr) {
-    const int64_t step = 256 * kVec;
-    int64_t e = begin + threadIdx.x * kVec;
-    for (; e + 3 * step + kVec <= end; e += 4 * step) {
-      vec v[4];
+  const uint32_t l = threadIdx.x * kVec;
+  // the reciprocal of the row length: a division, but one per workgroup
+  const uint64_t magic = active && row_len > 1 ? ~(uint64_t)0 / (uint32_t)row_len + 1 : 0;
+  int64_t base = begin;
+  uint32_t on[kAhead];
+  if (active && base + kAhead * kStep <= end)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const vec*>(g + e + u * step);
+    for (int u = 0; u < kAhead; ++u) on[u] = rows_on<kVec>(active, magic, row_len, base + u * kStep, l, kVec);
+  for (; base + kAhead * kStep <= end; base += kAhead * kStep) {
+    vec v[kAhead];
+    if (active == nullptr) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < kAhead; ++u) v[u] = *reinterpret_cast<const vec*>(g + base + u * kStep + l);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
 #pragma unroll
         for (int j = 0; j < kVec; ++j) {
           const double x = (double)(float)v[u][j];
           acc[u] = fma(x, x, acc[u]);
         }
-    }
-    for (; e < end; e += step)
-      for (int j = 0; j < kVec; ++j)
-        if (e + j < end) {
-          const double x = (double)(float)g[e + j];
-          acc[0] = fma(x, x, acc[0]);
+    } else {
+      // masked rows are not read; the next masks come while these elements do
+      uint32_t now[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        now[u] = on[u];
+        v[u] = (vec)(G)0.0f;
+        if (now[u]) v[u] = *reinterpret_cast<const vec*>(g + base + u * kStep + l);
+      }
+      if (base + 2 * kAhead * kStep <= end)
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+          on[u] = rows_on<kVec>(active, magic, row_len, base + (kAhead + u) * kStep, l, kVec);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+          const double x = now[u] >> j & 1u ? (double)(float)v[u][j] : 0.0;
+          acc[u] = fma(x, x, acc[u]);
         }
-  } else {
-    for (int64_t e = begin + threadIdx.x; e < end; e += 256) {
-      const uint64_t row = t.row_magic ? __umul64hi((uint64_t)e, t.row_magic) : (uint64_t)e;
-      const float gx = (float)g[e];
-      const double x = A.active[row] ? (double)gx : 0.0;
-      acc[0] = fma(x, x, acc[0]);
+    }
+  }
+  for (; base < end; base += kStep) {
+    const int64_t left = end - base - l;
+    const int n = left >= kVec ? kVec : left > 0 ? (int)left : 0;
+    const uint32_t some = active ? rows_on<kVec>(active, magic, row_len, base, l, n) : (1u << n) - 1u;
+    if (some == 0) continue;
+    vec v = (vec)(G)0.0f;
+    if (n == kVec) {
+      v = *reinterpret_cast<const vec*>(g + base + l);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kVec; ++j)
+        if (j < n) v[j] = g[base + l + j];
+    }
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+      const double x = some >> j & 1u ? (double)(float)v[j] : 0.0;
+      acc[j & 3] = fma(x, x, acc[j & 3]);
     }
   }
   return (acc[0] + acc[1]) + (acc[2] + acc[3]);
@@ -104,42 +133,61 @@ __device__ inline double run_sum(const NormArgs& A, const NormTensor& t, int64_t
 
 __global__ __launch_bounds__(256) void grad_norms_kernel(NormArgs A) {
   const uint32_t b = blockIdx.x;
-  if (b == 0 && threadIdx.x < (uint32_t)A.n)
-    A.first[threadIdx.x] = A.first_partial + (int32_t)A.begin[threadIdx.x];
+  const int lane = threadIdx.x & 63;
+  if (b == 0)
+    for (int k = threadIdx.x; k < A.n; k += 256) A.first[k] = A.first_partial + (int32_t)A.begin[k];
   if (b >= A.groups) return;  // every tensor is empty
-  const int k = __popcll(__ballot(b >= A.begin[threadIdx.x & 63u])) - 1;
-  const NormTensor t = A.t[k];
-  const uint32_t within = b - A.begin[k];
-  const int64_t begin = (int64_t)within * A.run;
-  const int64_t end = begin + A.run < t.count ? begin + A.run : t.count;
+  int k = -1;  // the last tensor that begins at or before this workgroup
+  for (int at = 0; at < A.n; at += 64) k += __popcll(__ballot(at + lane < A.n && b >= A.begin[min(at + lane, A.n - 1)]));
+  k = __builtin_amdgcn_readfirstlane(k);
+  const int64_t begin = (int64_t)(b - A.begin[k]) * A.run, count = A.count[k];
+  const int64_t end = begin + A.run < count ? begin + A.run : count;
+  const int type = A.type[k], row_len = A.row_len[k];
+  const void* g = A.grad[k];
   double x;
-  if (t.type == GS_TYPE_F32) x = run_sum<float>(A, t, begin, end);
-  else if (t.type == GS_TYPE_BF16) x = run_sum<__bf16>(A, t, begin, end);
-  else x = run_sum<_Float16>(A, t, begin, end);
+  if (type == GS_TYPE_F32) x = run_sum((const float*)g, A.active, row_len, begin, end);
+  else if (type == GS_TYPE_BF16) x = run_sum((const __bf16*)g, A.active, row_len, begin, end);
+  else x = run_sum((const _Float16*)g, A.active, row_len, begin, end);
   x = wave_sum(x);
   __shared__ double w[4];
-  if ((threadIdx.x & 63u) == 0) w[threadIdx.x >> 6] = x;
+  if (lane == 0) w[threadIdx.x >> 6] = x;
   __syncthreads();
   if (threadIdx.x == 0) A.partial[b] = (w[0] + w[1]) + (w[2] + w[3]);
 }
 
-// One workgroup: a wave sums a tensor's partial sums, the first wave the tensors'.
-__global__ __launch_bounds__(1024) void grad_norms_total_kernel(int num, int partials, const double* __restrict__ partial,
+// One workgroup: 2^group_log2 threads sum a tensor's partial sums, the first wave the tensors'.
+__global__ __launch_bounds__(1024) void grad_norms_total_kernel(int num, int partials, int group_log2,
+                                                                const double* __restrict__ partial,
                                                                 const int32_t* __restrict__ first, double* sums,
                                                                 const float* __restrict__ grad_scale, double max_norm,
                                                                 float* __restrict__ norms, float* __restrict__ out) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int group = 1 << group_log2, within = threadIdx.x & (group - 1);
   const double s = grad_scale ? fabs((double)*grad_scale) : 1.0;
-  for (int k = wave; k < num; k += 16) {
-    const int b = first[k], e = k + 1 < num ? first[k + 1] : partials;
+  __shared__ double w[16];
+  for (int k0 = 0; k0 < num; k0 += 1024 >> group_log2) {
+    const int k = k0 + (threadIdx.x >> group_log2);
     double acc[4] = {0.0, 0.0, 0.0, 0.0};
-    int i = b + lane;
-    for (; i + 192 < e; i += 256)
+    if (k < num) {
+      const int e = k + 1 < num ? first[k + 1] : partials;
+      for (int i = first[k] + within; i < e; i += 8 * group) {
+        double v[8];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) acc[u] += partial[i + 64 * u];
-    for (; i < e; i += 64) acc[0] += partial[i];
-    const double x = wave_sum((acc[0] + acc[1]) + (acc[2] + acc[3]));
-    if (lane == 0) {
+        for (int u = 0; u < 8; ++u) v[u] = partial[min(i + u * group, e - 1)];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) acc[u & 3] += i + u * group < e ? v[u] : 0.0;
+      }
+    }
+    double x = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+    for (int o = min(group, 64) >> 1; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
+    if (group > 64) {
+      if (lane == 0) w[wave] = x;
+      __syncthreads();
+      x = 0.0;
+      for (int q = 0; q < group >> 6; ++q) x += w[(wave & ~((group >> 6) - 1)) + q];
+      __syncthreads();
+    }
+    if (within == 0 && k < num) {
       sums[k] = x;
       if (norms) norms[k] = (float)(sqrt(x) * s);
     }
@@ -187,7 +235,7 @@ extern "C" int gs_grad_norms(void* stream, int num, const void* const* grads, co
     GS_REQUIRE((reinterpret_cast<uintptr_t>(grads[i]) & (grad_types[i] == GS_TYPE_F32 ? 3 : 1)) == 0,
                "gs_grad_norms: tensor %d is not aligned to its type", i);
     if (active && counts[i])
-      GS_REQUIRE(row_lens[i] >= 1 && row_lens[i] < ((int64_t)1 << 24) && rows >= 0 &&
+      GS_REQUIRE(row_lens[i] >= 1 && row_lens[i] < kMaxRowLen && rows >= 0 &&
                      counts[i] % row_lens[i] == 0 && counts[i] / row_lens[i] == rows,
                  "gs_grad_norms: tensor %d has %lld elements, not rows x row length", i, (long long)counts[i]);
   }
@@ -206,26 +254,26 @@ extern "C" int gs_grad_norms(void* stream, int num, const void* const* grads, co
     int k = 0;
     int64_t groups = 0;
     for (; i < num && k < kNormTensors; ++i) {
-      NormTensor& t = A.t[k];
-      t.grad = grads[i];
-      t.count = counts[i];
-      t.row_len = active && counts[i] ? (int32_t)row_lens[i] : 1;
-      t.row_magic = t.row_len > 1 ? ~(uint64_t)0 / (uint64_t)t.row_len + 1 : 0;
-      t.type = grad_types[i];
+      A.grad[k] = grads[i];
+      A.count[k] = counts[i];
+      A.row_len[k] = active && counts[i] ? (int32_t)row_lens[i] : 1;
+      A.type[k] = (uint8_t)grad_types[i];
       A.begin[k++] = (uint32_t)groups;
       groups += (counts[i] + L.run - 1) / L.run;
     }
     A.n = k;
     A.groups = (uint32_t)groups;
     A.first = (int32_t*)(ws + L.first) + (i - k);
-    for (; k < 64; ++k) A.begin[k] = 0xffffffffu;
     A.partial = (double*)ws + done;
     A.first_partial = (int32_t)done;
     done += groups;
     hipLaunchKernelGGL(grad_norms_kernel, dim3((unsigned)(groups > 0 ? groups : 1)), dim3(256), 0, s, A);
     GS_LAUNCH_CHECK("grad_norms_kernel");
   }
-  hipLaunchKernelGGL(grad_norms_total_kernel, dim3(1), dim3(1024), 0, s, num, (int)L.partials, (const double*)ws,
+  // all threads at once for few tensors; at least eight a tensor, whose loads then wait together
+  int group_log2 = 10;
+  while (group_log2 > 3 && (1024 >> group_log2) < num) --group_log2;
+  hipLaunchKernelGGL(grad_norms_total_kernel, dim3(1), dim3(1024), 0, s, num, (int)L.partials, group_log2, (const double*)ws,
                      (const int32_t*)(ws + L.first), (double*)(ws + L.sums), grad_scale, max_norm, norms, out);
   GS_LAUNCH_CHECK("grad_norms_total_kernel");
   return GS_OK;

@@ -173,6 +173,12 @@ def ptr(t: torch.Tensor | None):
     return ctypes.c_void_p(t.data_ptr())
 
 
+# the current stream's handle without a Stream object around it (2 us a call), where torch has it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_handle(device: torch.device):
     """The current torch stream of `device` as a hipStream_t."""
+    if _raw_stream is not None and device.index is not None:
+        return ctypes.c_void_p(_raw_stream(device.index))
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)

@@ -17,8 +17,9 @@ alone).  The arithmetic is float32; the kernels are ``gs_adamw_step``, ``gs_grad
 """
 from __future__ import annotations
 
-import ctypes
-from typing import Callable, Dict, List, NamedTuple, Optional, Sequence, Union
+from array import array
+from operator import attrgetter
+from typing import Callable, Optional, Union
 
 import torch
 
@@ -31,14 +32,27 @@ LearningRate = Union[float, Callable[[int], float]]
 BLOCK = 256  # elements that share an exponent in 8 bits; each tensor's moments begin at a multiple
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_MASK32 = 0xFFFFFFFF
 
 
-class GradNorms(NamedTuple):
-    """Device float32: the norm of all gradients, each tensor's, and the factor for the step."""
-    total: torch.Tensor
-    per_tensor: torch.Tensor
-    scale: torch.Tensor
+class GradNorms:
+    """Device float32: ``total``, the norm of all gradients; ``per_tensor``, each one's; ``scale``,
+    the factor for the step."""
+    __slots__ = ("_out",)
+
+    def __init__(self, out: torch.Tensor):
+        self._out = out  # total, scale, one per tensor
+
+    @property
+    def total(self) -> torch.Tensor:
+        return self._out[0]
+
+    @property
+    def scale(self) -> torch.Tensor:
+        return self._out[1]
+
+    @property
+    def per_tensor(self) -> torch.Tensor:
+        return self._out[2:]
 
 
 def _keys(x) -> Optional[list]:
@@ -61,18 +75,34 @@ def _like(keys, values):
     return list(values) if keys is None else dict(zip(keys, values))
 
 
+# a list of many tensors is looked over attribute by attribute, each in one sweep
+_shape, _dtype = attrgetter("shape"), attrgetter("dtype")
+_data_ptr, _numel = torch.Tensor.data_ptr, torch.Tensor.numel
+_contiguous, _index = torch.Tensor.is_contiguous, torch.Tensor.get_device
+
+
 def _device(tensors, what: str) -> torch.device:
+    """The one GPU the tensors are on."""
     dev = tensors[0].device
     if dev.type != "cuda":
         raise ValueError(f"{what}: tensors must live on the GPU (there is no CPU path)")
+    if set(map(_index, tensors)) != {dev.index}:
+        raise ValueError(f"{what}: tensors on different devices, the first on {dev}")
     return dev
 
 
-def _types(tensors, what: str) -> list:
+def _types(tensors, what: str) -> array:
+    kinds = set(map(_dtype, tensors))
     try:
-        return [_TYPES[t.dtype] for t in tensors]
+        if len(kinds) == 1:
+            return array("i", [_TYPES[kinds.pop()]]) * len(tensors)
+        return array("i", [_TYPES[t.dtype] for t in tensors])
     except KeyError as e:
         raise TypeError(f"{what}: tensors must be float32, bfloat16 or float16, not {e.args[0]}") from None
+
+
+def _at(a: array) -> int:
+    return a.buffer_info()[0]
 
 
 def _mask(active_mask, tensors, dev, what: str):
@@ -82,10 +112,9 @@ def _mask(active_mask, tensors, dev, what: str):
     if act.dim() != 1:
         raise ValueError(f"{what}: active_mask must have one dimension")
     for i, t in enumerate(tensors):
-        if t is not None and (t.dim() == 0 or t.shape[0] != rows):
+        if t.dim() == 0 or t.shape[0] != rows:
             raise ValueError(f"{what}: active_mask has {rows} entries, tensor {i} has shape {tuple(t.shape)}")
-    lens = [1 if t is None or rows == 0 else max(t.numel() // rows, 1) for t in tensors]
-    return act, rows, (ctypes.c_int64 * len(lens))(*lens)
+    return act, rows, array("q", [max(t.numel() // max(rows, 1), 1) for t in tensors])
 
 
 def _scalar(grad_scale, dev, what: str):
@@ -98,6 +127,24 @@ def _scalar(grad_scale, dev, what: str):
     return grad_scale
 
 
+def _address(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _norms(dev, pointers: array, types: array, counts: array, mask, max_norm, scale) -> GradNorms:
+    k = len(pointers)
+    act, rows, lens = mask or (None, 0, None)
+    nbytes = _lib.lib().gs_grad_norms_workspace_size(k, _at(counts))
+    # one allocation: the results, and from the next multiple of 8 bytes on the workspace
+    head = (k + 3) // 2 * 2
+    out = torch.empty((head + (nbytes + 3) // 4,), dtype=torch.float32, device=dev)
+    at = out.data_ptr()
+    _lib.call("gs_grad_norms", _lib.stream_handle(dev), k, _at(pointers), _at(types), _at(counts),
+              None if lens is None else _at(lens), _address(act), rows, 0.0 if max_norm is None else float(max_norm),
+              _address(scale), at + 4 * head, nbytes, at + 8, at)
+    return GradNorms(out[:k + 2])
+
+
 def grad_norms(grads, max_norm: Optional[float] = None, active_mask=None, grad_scale=None) -> GradNorms:
     """2-norms of grad_scale times the gradients, per tensor and of all, and the factor
     ``grad_scale * min(1, max_norm / (total + 1e-6))`` (``grad_scale`` without ``max_norm``),
@@ -108,36 +155,19 @@ def grad_norms(grads, max_norm: Optional[float] = None, active_mask=None, grad_s
     if not have:
         raise ValueError("grad_norms: no gradients")
     dev = _device(have, "grad_norms")
-    k = len(gs)
-    act, rows, lens = None, 0, None
-    if active_mask is not None:
-        act, rows, lens = _mask(active_mask, gs, dev, "grad_norms")
-    if len(have) < k or not all([g.is_contiguous() for g in gs]):
-        some = have[0].new_empty(0)
-        gs = [some if g is None else g.contiguous() for g in gs]
-        if act is not None:
-            # an empty tensor has no rows: pass the others, and put zeros in its place
-            at = [i for i, g in enumerate(gs) if g.numel() or rows == 0]
-            if len(at) < k:
-                got = grad_norms([gs[i] for i in at], max_norm, active_mask, grad_scale)
-                each = got.per_tensor.new_zeros(k)
-                each[at] = got.per_tensor
-                return GradNorms(got.total, each, got.scale)
-    types = _types(gs, "grad_norms")
-    if any([g.device != dev for g in gs]):
-        raise ValueError(f"grad_norms: tensors on different devices, the first on {dev}")
-    scale = _scalar(grad_scale, dev, "grad_norms")
-    I64 = ctypes.c_int64 * k
-    counts = I64(*[g.numel() for g in gs])
-    nbytes = _lib.lib().gs_grad_norms_workspace_size(k, counts)
-    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-    out = torch.empty((k + 2,), dtype=torch.float32, device=dev)
-    at = out.data_ptr()
-    _lib.call("gs_grad_norms", _lib.stream_handle(dev), k, (ctypes.c_void_p * k)(*[g.data_ptr() for g in gs]),
-              (ctypes.c_int * k)(*types), counts, lens, _lib.ptr(act), rows,
-              0.0 if max_norm is None else float(max_norm), _lib.ptr(scale), ctypes.c_void_p(ws.data_ptr()), nbytes,
-              ctypes.c_void_p(at + 8), ctypes.c_void_p(at))
-    return GradNorms(out[0], out[2:], out[1])
+    mask = None if active_mask is None else _mask(active_mask, have, dev, "grad_norms")
+    if not all(map(_contiguous, have)):
+        have = [g.contiguous() for g in have]
+    pointers, counts = array("q", map(_data_ptr, have)), array("q", map(_numel, have))
+    types = _types(have, "grad_norms")
+    if len(have) < len(gs):
+        each = iter(range(len(have)))
+        at = [None if g is None else next(each) for g in gs]
+        pointers, counts, types = (array(a.typecode, [0 if i is None else a[i] for i in at])
+                                   for a in (pointers, counts, types))
+        if mask is not None:
+            mask = (*mask[:2], array("q", [1 if i is None else mask[2][i] for i in at]))
+    return _norms(dev, pointers, types, counts, mask, max_norm, _scalar(grad_scale, dev, "grad_norms"))
 
 
 class AdamWState:
@@ -153,19 +183,15 @@ class AdamWState:
     are fewer if a scale was not finite."""
 
     def __init__(self, keys, shapes, bits: int):
-        self.keys, self.shapes, self.bits = keys, [tuple(s) for s in shapes], bits
+        self.keys, self.shapes, self.bits = keys, [torch.Size(s) for s in shapes], bits
         self.counts, self.offsets, at = [], [], 0
         for s in self.shapes:
-            n = 1
-            for d in s:
-                n *= d
+            n = s.numel()
             self.counts.append(n)
             self.offsets.append(at)
             at += -(-n // BLOCK) * BLOCK
         self.size = at
-        k = len(self.shapes)
-        self._counts = (ctypes.c_int64 * k)(*self.counts)
-        self._offsets = (ctypes.c_int64 * k)(*self.offsets)
+        self._counts, self._offsets = array("q", self.counts), array("q", self.offsets)
         self.mu_flat = self.nu_flat = self.fields = self.master_flat = self.powers = None
         self.count = 0
         self.norms: Optional[GradNorms] = None
@@ -234,7 +260,7 @@ class AdamWState:
 
     def state_dict(self) -> dict:
         """The state as a dict of tensors (the state's own) and plain values, for a checkpoint."""
-        return {"bits": self.bits, "shapes": list(self.shapes), "count": self.count, "mu_flat": self.mu_flat,
+        return {"bits": self.bits, "shapes": [tuple(s) for s in self.shapes], "count": self.count, "mu_flat": self.mu_flat,
                 "nu_flat": self.nu_flat, "fields": self.fields, "master_flat": self.master_flat,
                 "powers": self.powers}
 
@@ -333,7 +359,7 @@ class AdamW:
         """The state of a checkpoint (``AdamWState.state_dict``) for these parameters."""
         state = self._state(params, int(d["bits"]))
         dev = _tensors(params)[0].device
-        if [tuple(s) for s in d["shapes"]] != state.shapes:
+        if [tuple(s) for s in d["shapes"]] != [tuple(s) for s in state.shapes]:
             raise ValueError("AdamW.load_state_dict: the checkpoint is of other tensors")
         state._allocate(dev, zero=True)
         for name in ("mu_flat", "nu_flat", "fields"):
@@ -353,44 +379,46 @@ class AdamW:
         ``grad_scale`` (one float32 on the device, or a number) multiplies the gradients; when it
         is not finite nothing changes.  Rows whose ``active_mask`` entry is False keep their
         parameters and take a zero gradient, whatever theirs holds."""
-        ps = _tensors(params, state.keys)
-        gs = _tensors(grads, state.keys)
-        k = len(ps)
-        if [tuple(p.shape) for p in ps] != state.shapes:
+        ps, gs = _tensors(params, state.keys), _tensors(grads, state.keys)
+        k, dev = len(ps), state.mu_flat.device
+        if list(map(_shape, ps)) != state.shapes:
             raise ValueError("AdamW: the parameters are not those of the state")
         if len(gs) != k:
             raise ValueError(f"AdamW: {len(gs)} gradients for {k} tensors")
-        dev = state.mu_flat.device
-        for i, (p, g) in enumerate(zip(ps, gs)):
-            if not p.is_contiguous() or p.device != dev:
-                raise ValueError(f"AdamW: parameter {i} must be a contiguous tensor on {dev}")
-            if g is not None:
-                if g.shape != p.shape or g.device != dev:
-                    raise ValueError(f"AdamW: gradient {i} must be shaped like its parameter on {dev}")
-                if not g.is_contiguous():
-                    gs[i] = g.contiguous()
-        at = [p.data_ptr() for p in ps]
-        if len(set(at)) < k and len({a for a, n in zip(at, state.counts) if n}) < sum(n > 0 for n in state.counts):
+        if not all(map(_contiguous, ps)) or set(map(_index, ps)) != {dev.index}:
+            raise ValueError(f"AdamW: the parameters must be contiguous tensors on {dev}")
+        missing = [i for i, g in enumerate(gs) if g is None]
+        for i in missing:
+            gs[i] = ps[i]  # in its place; its pointer is not passed on
+        if list(map(_shape, gs)) != state.shapes or set(map(_index, gs)) != {dev.index}:
+            raise ValueError(f"AdamW: the gradients must be shaped like their parameters on {dev}")
+        if not all(map(_contiguous, gs)):
+            gs = [g.contiguous() for g in gs]
+        to, of = array("q", map(_data_ptr, ps)), array("q", map(_data_ptr, gs))
+        if len(set(to)) < k and len({a for a, n in zip(to, state.counts) if n}) < sum(n > 0 for n in state.counts):
             raise ValueError("AdamW: a parameter is given twice")
+        counts, types = state._counts, _types(gs, "AdamW")
+        if missing:
+            counts = array("q", counts)
+            for i in missing:
+                of[i] = counts[i] = 0
+        mask = None if active_mask is None else _mask(active_mask, ps, dev, "AdamW")
+        act, rows, lens = mask or (None, 0, None)
         scale = _scalar(grad_scale, dev, "AdamW")
         if self.max_grad_norm is not None:
-            state.norms = grad_norms(gs, self.max_grad_norm, active_mask, scale)
+            state.norms = _norms(dev, of, types, counts, mask, self.max_grad_norm, scale)
             scale = state.norms.scale
-        act, rows, lens = None, 0, None
-        if active_mask is not None:
-            act, rows, lens = _mask(active_mask, ps, dev, "AdamW")
-        P, I, D = ctypes.c_void_p * k, ctypes.c_int * k, ctypes.c_double * k
-        rates = [self.lr_at(x, state.count) for x in self._each(self.lrs, state, "the learning rate")]
-        nxt = torch.empty_like(state.powers)
-        key = (self.seed * 0x85EBCA6B + (state.count + 1) * 0xC2B2AE3D + 0x27D4EB2F) & _MASK32
-        _lib.call("gs_adamw_step", _lib.stream_handle(dev), k, P(*at), I(*_types(ps, "AdamW")),
-                  P(*[0 if g is None else g.data_ptr() for g in gs]),
-                  I(*_types([p if g is None else g for p, g in zip(ps, gs)], "AdamW")), state._offsets, state._counts,
-                  lens, D(*rates), D(*[float(x) for x in self._each(self.decay, state, "weight_decay")]), state.bits,
-                  state.size, _lib.ptr(state.mu_flat), _lib.ptr(state.nu_flat), _lib.ptr(state.fields),
-                  _lib.ptr(state.master_flat), _lib.ptr(act), rows, _lib.ptr(scale), _lib.ptr(state.powers),
-                  _lib.ptr(nxt), self.b1, self.b2, self.eps, key)
-        state.powers = nxt
+        rates = array("d", [self.lr_at(x, state.count) for x in self._each(self.lrs, state, "the learning rate")])
+        decays = array("d", self._each(self.decay, state, "weight_decay"))
+        ptypes = _types(ps, "AdamW")
+        powers = torch.empty_like(state.powers)
+        key = (self.seed * 0x85EBCA6B + (state.count + 1) * 0xC2B2AE3D + 0x27D4EB2F) & 0xFFFFFFFF
+        _lib.call("gs_adamw_step", _lib.stream_handle(dev), k, _at(to), _at(ptypes), _at(of), _at(types),
+                  _at(state._offsets), _at(counts), None if lens is None else _at(lens), _at(rates), _at(decays),
+                  state.bits, state.size, state.mu_flat.data_ptr(), state.nu_flat.data_ptr(), _address(state.fields),
+                  _address(state.master_flat), _address(act), rows, _address(scale), state.powers.data_ptr(),
+                  powers.data_ptr(), self.b1, self.b2, self.eps, key)
+        state.powers = powers
         state.count += 1
         return state
 
