@@ -50,48 +50,86 @@ struct StepArgs {
 };
 static_assert(sizeof(StepArgs) <= 4096, "kernel arguments");
 
-// Four consecutive elements of a lane; `whole`: all of the wave's 256 exist, else the first n.
+// Four elements at p, which is only as aligned as its element: a tensor may begin anywhere.
 template <class T>
-__device__ inline void load4(const T* p, bool whole, int n, float (&x)[4]) {
-  // the vector is only as aligned as its element: a tensor may begin anywhere
+__device__ inline void load4(const T* p, float (&x)[4]) {
   typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-  if (whole) {
-    const vec v = *reinterpret_cast<const vec*>(p);
+  const vec v = *reinterpret_cast<const vec*>(p);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = (float)v[j];
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = j < n ? (float)p[j] : 0.0f;
-  }
+  for (int j = 0; j < 4; ++j) x[j] = (float)v[j];
 }
 template <class T>
-__device__ inline void store4(T* p, bool whole, int n, const float (&x)[4]) {
+__device__ inline void store4(T* p, const float (&x)[4]) {
   typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-  if (whole) {
-    vec v;
+  vec v;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = (T)x[j];
-    *reinterpret_cast<vec*>(p) = v;
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j < n) p[j] = (T)x[j];
-  }
+  for (int j = 0; j < 4; ++j) v[j] = (T)x[j];
+  *reinterpret_cast<vec*>(p) = v;
 }
 
-template <bool k8, bool kMask, class P, class G, bool kMaster>
-__device__ inline void step_chunk(const StepArgs& A, const StepTensor& t, int64_t chunk, float scale, float r1,
+// How a wave reads and writes its 256 elements of gradient and weight, the lane's four from l4 on.
+// Whole blocks know their types, so that all loads are on their way before the first wait.
+template <class P, class G, bool kMaster>
+struct WholeBlock {
+  const G* grad;
+  P* param;
+  float* master;
+  __device__ WholeBlock(const StepArgs& A, const StepTensor& t, int64_t base)
+      : grad((const G*)t.grad + base), param((P*)t.param + base), master(A.master + t.at + base) {}
+  __device__ int n(uint32_t) const { return 4; }
+  __device__ void load(uint32_t l4, float (&g)[4], float (&w)[4]) const {
+    load4(grad + l4, g);
+    if (kMaster) load4(master + l4, w);
+    else load4((const P*)param + l4, w);
+  }
+  __device__ void store(uint32_t l4, const float (&w)[4]) const {
+    store4(param + l4, w);
+    if (kMaster) store4(master + l4, w);
+  }
+};
+
+// The last, partial block of a tensor: element by element, of any types.
+struct PartBlock {
+  const void* grad;
+  void* param;
+  float* master;
+  int64_t base;
+  int left, gtype, ptype;
+  __device__ PartBlock(const StepArgs& A, const StepTensor& t, int64_t base_)
+      : grad(t.grad), param(t.param), master(t.kind & 1 ? A.master + t.at + base_ : nullptr), base(base_),
+        left((int)(t.count - base_)), gtype((t.kind >> 1) % 3), ptype(t.kind / 6) {}
+  __device__ int n(uint32_t l4) const { return min(max(left - (int)l4, 0), 4); }
+  static __device__ float get(const void* p, int type, int64_t i) {
+    return type == GS_TYPE_F32 ? ((const float*)p)[i]
+           : type == GS_TYPE_BF16 ? (float)((const __bf16*)p)[i] : (float)((const _Float16*)p)[i];
+  }
+  __device__ void load(uint32_t l4, float (&g)[4], float (&w)[4]) const {
+    const int k = n(l4);
+    for (int j = 0; j < 4; ++j) {
+      if (j >= k) continue;
+      g[j] = get(grad, gtype, base + l4 + j);
+      w[j] = master ? master[l4 + j] : get(param, ptype, base + l4 + j);
+    }
+  }
+  __device__ void store(uint32_t l4, const float (&w)[4]) const {
+    const int k = n(l4);
+    for (int j = 0; j < 4; ++j) {
+      if (j >= k) continue;
+      const int64_t i = base + l4 + j;
+      if (ptype == GS_TYPE_F32) ((float*)param)[i] = w[j];
+      else if (ptype == GS_TYPE_BF16) ((__bf16*)param)[i] = (__bf16)w[j];
+      else ((_Float16*)param)[i] = (_Float16)w[j];
+      if (master) master[l4 + j] = w[j];
+    }
+  }
+};
+
+template <bool k8, bool kMask, class Block>
+__device__ inline void step_block(const StepArgs& A, const StepTensor& t, int64_t base, float scale, float r1,
                                   float r2) {
   const uint32_t l4 = (threadIdx.x & 63u) * 4u;
-  const int64_t base = chunk + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) * kMomBlock;
-  const int64_t left = t.count - base;
-  if (left <= 0) return;  // the wave's block is past the end
-  const bool whole = left >= kMomBlock;
-  const int n = whole ? 4 : min(max((int)left - (int)l4, 0), 4);
   const int64_t at = t.at + base;
-  G* const grad = (G*)t.grad + base;
-  P* const param = (P*)t.param + base;
-  float* const master = A.master + at;
+  const Block io(A, t, base);
   float w[4] = {0.0f, 0.0f, 0.0f, 0.0f}, g[4] = {0.0f, 0.0f, 0.0f, 0.0f}, m[4], r[4], v[4];
   uint32_t m8 = 0, r8 = 0, f = 0;
   if (k8) {
@@ -99,16 +137,12 @@ __device__ inline void step_chunk(const StepArgs& A, const StepTensor& t, int64_
     r8 = *(const uint32_t*)((const uint8_t*)A.nu + at + l4);
     f = *(const uint16_t*)(A.fields + (at >> 7));
   } else {
-    load4((const float*)A.mu + at + l4, true, 4, m);
-    load4((const float*)A.nu + at + l4, true, 4, v);
+    load4((const float*)A.mu + at + l4, m);
+    load4((const float*)A.nu + at + l4, v);
   }
   // masked rows: neither gradient nor parameter is read or written
-  const uint32_t on = kMask ? rows_on<4>(A.active, t.row_magic, (uint32_t)t.row_len, base, l4, n) : 15u;
-  if (!kMask || on) {
-    load4(grad + l4, whole, n, g);
-    if (kMaster) load4(master + l4, whole, n, w);
-    else load4(param + l4, whole, n, w);
-  }
+  const uint32_t on = kMask ? rows_on<4>(A.active, t.row_magic, (uint32_t)t.row_len, base, l4, io.n(l4)) : 15u;
+  if (!kMask || on) io.load(l4, g, w);
   if (k8) {
     decode_m4(m8, (int)(f & 255u), m);
     decode_r4(r8, (int)(f >> 8), r);
@@ -129,10 +163,7 @@ __device__ inline void step_chunk(const StepArgs& A, const StepTensor& t, int64_
     const float y = w[j] - t.lr * (u + t.decay * w[j]);
     w[j] = !kMask || (on >> j & 1u) ? y : w[j];
   }
-  if (!kMask || on) {
-    store4(param + l4, whole, n, w);
-    if (kMaster) store4(master + l4, whole, n, w);
-  }
+  if (!kMask || on) io.store(l4, w);
   if (k8) {
     uint32_t h[4];
 #pragma unroll
@@ -142,8 +173,8 @@ __device__ inline void step_chunk(const StepArgs& A, const StepTensor& t, int64_
     *(uint32_t*)((uint8_t*)A.nu + at + l4) = r8;
     if (l4 == 0) *(uint16_t*)(A.fields + (at >> 7)) = (uint16_t)f;
   } else {
-    store4((float*)A.mu + at + l4, true, 4, m);
-    store4((float*)A.nu + at + l4, true, 4, v);
+    store4((float*)A.mu + at + l4, m);
+    store4((float*)A.nu + at + l4, v);
   }
 }
 
@@ -167,12 +198,18 @@ __global__ __launch_bounds__(256) void adamw_kernel(StepArgs A) {
   const int k = __popcll(__ballot(b >= A.begin[threadIdx.x & 63u])) - 1;
   if (k < 0) return;
   const StepTensor t = A.t[k];
-  const int64_t chunk = (int64_t)(b - A.begin[k]) * kStepChunk;
+  const int64_t base =
+      (int64_t)(b - A.begin[k]) * kStepChunk + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) * kMomBlock;
+  if (base >= t.count) return;  // the wave's block is past the end
   const float r1 = (float)A.powers[2], r2 = (float)A.powers[3];
+  if (t.count - base < kMomBlock) {
+    step_block<k8, kMask, PartBlock>(A, t, base, scale, r1, r2);
+    return;
+  }
   switch (t.kind) {
-#define GS_STEP(i, P, G, M)                                       \
-  case i:                                                         \
-    step_chunk<k8, kMask, P, G, M>(A, t, chunk, scale, r1, r2);   \
+#define GS_STEP(i, P, G, M)                                                    \
+  case i:                                                                      \
+    step_block<k8, kMask, WholeBlock<P, G, M>>(A, t, base, scale, r1, r2);     \
     break;
     GS_STEP(0, float, float, false)
     GS_STEP(2, float, __bf16, false)
@@ -200,8 +237,8 @@ __global__ __launch_bounds__(256) void moments_encode_kernel(int64_t blocks, con
   if (block >= blocks) return;
   const int64_t at = block * kMomBlock + (threadIdx.x & 63u) * 4;
   float m[4], r[4], v[4];
-  load4(mu + at, true, 4, m);
-  load4(nu + at, true, 4, v);
+  load4(mu + at, m);
+  load4(nu + at, v);
   roots4(v, r);
   const uint32_t none[4] = {0, 0, 0, 0};
   uint32_t cm, cr, f;
@@ -224,8 +261,8 @@ __global__ __launch_bounds__(256) void moments_decode_kernel(int64_t blocks, con
   decode_r4(*(const uint32_t*)(r8 + at), (int)(f >> 8), r);
 #pragma unroll
   for (int j = 0; j < 4; ++j) r[j] = r[j] * r[j];
-  store4(mu + at, true, 4, m);
-  store4(nu + at, true, 4, r);
+  store4(mu + at, m);
+  store4(nu + at, r);
 }
 
 bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }

@@ -57,23 +57,28 @@ __device__ inline uint32_t moment_field(uint32_t most) {
   return f < 254u ? f : 254u;
 }
 
-// A finite value x >= 0 scaled so that its code is the top of the bits (from bit 23 - kMant on),
-// with what rounds it added: a random number of 23 - kMant bits, or kNearest for round to nearest
-// even.  A root (kMant 4) above zero gets at least code 1; its bits are at least those of the
-// least normal float, as the root of any float32 is.
+// The code of a finite value x >= 0 in the top bits of the result (kMant 4: in the upper eight,
+// 3: in the seven below the sign's): x scaled so that its code is the top of its bits, with what
+// rounds it added.  noise: 16 random bits in bits 8..23, or kNearest for round to nearest even.
+// A root (kMant 4) above zero gets at least code 1, which lies in bit 24; the root of a float32
+// that is not zero has larger bits than that.
 constexpr uint32_t kNearest = 0xffffffffu;
 template <int kMant>
-__device__ inline uint32_t moment_bits(uint32_t x, int field, uint32_t low) {
-  constexpr int drop = 23 - kMant;
-  uint32_t b = float_to_bits(ldexpf(bits_to_float(x), 15 - field));
-  if (low == kNearest) low = (1u << (drop - 1)) - 1u + ((b >> drop) & 1u);
-  b += low;
+__device__ inline uint32_t moment_top(float x, int field, uint32_t noise) {
+  constexpr int drop = 23 - kMant, up = 24 - drop;  // the code's lowest bit goes to bit 24
+  const uint32_t b = float_to_bits(ldexpf(x, 15 - field));
+  uint32_t c;
+  if (noise == kNearest) c = (b + (1u << (drop - 1)) - 1u + ((b >> drop) & 1u)) << up;
+  else c = (b << up) + noise;
   if (kMant == 4) {
-    const uint32_t least = x < (1u << drop) ? x : 1u << drop;
-    b = b > least ? b : least;
+    const uint32_t least = min(float_to_bits(x), 1u << 24);
+    c = max(c, least);
   }
-  return b;
+  return c;
 }
+// Upper and lower half of 32 random bits, where moment_top takes them.
+__device__ inline uint32_t noise_hi(uint32_t h) { return __builtin_amdgcn_perm(0, h, 0x0c03020cu); }
+__device__ inline uint32_t noise_lo(uint32_t h) { return __builtin_amdgcn_perm(0, h, 0x0c01000cu); }
 
 // Four decoded values of the packed codes w of one lane; field as stored.  The signed code is the
 // machine's own 8-bit float (bias 7, the same "not finite" code).
@@ -122,8 +127,8 @@ __device__ inline void encode_block_odd(const float (&m)[4], const float (&r)[4]
   m8 = r8 = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    uint32_t cm = moment_bits<3>(mb[j], (int)fm, kStochastic ? (h[j] >> 16) << 4 : kNearest) >> 20;
-    uint32_t cr = moment_bits<4>(rb[j], (int)fr, kStochastic ? (h[j] & 0xffffu) << 3 : kNearest) >> 19;
+    uint32_t cm = moment_top<3>(bits_to_float(mb[j]), (int)fm, kStochastic ? noise_hi(h[j]) : kNearest) >> 24;
+    uint32_t cr = moment_top<4>(bits_to_float(rb[j]), (int)fr, kStochastic ? noise_lo(h[j]) : kNearest) >> 24;
     cm = mb[j] >= kInf ? 127u : cm < 126u ? cm : 126u;
     cr = rb[j] >= kInf ? 255u : cr < 254u ? cr : 254u;
     cm |= (float_to_bits(m[j]) >> 24) & 128u;
@@ -157,9 +162,9 @@ __device__ inline void encode_block(const float (&m)[4], const float (&r)[4], co
   uint32_t cm[4], cr[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    cm[j] = moment_bits<3>(mb[j], (int)fm, kStochastic ? (h[j] >> 16) << 4 : kNearest) << 4;
-    cm[j] |= float_to_bits(m[j]) & 0x80000000u;
-    cr[j] = moment_bits<4>(rb[j], (int)fr, kStochastic ? (h[j] & 0xffffu) << 3 : kNearest) << 5;
+    const uint32_t c = moment_top<3>(fabsf(m[j]), (int)fm, kStochastic ? noise_hi(h[j]) : kNearest);
+    cm[j] = (c & 0x7fffffffu) | (float_to_bits(m[j]) & 0x80000000u);
+    cr[j] = moment_top<4>(r[j], (int)fr, kStochastic ? noise_lo(h[j]) : kNearest);
   }
   m8 = pack_top(cm);
   r8 = pack_top(cr);
@@ -170,18 +175,18 @@ __device__ inline void encode_block(const float (&m)[4], const float (&r)[4], co
 // 1.9e9 of them compared with the compiler's sequence); a lane with smaller ones, whose residual
 // would underflow, or with one that is not finite takes that sequence.
 __device__ inline void roots4(const float (&v)[4], float (&r)[4]) {
-  constexpr float kLeast = 7.888609052210118e-31f;  // 2^-100
-  bool odd = false;
+  constexpr float kLeast = 7.888609052210118e-31f;  // 2^-100: bits 0x0d800000
+  uint32_t lo = 0xffffffffu, hi = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const float up = fmaxf(v[j], kLeast);
     const float y = __builtin_amdgcn_rsqf(up);
     const float s = v[j] * y;
     r[j] = fmaf(fmaf(-s, s, v[j]), 0.5f * y, s);
-    // between 0 and 2^-100, infinite or not a number
-    odd |= float_to_bits(v[j]) - 1u < float_to_bits(kLeast) - 1u || float_to_bits(v[j]) >= 0x7f800000u;
+    lo = min(lo, float_to_bits(v[j]) - 1u);
+    hi = max(hi, float_to_bits(v[j]));
   }
-  if (odd) {
+  if (lo < 0x0d7fffffu || hi >= 0x7f800000u) {  // above 0 and below 2^-100, or not finite
 #pragma unroll
     for (int j = 0; j < 4; ++j) r[j] = sqrtf(v[j]);
   }
