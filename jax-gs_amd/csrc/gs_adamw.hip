@@ -47,44 +47,78 @@ struct StepArgs {
   double b1d, b2d;
   float b1, b2, omb1, omb2, eps;
   uint32_t key;
+  bool stream_params;
 };
 static_assert(sizeof(StepArgs) <= 4096, "kernel arguments");
 
+// From this many bytes on (parameters, gradients and moments of a call) the arrays go past the
+// caches: nothing of them is left there for the next call, and what is written does not push out
+// what is about to be read.  float32, us with caches -> past them: 4M elements 21 -> 24, 8M
+// (128 MB) 46 -> 41, 16M 87 -> 73, 59M 296 -> 272, 177M 901 -> 823; in 8 bits 8M (80 MB)
+// 25 -> 27, 16M 52 -> 46, 32M 98 -> 89; encoding 12M (120 MB) 20 -> 23, 30M 55 -> 50, decoding
+// 30M 55 -> 45.
+constexpr int64_t kStreamBytes = (int64_t)128 << 20;
+// Parameters are read next by whatever uses the model: they go past the caches only when they
+// alone are as large (16M: 79 us past them, 73 not; 59M: 272 and 304).
+
 // Four elements at p, which is only as aligned as its element: a tensor may begin anywhere.
-template <class T>
+template <bool kStream, class T>
 __device__ inline void load4(const T* p, float (&x)[4]) {
   typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-  const vec v = *reinterpret_cast<const vec*>(p);
+  const vec* q = reinterpret_cast<const vec*>(p);
+  const vec v = kStream ? __builtin_nontemporal_load(q) : *q;
 #pragma unroll
   for (int j = 0; j < 4; ++j) x[j] = (float)v[j];
 }
-template <class T>
+template <bool kStream, class T>
 __device__ inline void store4(T* p, const float (&x)[4]) {
   typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
   vec v;
 #pragma unroll
   for (int j = 0; j < 4; ++j) v[j] = (T)x[j];
-  *reinterpret_cast<vec*>(p) = v;
+  vec* q = reinterpret_cast<vec*>(p);
+  if (kStream) __builtin_nontemporal_store(v, q);
+  else *q = v;
+}
+// Four 8-bit codes.
+template <bool kStream>
+__device__ inline uint32_t load_codes(const void* p, int64_t at) {
+  const uint32_t* q = (const uint32_t*)((const uint8_t*)p + at);
+  return kStream ? __builtin_nontemporal_load(q) : *q;
+}
+template <bool kStream>
+__device__ inline void store_codes(void* p, int64_t at, uint32_t x) {
+  uint32_t* q = (uint32_t*)((uint8_t*)p + at);
+  if (kStream) __builtin_nontemporal_store(x, q);
+  else *q = x;
 }
 
 // How a wave reads and writes its 256 elements of gradient and weight, the lane's four from l4 on.
 // Whole blocks know their types, so that all loads are on their way before the first wait.
-template <class P, class G, bool kMaster>
+template <bool kStream, class P, class G, bool kMaster>
 struct WholeBlock {
   const G* grad;
   P* param;
   float* master;
+  bool stream_params;
   __device__ WholeBlock(const StepArgs& A, const StepTensor& t, int64_t base)
-      : grad((const G*)t.grad + base), param((P*)t.param + base), master(A.master + t.at + base) {}
+      : grad((const G*)t.grad + base), param((P*)t.param + base), master(A.master + t.at + base),
+        stream_params(A.stream_params) {}
   __device__ int n(uint32_t) const { return 4; }
   __device__ void load(uint32_t l4, float (&g)[4], float (&w)[4]) const {
-    load4(grad + l4, g);
-    if (kMaster) load4(master + l4, w);
-    else load4((const P*)param + l4, w);
+    load4<kStream>(grad + l4, g);
+    if (kMaster) load4<kStream>(master + l4, w);
+    else load4<kStream>((const P*)param + l4, w);
   }
   __device__ void store(uint32_t l4, const float (&w)[4]) const {
-    store4(param + l4, w);
-    if (kMaster) store4(master + l4, w);
+    if (kStream && stream_params) {
+      asm volatile("");  // keeps the compiler from merging the two stores into one of the second kind
+      store4<true>(param + l4, w);
+      asm volatile("");
+    } else {
+      store4<false>(param + l4, w);
+    }
+    if (kMaster) store4<kStream>(master + l4, w);
   }
 };
 
@@ -124,7 +158,7 @@ struct PartBlock {
   }
 };
 
-template <bool k8, bool kMask, class Block>
+template <bool k8, bool kMask, bool kStream, class Block>
 __device__ inline void step_block(const StepArgs& A, const StepTensor& t, int64_t base, float scale, float r1,
                                   float r2) {
   const uint32_t l4 = (threadIdx.x & 63u) * 4u;
@@ -133,12 +167,12 @@ __device__ inline void step_block(const StepArgs& A, const StepTensor& t, int64_
   float w[4] = {0.0f, 0.0f, 0.0f, 0.0f}, g[4] = {0.0f, 0.0f, 0.0f, 0.0f}, m[4], r[4], v[4];
   uint32_t m8 = 0, r8 = 0, f = 0;
   if (k8) {
-    m8 = *(const uint32_t*)((const uint8_t*)A.mu + at + l4);
-    r8 = *(const uint32_t*)((const uint8_t*)A.nu + at + l4);
+    m8 = load_codes<kStream>(A.mu, at + l4);
+    r8 = load_codes<kStream>(A.nu, at + l4);
     f = *(const uint16_t*)(A.fields + (at >> 7));
   } else {
-    load4((const float*)A.mu + at + l4, m);
-    load4((const float*)A.nu + at + l4, v);
+    load4<kStream>((const float*)A.mu + at + l4, m);
+    load4<kStream>((const float*)A.nu + at + l4, v);
   }
   // masked rows: neither gradient nor parameter is read or written
   const uint32_t on = kMask ? rows_on<4>(A.active, t.row_magic, (uint32_t)t.row_len, base, l4, io.n(l4)) : 15u;
@@ -169,16 +203,16 @@ __device__ inline void step_block(const StepArgs& A, const StepTensor& t, int64_
 #pragma unroll
     for (int j = 0; j < 4; ++j) h[j] = place_hash(at, l4 + j, A.key);
     encode_block<true>(m, r, h, m8, r8, f);
-    *(uint32_t*)((uint8_t*)A.mu + at + l4) = m8;
-    *(uint32_t*)((uint8_t*)A.nu + at + l4) = r8;
+    store_codes<kStream>(A.mu, at + l4, m8);
+    store_codes<kStream>(A.nu, at + l4, r8);
     if (l4 == 0) *(uint16_t*)(A.fields + (at >> 7)) = (uint16_t)f;
   } else {
-    store4((float*)A.mu + at + l4, m);
-    store4((float*)A.nu + at + l4, v);
+    store4<kStream>((float*)A.mu + at + l4, m);
+    store4<kStream>((float*)A.nu + at + l4, v);
   }
 }
 
-template <bool k8, bool kMask>
+template <bool k8, bool kMask, bool kStream>
 __global__ __launch_bounds__(256) void adamw_kernel(StepArgs A) {
   const float scale = A.scale ? *A.scale : 1.0f;
   const bool ok = fabsf(scale) < __builtin_huge_valf();
@@ -203,13 +237,13 @@ __global__ __launch_bounds__(256) void adamw_kernel(StepArgs A) {
   if (base >= t.count) return;  // the wave's block is past the end
   const float r1 = (float)A.powers[2], r2 = (float)A.powers[3];
   if (t.count - base < kMomBlock) {
-    step_block<k8, kMask, PartBlock>(A, t, base, scale, r1, r2);
+    step_block<k8, kMask, false, PartBlock>(A, t, base, scale, r1, r2);
     return;
   }
   switch (t.kind) {
-#define GS_STEP(i, P, G, M)                                                    \
-  case i:                                                                      \
-    step_block<k8, kMask, WholeBlock<P, G, M>>(A, t, base, scale, r1, r2);     \
+#define GS_STEP(i, P, G, M)                                                                       \
+  case i:                                                                                         \
+    step_block<k8, kMask, kStream, WholeBlock<kStream, P, G, M>>(A, t, base, scale, r1, r2);      \
     break;
     GS_STEP(0, float, float, false)
     GS_STEP(2, float, __bf16, false)
@@ -230,6 +264,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(StepArgs A) {
   }
 }
 
+template <bool kStream>
 __global__ __launch_bounds__(256) void moments_encode_kernel(int64_t blocks, const float* __restrict__ mu,
                                                              const float* __restrict__ nu, uint8_t* __restrict__ m8,
                                                              uint8_t* __restrict__ r8, uint8_t* __restrict__ fields) {
@@ -237,17 +272,18 @@ __global__ __launch_bounds__(256) void moments_encode_kernel(int64_t blocks, con
   if (block >= blocks) return;
   const int64_t at = block * kMomBlock + (threadIdx.x & 63u) * 4;
   float m[4], r[4], v[4];
-  load4(mu + at, m);
-  load4(nu + at, v);
+  load4<kStream>(mu + at, m);
+  load4<kStream>(nu + at, v);
   roots4(v, r);
   const uint32_t none[4] = {0, 0, 0, 0};
   uint32_t cm, cr, f;
   encode_block<false>(m, r, none, cm, cr, f);
-  *(uint32_t*)(m8 + at) = cm;
-  *(uint32_t*)(r8 + at) = cr;
+  store_codes<kStream>(m8, at, cm);
+  store_codes<kStream>(r8, at, cr);
   if ((threadIdx.x & 63u) == 0) *(uint16_t*)(fields + 2 * block) = (uint16_t)f;
 }
 
+template <bool kStream>
 __global__ __launch_bounds__(256) void moments_decode_kernel(int64_t blocks, const uint8_t* __restrict__ m8,
                                                              const uint8_t* __restrict__ r8,
                                                              const uint8_t* __restrict__ fields,
@@ -257,12 +293,12 @@ __global__ __launch_bounds__(256) void moments_decode_kernel(int64_t blocks, con
   const int64_t at = block * kMomBlock + (threadIdx.x & 63u) * 4;
   const uint32_t f = *(const uint16_t*)(fields + 2 * block);
   float m[4], r[4];
-  decode_m4(*(const uint32_t*)(m8 + at), (int)(f & 255u), m);
-  decode_r4(*(const uint32_t*)(r8 + at), (int)(f >> 8), r);
+  decode_m4(load_codes<kStream>(m8, at), (int)(f & 255u), m);
+  decode_r4(load_codes<kStream>(r8, at), (int)(f >> 8), r);
 #pragma unroll
   for (int j = 0; j < 4; ++j) r[j] = r[j] * r[j];
-  store4(mu + at, m);
-  store4(nu + at, r);
+  store4<kStream>(mu + at, m);
+  store4<kStream>(nu + at, r);
 }
 
 bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
@@ -330,6 +366,19 @@ extern "C" int gs_adamw_step(void* stream, int num, void* const* params, const i
   A.eps = (float)eps;
   A.key = key;
   hipStream_t s = (hipStream_t)stream;
+  const int64_t state_bytes = (moment_bits == 8 ? 2 : 8) + (master ? 4 : 0);
+  int64_t param_bytes = 0, bytes = 0;
+  for (int j = 0; j < num; ++j)
+    if (grads[j]) {
+      param_bytes += counts[j] * (int64_t)size_of(param_types[j]);
+      bytes += counts[j] * ((int64_t)size_of(grad_types[j]) + state_bytes);
+    }
+  A.stream_params = param_bytes >= kStreamBytes;
+  const bool stream_all = param_bytes + bytes >= kStreamBytes;
+#define GS_KERNEL(k8, kMask) (stream_all ? adamw_kernel<k8, kMask, true> : adamw_kernel<k8, kMask, false>)
+  auto* kernel = moment_bits == 8 ? (active ? GS_KERNEL(true, true) : GS_KERNEL(true, false))
+                                  : (active ? GS_KERNEL(false, true) : GS_KERNEL(false, false));
+#undef GS_KERNEL
   // always one launch, so that the powers move on; further ones take what does not fit it
   int i = 0;
   do {
@@ -354,8 +403,6 @@ extern "C" int gs_adamw_step(void* stream, int num, void* const* params, const i
     }
     for (; k < 64; ++k) A.begin[k] = 0xffffffffu;
     const dim3 grid((unsigned)(groups > 0 ? groups : 1));
-    auto* kernel = moment_bits == 8 ? (active ? adamw_kernel<true, true> : adamw_kernel<true, false>)
-                                    : (active ? adamw_kernel<false, true> : adamw_kernel<false, false>);
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, A);
     GS_LAUNCH_CHECK("adamw_kernel");
     A.powers_next = nullptr;
@@ -373,7 +420,8 @@ extern "C" int gs_moments_encode(void* stream, int64_t state_size, const float* 
   GS_REQUIRE(aligned(mu, 16) && aligned(nu, 16) && aligned(mu8, 16) && aligned(nu8, 16) && aligned(fields, 2),
              "gs_moments_encode: the state's arrays must be 16-byte aligned");
   const int64_t blocks = state_size / kMomBlock;
-  hipLaunchKernelGGL(moments_encode_kernel, dim3((unsigned)div_up(blocks, 4)), dim3(256), 0, (hipStream_t)stream,
+  auto* kernel = state_size * 10 >= kStreamBytes ? moments_encode_kernel<true> : moments_encode_kernel<false>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)div_up(blocks, 4)), dim3(256), 0, (hipStream_t)stream,
                      blocks, mu, nu, mu8, nu8, fields);
   GS_LAUNCH_CHECK("moments_encode_kernel");
   return GS_OK;
@@ -388,7 +436,8 @@ extern "C" int gs_moments_decode(void* stream, int64_t state_size, const uint8_t
   GS_REQUIRE(aligned(mu, 16) && aligned(nu, 16) && aligned(mu8, 16) && aligned(nu8, 16) && aligned(fields, 2),
              "gs_moments_decode: the state's arrays must be 16-byte aligned");
   const int64_t blocks = state_size / kMomBlock;
-  hipLaunchKernelGGL(moments_decode_kernel, dim3((unsigned)div_up(blocks, 4)), dim3(256), 0, (hipStream_t)stream,
+  auto* kernel = state_size * 10 >= kStreamBytes ? moments_decode_kernel<true> : moments_decode_kernel<false>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)div_up(blocks, 4)), dim3(256), 0, (hipStream_t)stream,
                      blocks, mu8, nu8, fields, mu, nu);
   GS_LAUNCH_CHECK("moments_decode_kernel");
   return GS_OK;
