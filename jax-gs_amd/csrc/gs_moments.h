@@ -59,17 +59,16 @@ __device__ inline uint32_t moment_field(uint32_t most) {
 
 // The code of a finite value x >= 0 in the top bits of the result (kMant 4: in the upper eight,
 // 3: in the seven below the sign's): x scaled so that its code is the top of its bits, with what
-// rounds it added.  noise: 16 random bits in bits 8..23, or kNearest for round to nearest even.
+// rounds it added: 16 random bits in bits 8..23 (kStochastic), or what rounds to nearest even.
 // A root (kMant 4) above zero gets at least code 1, which lies in bit 24; the root of a float32
 // that is not zero has larger bits than that.
-constexpr uint32_t kNearest = 0xffffffffu;
-template <int kMant>
+template <int kMant, bool kStochastic>
 __device__ inline uint32_t moment_top(float x, int field, uint32_t noise) {
   constexpr int drop = 23 - kMant, up = 24 - drop;  // the code's lowest bit goes to bit 24
   const uint32_t b = float_to_bits(ldexpf(x, 15 - field));
   uint32_t c;
-  if (noise == kNearest) c = (b + (1u << (drop - 1)) - 1u + ((b >> drop) & 1u)) << up;
-  else c = (b << up) + noise;
+  if (kStochastic) c = (b << up) + noise;
+  else c = (b + (1u << (drop - 1)) - 1u + ((b >> drop) & 1u)) << up;
   if (kMant == 4) {
     const uint32_t least = min(float_to_bits(x), 1u << 24);
     c = max(c, least);
@@ -127,8 +126,8 @@ __device__ inline void encode_block_odd(const float (&m)[4], const float (&r)[4]
   m8 = r8 = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    uint32_t cm = moment_top<3>(bits_to_float(mb[j]), (int)fm, kStochastic ? noise_hi(h[j]) : kNearest) >> 24;
-    uint32_t cr = moment_top<4>(bits_to_float(rb[j]), (int)fr, kStochastic ? noise_lo(h[j]) : kNearest) >> 24;
+    uint32_t cm = moment_top<3, kStochastic>(bits_to_float(mb[j]), (int)fm, noise_hi(h[j])) >> 24;
+    uint32_t cr = moment_top<4, kStochastic>(bits_to_float(rb[j]), (int)fr, noise_lo(h[j])) >> 24;
     cm = mb[j] >= kInf ? 127u : cm < 126u ? cm : 126u;
     cr = rb[j] >= kInf ? 255u : cr < 254u ? cr : 254u;
     cm |= (float_to_bits(m[j]) >> 24) & 128u;
@@ -162,9 +161,9 @@ __device__ inline void encode_block(const float (&m)[4], const float (&r)[4], co
   uint32_t cm[4], cr[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint32_t c = moment_top<3>(fabsf(m[j]), (int)fm, kStochastic ? noise_hi(h[j]) : kNearest);
+    const uint32_t c = moment_top<3, kStochastic>(fabsf(m[j]), (int)fm, noise_hi(h[j]));
     cm[j] = (c & 0x7fffffffu) | (float_to_bits(m[j]) & 0x80000000u);
-    cr[j] = moment_top<4>(r[j], (int)fr, kStochastic ? noise_lo(h[j]) : kNearest);
+    cr[j] = moment_top<4, kStochastic>(r[j], (int)fr, noise_lo(h[j]));
   }
   m8 = pack_top(cm);
   r8 = pack_top(cr);
