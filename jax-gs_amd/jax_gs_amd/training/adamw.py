@@ -3,7 +3,7 @@ the factor that clips them.
 
 For models of any number of tensors of any sizes (the five Gaussian arrays, and whatever is
 trained next to them); ``optimizer.Adam`` stays the reference trainer's own step.  One launch
-updates up to 56 tensors, nothing waits for the host, and a step whose gradients are not finite
+updates up to 76 tensors, nothing waits for the host, and a step whose gradients are not finite
 changes nothing when its scale comes from ``grad_norms``:
 
     optimizer = AdamW(1e-3, weight_decay=0.01, moment_bits=8, max_grad_norm=1.0)
