@@ -18,6 +18,7 @@ alone).  The arithmetic is float32; the kernels are ``gs_adamw_step``, ``gs_grad
 from __future__ import annotations
 
 from array import array
+from copy import copy
 from operator import attrgetter
 from typing import Callable, Optional, Union
 
@@ -235,8 +236,8 @@ class AdamWState:
         """A state of its own with the same moments in ``bits`` (32 or 8), to nearest."""
         if bits not in (32, 8):
             raise ValueError(f"AdamWState.convert: 32 or 8 bits, not {bits}")
-        to = AdamWState(self.keys, self.shapes, bits)
-        to.count, to.powers = self.count, self.powers  # never written in place
+        to = copy(self)  # the layout and the powers are never written in place
+        to.bits, to.norms = bits, None
         to.master_flat = None if self.master_flat is None else self.master_flat.clone()
         to._allocate(self.mu_flat.device, zero=False)
         to.set_moments(self)
@@ -408,7 +409,11 @@ class AdamW:
         if self.max_grad_norm is not None:
             state.norms = _norms(dev, of, types, counts, mask, self.max_grad_norm, scale)
             scale = state.norms.scale
-        rates = array("d", [self.lr_at(x, state.count) for x in self._each(self.lrs, state, "the learning rate")])
+        rates = self._each(self.lrs, state, "the learning rate")
+        try:
+            rates = array("d", rates)
+        except TypeError:  # schedules among them
+            rates = array("d", [self.lr_at(x, state.count) for x in rates])
         decays = array("d", self._each(self.decay, state, "weight_decay"))
         ptypes = _types(ps, "AdamW")
         powers = torch.empty_like(state.powers)

@@ -431,6 +431,21 @@ def test_norms(cuda, kind, apart):
     assert torch.equal(grad_norms(gs).per_tensor, grad_norms(gs).per_tensor)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("sizes", [[1], [8191, 8192, 8193], [131_072], [131_073], [0, 131_071, 0, 1], [8192] * 16,
+                                   [100] * 17, [0] * 16])
+def test_norms_of_few_and_of_empty_tensors(cuda, kind, sizes):
+    """Around whole runs of a workgroup (8192 elements) and with empty tensors between."""
+    rng = np.random.default_rng(12)
+    gs = tensors(cuda, [rng.normal(0, 1, n).astype(np.float32) for n in sizes], TYPES[kind], apart=True)
+    each = np.array([np.sqrt((np64(g) ** 2).sum()) for g in gs])
+    total = np.sqrt((each ** 2).sum())
+    got = grad_norms(gs, max_norm=3.0, grad_scale=torch.full((), 0.5, device=cuda))
+    np.testing.assert_allclose(np64(got.per_tensor), 0.5 * each, rtol=2 * E)
+    assert abs(float(got.total) - 0.5 * total) <= 2 * E * total
+    assert abs(float(got.scale) - 0.5 * min(1.0, 3.0 / (0.5 * total + 1e-6))) <= 2 * E
+
+
 def test_norms_of_very_large_and_very_small_values(cuda):
     for x in (1e30, 3e38, 1e-30, 1e-44):
         g = torch.full((1000,), x, device=cuda)
@@ -454,7 +469,8 @@ def test_norms_that_are_not_finite(cuda, bad):
     assert float(ok.total) == pytest.approx(4999 ** 0.5)
 
 
-@pytest.mark.parametrize("rows, lens", [(1, [1, 7]), (379, [3, 48, 1]), (3, [5000, 4097]), (20_000, [48, 9])])
+@pytest.mark.parametrize("rows, lens", [(1, [1, 7]), (379, [3, 48, 1]), (3, [5000, 4097]), (20_000, [48, 9]),
+                                        (41, [5000, 8191, 8193, 9001]), (70_003, [1, 2, 3, 5, 6, 7, 8])])
 def test_norms_with_a_row_mask(cuda, rows, lens):
     rng = np.random.default_rng(10)
     on = rng.random(rows) < 0.5
@@ -465,6 +481,20 @@ def test_norms_with_a_row_mask(cuda, rows, lens):
         np.testing.assert_allclose(np64(got.per_tensor), each, rtol=2 * E)
         want = min(1.0, 0.1 / (np.linalg.norm(each) + 1e-6))
         assert abs(float(got.scale) - want) <= 2 * E
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("rows, lens", [(500, [1, 2, 3, 7, 8, 9, 48]), (9000, [1, 3, 5, 6, 16, 31])])
+def test_norms_of_half_types_with_a_row_mask(cuda, kind, rows, lens):
+    """Eight elements a lane, over up to eight rows; NaN in the masked ones."""
+    rng = np.random.default_rng(13)
+    on = rng.random(rows) < 0.4
+    gs = [torch.tensor(rng.normal(0, 1, (rows, n)).astype(np.float32), device=cuda).to(TYPES[kind]) for n in lens]
+    for g in gs:
+        g[torch.tensor(~on, device=cuda)] = float("nan")
+    each = [np.sqrt((np64(g)[on] ** 2).sum()) for g in gs]
+    got = grad_norms(gs, active_mask=torch.tensor(on, device=cuda))
+    np.testing.assert_allclose(np64(got.per_tensor), each, rtol=2 * E)
 
 
 def test_norms_of_nothing(cuda):
