@@ -411,6 +411,12 @@ extern "C" int gs_adamw_step(void* stream, int num, void* const* params, const i
   auto* kernel = moment_bits == 8 ? (active ? GS_KERNEL(true, true) : GS_KERNEL(true, false))
                                   : (active ? GS_KERNEL(false, true) : GS_KERNEL(false, false));
 #undef GS_KERNEL
+  // Shared memory that nobody uses, so that four workgroups of 32-bit moments fit a CU instead of
+  // eight: past the caches, seven streams of more waves than that crowd the memory (59M float32
+  // 275 us with eight, 265 with six, 260 with four; 177M 869, 840, 829; 35M bfloat16 with masters
+  // 158, 156, 151).  In 8 bits, where the arithmetic counts, eight are best (35M 91 us, 114
+  // with four), and under a mask, whose loads come first (124M, 40 % off: 489 us, 502 with four).
+  const unsigned lds = stream_all && moment_bits == 32 && !active ? 40960 : 0;
   // always one launch, so that the powers move on; further ones take what does not fit it
   int some = 0, i = 0;
   for (int j = 0; j < num; ++j) some += grads[j] && counts[j];
@@ -441,7 +447,7 @@ extern "C" int gs_adamw_step(void* stream, int num, void* const* params, const i
     A.n = k;
     A.groups = (uint32_t)groups;
     const dim3 grid((unsigned)(groups > 0 ? groups : 1));
-    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, A, grad_scale, powers, powers_next);
+    hipLaunchKernelGGL(kernel, grid, dim3(256), lds, s, A, grad_scale, powers, powers_next);
     GS_LAUNCH_CHECK("adamw_kernel");
     powers_next = nullptr;
     while (i < num && (!grads[i] || counts[i] == 0)) ++i;

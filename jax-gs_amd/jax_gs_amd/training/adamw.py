@@ -68,6 +68,9 @@ def _tensors(x, keys=None) -> list:
     if isinstance(x, Gaussians):
         return [getattr(x, f) for f in FIELDS]
     if isinstance(x, dict):
+        missing = [k for k in keys or () if k not in x]
+        if missing:
+            raise ValueError(f"AdamW: no tensor for {missing}")
         return [x[k] for k in (x if keys is None else keys)]
     return list(x)
 
@@ -151,6 +154,8 @@ def grad_norms(grads, max_norm: Optional[float] = None, active_mask=None, grad_s
     ``grad_scale * min(1, max_norm / (total + 1e-6))`` (``grad_scale`` without ``max_norm``),
     NaN when the total is not finite, all on the device.  Rows where ``active_mask`` is False
     are left out, whatever they hold; ``None`` gradients count as empty."""
+    if max_norm is not None and not max_norm > 0.0:
+        raise ValueError(f"grad_norms: max_norm must be positive, not {max_norm}")
     gs = _tensors(grads)
     have = [g for g in gs if g is not None]
     if not have:

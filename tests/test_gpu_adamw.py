@@ -586,7 +586,12 @@ def test_refusals(cuda):
         opt.restore([p], [p[:3]], [p], 1)
     with pytest.raises(ValueError, match="no gradients"):
         grad_norms([None])
-    assert state.count == 0 and not p.any()
+    with pytest.raises(ValueError, match="max_norm"):
+        grad_norms([g], max_norm=0.0)
+    named = AdamW(1e-3).init({"a": p, "b": p.clone()})
+    with pytest.raises(ValueError, match="no tensor for"):
+        opt.step({"a": p, "b": p.clone()}, {"a": g}, named)
+    assert state.count == 0 and named.count == 0 and not p.any()
 
 
 # ---- as it is used: the training step and density control -------------------------------------
