@@ -8,7 +8,10 @@
 //
 // Every workgroup sums one run of consecutive elements of one tensor (the runs' length is chosen
 // so that about 2048 of them cover all tensors) into one partial sum; a second launch of one
-// workgroup adds the partial sums of each tensor and the tensors' sums.
+// workgroup adds the partial sums of each tensor and the tensors' sums.  Reading bounds the first:
+// 59M float32 44 us (5.3 TB/s), 148 bfloat16 tensors of 22M elements 13 us, 124M float32 under a
+// mask 110 us (150 us behind a step, whose dirty lines are written back meanwhile); the second
+// takes 3 to 5 us, a chain of two reads and two reductions.
 #include "gs_rows.h"
 
 #include <algorithm>
