@@ -154,6 +154,22 @@ def lib():
     return _lib
 
 
+def tensors():
+    """The module _tensors (csrc/gs_tensors.cpp).  Raises NativeLibraryMissing if it was not built."""
+    global _tensors
+    if _tensors is None:
+        try:
+            from . import _tensors as module
+        except ImportError as e:
+            raise NativeLibraryMissing(f"jax_gs_amd._tensors does not load ({e}): build it with "
+                                       "`python -c 'import __graft_entry__ as g; g.build()'`") from e
+        _tensors = module
+    return _tensors
+
+
+_tensors = None
+
+
 def call(name: str, *args) -> None:
     """Call an int-returning entry point and raise on a non-zero status."""
     rc = getattr(lib(), name)(*args)

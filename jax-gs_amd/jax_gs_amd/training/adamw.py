@@ -19,7 +19,6 @@ from __future__ import annotations
 
 from array import array
 from copy import copy
-from operator import attrgetter
 from typing import Callable, Optional, Union
 
 import torch
@@ -32,16 +31,14 @@ from .optimizer import FIELDS, make_optimizer
 LearningRate = Union[float, Callable[[int], float]]
 BLOCK = 256  # elements that share an exponent in 8 bits; each tensor's moments begin at a multiple
 
-_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-
 
 class GradNorms:
     """Device float32: ``total``, the norm of all gradients; ``per_tensor``, each one's; ``scale``,
     the factor for the step."""
-    __slots__ = ("_out",)
+    __slots__ = ("_out", "_k")
 
-    def __init__(self, out: torch.Tensor):
-        self._out = out  # total, scale, one per tensor
+    def __init__(self, out: torch.Tensor, k: int):
+        self._out, self._k = out, k  # total, scale, one for each of k tensors, the call's workspace
 
     @property
     def total(self) -> torch.Tensor:
@@ -53,7 +50,7 @@ class GradNorms:
 
     @property
     def per_tensor(self) -> torch.Tensor:
-        return self._out[2:]
+        return self._out[2:2 + self._k]
 
 
 def _keys(x) -> Optional[list]:
@@ -79,34 +76,10 @@ def _like(keys, values):
     return list(values) if keys is None else dict(zip(keys, values))
 
 
-# a list of many tensors is looked over attribute by attribute, each in one sweep
-_shape, _dtype = attrgetter("shape"), attrgetter("dtype")
-_data_ptr, _numel = torch.Tensor.data_ptr, torch.Tensor.numel
-_contiguous, _index = torch.Tensor.is_contiguous, torch.Tensor.get_device
-
-
-def _device(tensors, what: str) -> torch.device:
-    """The one GPU the tensors are on."""
-    dev = tensors[0].device
-    if dev.type != "cuda":
+def _device(tensor, what: str) -> torch.device:
+    if not isinstance(tensor, torch.Tensor) or tensor.device.type != "cuda":
         raise ValueError(f"{what}: tensors must live on the GPU (there is no CPU path)")
-    if set(map(_index, tensors)) != {dev.index}:
-        raise ValueError(f"{what}: tensors on different devices, the first on {dev}")
-    return dev
-
-
-def _types(tensors, what: str) -> array:
-    kinds = set(map(_dtype, tensors))
-    try:
-        if len(kinds) == 1:
-            return array("i", [_TYPES[kinds.pop()]]) * len(tensors)
-        return array("i", [_TYPES[t.dtype] for t in tensors])
-    except KeyError as e:
-        raise TypeError(f"{what}: tensors must be float32, bfloat16 or float16, not {e.args[0]}") from None
-
-
-def _at(a: array) -> int:
-    return a.buffer_info()[0]
+    return tensor.device
 
 
 def _mask(active_mask, tensors, dev, what: str):
@@ -116,9 +89,10 @@ def _mask(active_mask, tensors, dev, what: str):
     if act.dim() != 1:
         raise ValueError(f"{what}: active_mask must have one dimension")
     for i, t in enumerate(tensors):
-        if t.dim() == 0 or t.shape[0] != rows:
+        if t is not None and (t.dim() == 0 or t.shape[0] != rows):
             raise ValueError(f"{what}: active_mask has {rows} entries, tensor {i} has shape {tuple(t.shape)}")
-    return act, rows, array("q", [max(t.numel() // max(rows, 1), 1) for t in tensors])
+    lens = [1 if t is None else max(t.numel() // max(rows, 1), 1) for t in tensors]
+    return act, rows, array("q", lens).tobytes()
 
 
 def _scalar(grad_scale, dev, what: str):
@@ -135,18 +109,16 @@ def _address(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-def _norms(dev, pointers: array, types: array, counts: array, mask, max_norm, scale) -> GradNorms:
-    k = len(pointers)
+def _norms(dev, k: int, pointers: bytes, types: bytes, counts: bytes, mask, max_norm, scale) -> GradNorms:
     act, rows, lens = mask or (None, 0, None)
-    nbytes = _lib.lib().gs_grad_norms_workspace_size(k, _at(counts))
+    nbytes = _lib.lib().gs_grad_norms_workspace_size(k, counts)
     # one allocation: the results, and from the next multiple of 8 bytes on the workspace
     head = (k + 3) // 2 * 2
     out = torch.empty((head + (nbytes + 3) // 4,), dtype=torch.float32, device=dev)
     at = out.data_ptr()
-    _lib.call("gs_grad_norms", _lib.stream_handle(dev), k, _at(pointers), _at(types), _at(counts),
-              None if lens is None else _at(lens), _address(act), rows, 0.0 if max_norm is None else float(max_norm),
-              _address(scale), at + 4 * head, nbytes, at + 8, at)
-    return GradNorms(out[:k + 2])
+    _lib.call("gs_grad_norms", _lib.stream_handle(dev), k, pointers, types, counts, lens, _address(act), rows,
+              0.0 if max_norm is None else float(max_norm), _address(scale), at + 4 * head, nbytes, at + 8, at)
+    return GradNorms(out, k)
 
 
 def grad_norms(grads, max_norm: Optional[float] = None, active_mask=None, grad_scale=None) -> GradNorms:
@@ -157,23 +129,13 @@ def grad_norms(grads, max_norm: Optional[float] = None, active_mask=None, grad_s
     if max_norm is not None and not max_norm > 0.0:
         raise ValueError(f"grad_norms: max_norm must be positive, not {max_norm}")
     gs = _tensors(grads)
-    have = [g for g in gs if g is not None]
-    if not have:
+    first = next((g for g in gs if g is not None), None)
+    if first is None:
         raise ValueError("grad_norms: no gradients")
-    dev = _device(have, "grad_norms")
-    mask = None if active_mask is None else _mask(active_mask, have, dev, "grad_norms")
-    if not all(map(_contiguous, have)):
-        have = [g.contiguous() for g in have]
-    pointers, counts = array("q", map(_data_ptr, have)), array("q", map(_numel, have))
-    types = _types(have, "grad_norms")
-    if len(have) < len(gs):
-        each = iter(range(len(have)))
-        at = [None if g is None else next(each) for g in gs]
-        pointers, counts, types = (array(a.typecode, [0 if i is None else a[i] for i in at])
-                                   for a in (pointers, counts, types))
-        if mask is not None:
-            mask = (*mask[:2], array("q", [1 if i is None else mask[2][i] for i in at]))
-    return _norms(dev, pointers, types, counts, mask, max_norm, _scalar(grad_scale, dev, "grad_norms"))
+    dev = _device(first, "grad_norms")
+    pointers, types, counts, kept = _lib.tensors().gather(gs, dev.index, "grad_norms")
+    mask = None if active_mask is None else _mask(active_mask, gs, dev, "grad_norms")
+    return _norms(dev, len(gs), pointers, types, counts, mask, max_norm, _scalar(grad_scale, dev, "grad_norms"))
 
 
 class AdamWState:
@@ -197,7 +159,7 @@ class AdamWState:
             self.offsets.append(at)
             at += -(-n // BLOCK) * BLOCK
         self.size = at
-        self._counts, self._offsets = array("q", self.counts), array("q", self.offsets)
+        self._offsets = array("q", self.offsets).tobytes()
         self.mu_flat = self.nu_flat = self.fields = self.master_flat = self.powers = None
         self.count = 0
         self.norms: Optional[GradNorms] = None
@@ -321,8 +283,8 @@ class AdamW:
         ps = _tensors(params)
         if not ps:
             raise ValueError("AdamW: no parameters")
-        _device(ps, "AdamW")
-        _types(ps, "AdamW")
+        if _lib.tensors().gather(ps, _device(ps[0], "AdamW").index, "AdamW")[3] is not None:
+            raise ValueError("AdamW: parameters must be contiguous")
         state = AdamWState(_keys(params), [p.shape for p in ps], bits)
         self._each(self.lrs, state, "the learning rate")
         self._each(self.decay, state, "weight_decay")
@@ -387,32 +349,12 @@ class AdamW:
         parameters and take a zero gradient, whatever theirs holds."""
         ps, gs = _tensors(params, state.keys), _tensors(grads, state.keys)
         k, dev = len(ps), state.mu_flat.device
-        if list(map(_shape, ps)) != state.shapes:
-            raise ValueError("AdamW: the parameters are not those of the state")
-        if len(gs) != k:
-            raise ValueError(f"AdamW: {len(gs)} gradients for {k} tensors")
-        if not all(map(_contiguous, ps)) or set(map(_index, ps)) != {dev.index}:
-            raise ValueError(f"AdamW: the parameters must be contiguous tensors on {dev}")
-        missing = [i for i, g in enumerate(gs) if g is None]
-        for i in missing:
-            gs[i] = ps[i]  # in its place; its pointer is not passed on
-        if list(map(_shape, gs)) != state.shapes or set(map(_index, gs)) != {dev.index}:
-            raise ValueError(f"AdamW: the gradients must be shaped like their parameters on {dev}")
-        if not all(map(_contiguous, gs)):
-            gs = [g.contiguous() for g in gs]
-        to, of = array("q", map(_data_ptr, ps)), array("q", map(_data_ptr, gs))
-        if len(set(to)) < k and len({a for a, n in zip(to, state.counts) if n}) < sum(n > 0 for n in state.counts):
-            raise ValueError("AdamW: a parameter is given twice")
-        counts, types = state._counts, _types(gs, "AdamW")
-        if missing:
-            counts = array("q", counts)
-            for i in missing:
-                of[i] = counts[i] = 0
+        to, to_types, of, of_types, counts, kept = _lib.tensors().pair(ps, gs, state.shapes, dev.index)
         mask = None if active_mask is None else _mask(active_mask, ps, dev, "AdamW")
         act, rows, lens = mask or (None, 0, None)
         scale = _scalar(grad_scale, dev, "AdamW")
         if self.max_grad_norm is not None:
-            state.norms = _norms(dev, of, types, counts, mask, self.max_grad_norm, scale)
+            state.norms = _norms(dev, k, of, of_types, counts, mask, self.max_grad_norm, scale)
             scale = state.norms.scale
         rates = self._each(self.lrs, state, "the learning rate")
         try:
@@ -420,14 +362,12 @@ class AdamW:
         except TypeError:  # schedules among them
             rates = array("d", [self.lr_at(x, state.count) for x in rates])
         decays = array("d", self._each(self.decay, state, "weight_decay"))
-        ptypes = _types(ps, "AdamW")
         powers = torch.empty_like(state.powers)
         key = (self.seed * 0x85EBCA6B + (state.count + 1) * 0xC2B2AE3D + 0x27D4EB2F) & 0xFFFFFFFF
-        _lib.call("gs_adamw_step", _lib.stream_handle(dev), k, _at(to), _at(ptypes), _at(of), _at(types),
-                  _at(state._offsets), _at(counts), None if lens is None else _at(lens), _at(rates), _at(decays),
-                  state.bits, state.size, state.mu_flat.data_ptr(), state.nu_flat.data_ptr(), _address(state.fields),
-                  _address(state.master_flat), _address(act), rows, _address(scale), state.powers.data_ptr(),
-                  powers.data_ptr(), self.b1, self.b2, self.eps, key)
+        _lib.call("gs_adamw_step", _lib.stream_handle(dev), k, to, to_types, of, of_types, state._offsets, counts,
+                  lens, rates.tobytes(), decays.tobytes(), state.bits, state.size, state.mu_flat.data_ptr(),
+                  state.nu_flat.data_ptr(), _address(state.fields), _address(state.master_flat), _address(act), rows,
+                  _address(scale), state.powers.data_ptr(), powers.data_ptr(), self.b1, self.b2, self.eps, key)
         state.powers = powers
         state.count += 1
         return state

@@ -558,6 +558,17 @@ def test_refusals(cuda):
         opt.step([p], [g], state)
     with pytest.raises(ValueError, match="given twice"):
         opt.step([p, p], [g, g], state)
+    both = torch.zeros(12, device=cuda)
+    with pytest.raises(ValueError, match="overlap"):
+        opt.step([both[:8], both[4:]], [g, g], state)
+    with pytest.raises(TypeError, match="entry 1 is not a tensor"):
+        opt.step([p, 3.0], [g, g], state)
+    with pytest.raises(TypeError, match="int64"):
+        grad_norms([g, torch.zeros(3, dtype=torch.int64, device=cuda)])
+    with pytest.raises(ValueError, match="is on cpu"):
+        grad_norms([g, torch.zeros(3)])
+    with pytest.raises(ValueError, match="contiguous"):
+        opt.init([torch.zeros(4, 6, device=cuda).t()])
     with pytest.raises(ValueError, match="2 tensors"):
         opt.step([p, p.clone()], [g], state)
     with pytest.raises(ValueError, match="shaped like"):
