@@ -549,7 +549,7 @@ int gs_grad_norms(void* stream, int num, const void* const* grads, const int* gr
  * in float32 with t = updates made, this one included; rows whose mask is 0 keep w.  s =
  * grad_scale[0] (device scalar, NULL for 1); when it is not finite nothing changes and t stays.
  * The moments are flat arrays of state_size elements, tensor i's from offsets[i] (a multiple of
- * GS_MOMENT_BLOCK) on, each tensor in blocks of its own.  moment_bits 32: mu, nu are float32 (m
+ * GS_MOMENT_BLOCK) on, each tensor in blocks of its own, in the order of the tensors.  moment_bits 32: mu, nu are float32 (m
  * and v), fields NULL.  moment_bits 8: mu, nu are bytes and fields holds two bytes per block
  * (see gs_moments_encode), rounded stochastically by a hash of the element's place and key,
  * which the caller changes from step to step.  Elements between tensors are left alone or

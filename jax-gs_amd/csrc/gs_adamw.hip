@@ -144,7 +144,8 @@ struct WholeBlock {
   }
 };
 
-// The last, partial block of a tensor: element by element, of any types.
+// The last, partial block of a tensor: element by element, of any types.  All loads are on their
+// way before the first is looked at: lanes past the end read the last element again.
 struct PartBlock {
   const void* grad;
   void* param;
@@ -155,16 +156,30 @@ struct PartBlock {
       : grad(t.grad), param(t.param), master(t.kind & 1 ? A.master + t.at + base_ : nullptr), base(base_),
         left((int)(t.count - base_)), gtype((t.kind >> 1) % 3), ptype(t.kind / 6) {}
   __device__ int n(uint32_t l4) const { return min(max(left - (int)l4, 0), 4); }
-  static __device__ float get(const void* p, int type, int64_t i) {
-    return type == GS_TYPE_F32 ? ((const float*)p)[i]
-           : type == GS_TYPE_BF16 ? (float)((const __bf16*)p)[i] : (float)((const _Float16*)p)[i];
+  __device__ void raw(const void* p, int64_t from, bool wide, uint32_t l4, uint32_t (&x)[4]) const {
+    const int last = left - 1;
+    if (wide) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = ((const uint32_t*)p)[from + min((int)l4 + j, last)];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = ((const uint16_t*)p)[from + min((int)l4 + j, last)];
+    }
+  }
+  static __device__ float value(uint32_t x, int type) {
+    if (type == GS_TYPE_F32) return bits_to_float(x);
+    if (type == GS_TYPE_BF16) return bits_to_float(x << 16);
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)x);
   }
   __device__ void load(uint32_t l4, float (&g)[4], float (&w)[4]) const {
+    uint32_t a[4], b[4];
+    raw(grad, base, gtype == GS_TYPE_F32, l4, a);
+    raw(master ? (const void*)master : param, master ? 0 : base, master || ptype == GS_TYPE_F32, l4, b);
     const int k = n(l4);
+#pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if (j >= k) continue;
-      g[j] = get(grad, gtype, base + l4 + j);
-      w[j] = master ? master[l4 + j] : get(param, ptype, base + l4 + j);
+      g[j] = j < k ? value(a[j], gtype) : 0.0f;
+      w[j] = j < k ? value(b[j], master ? GS_TYPE_F32 : ptype) : 0.0f;
     }
   }
   __device__ void store(uint32_t l4, const float (&w)[4]) const {
@@ -375,6 +390,7 @@ extern "C" int gs_adamw_step(void* stream, int num, void* const* params, const i
   GS_REQUIRE(b1 >= 0.0 && b1 < 1.0 && b2 >= 0.0 && b2 < 1.0, "gs_adamw_step: b1 and b2 must be in [0, 1)");
   GS_REQUIRE(eps >= 0.0, "gs_adamw_step: eps must not be negative");
   GS_REQUIRE(!active || row_lens, "gs_adamw_step: a mask needs row lengths");
+  int64_t used = 0;  // end of the moments of the tensors before
   for (int i = 0; i < num; ++i) {
     if (!grads[i] || counts[i] == 0) continue;
     const int pt = param_types[i], gt = grad_types[i];
@@ -388,6 +404,8 @@ extern "C" int gs_adamw_step(void* stream, int num, void* const* params, const i
     GS_REQUIRE(offsets[i] >= 0 && offsets[i] % kMomBlock == 0 && offsets[i] <= state_size &&
                    counts[i] <= state_size - offsets[i],
                "gs_adamw_step: tensor %d lies outside the state", i);
+    GS_REQUIRE(offsets[i] >= used, "gs_adamw_step: the moments of tensor %d do not lie behind those before", i);
+    used = offsets[i] + counts[i];
     if (active)
       GS_REQUIRE(row_lens[i] >= 1 && row_lens[i] < kMaxRowLen && rows >= 0 &&
                      counts[i] % row_lens[i] == 0 && counts[i] / row_lens[i] == rows,

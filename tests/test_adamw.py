@@ -54,6 +54,15 @@ def test_step_refusals(change, words):
     assert words in L.gs_last_error(), L.gs_last_error()
 
 
+def test_step_refuses_moments_that_overlap():
+    L = _lib.lib()
+    two = dict(num=2, params=(P * 2)(4096, 8192), ptypes=(I * 2)(), grads=(P * 2)(4096, 8192), gtypes=(I * 2)(),
+               counts=(I64 * 2)(300, 100), row_lens=None, lrs=(D * 2)(), decays=(D * 2)(), size=1024)
+    for offsets in ((0, 256), (256, 0), (512, 512)):
+        assert L.gs_adamw_step(*step_args(offsets=(I64 * 2)(*offsets), **two)) == 1
+        assert b"do not lie behind" in L.gs_last_error()
+
+
 @pytest.mark.parametrize("change, words", [
     (dict(num=-1), b"tensors"), (dict(grads=None), b"NULL"), (dict(out=None), b"NULL"), (dict(ws=None), b"NULL"),
     (dict(nbytes=8), b"workspace"), (dict(ws=P(68)), b"8-byte"), (dict(gtypes=(I * 1)(7)), b"type"),
