@@ -8,7 +8,7 @@
 //
 // The first three (five) are bytes objects holding int64 pointers, int32 types and int64 element
 // counts.  A None among the tensors (gradients) has pointer 0 and count 0.  A tensor that is not
-// contiguous is copied; `kept` holds the copies until the caller lets go of it.
+// contiguous (or a lazily negated view) is copied; `kept` holds the copies until the caller lets go of it.
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -84,7 +84,7 @@ struct Kept {
   ~Kept() { Py_XDECREF(list); }
   const at::Tensor& add(const at::Tensor& t) {
     if (!list && !(list = PyList_New(0))) refuse(PyExc_MemoryError, "out of memory");
-    PyObject* o = THPVariable_Wrap(t.contiguous());
+    PyObject* o = THPVariable_Wrap(t.resolve_neg().contiguous());
     if (!o || PyList_Append(list, o) != 0) {
       Py_XDECREF(o);
       refuse(PyExc_MemoryError, "out of memory");
@@ -98,6 +98,9 @@ struct Kept {
     return l;
   }
 };
+
+// Whether the memory at data_ptr() is the tensor's values one after another.
+bool plain(const at::Tensor& t) { return t.is_contiguous() && !t.is_neg(); }
 
 bool same_shape(const at::Tensor& t, PyObject* shape) {
   const auto sizes = t.sizes();
@@ -118,7 +121,7 @@ PyObject* do_gather(PyObject* list, int64_t device, const char* what) {
     const at::Tensor* t = &tensor_at(list, i, what);
     on_device(*t, device, what, i);
     types.at[i] = type_of(*t, PyList_GET_ITEM(list, i), what);
-    if (!t->is_contiguous()) t = &kept.add(*t);
+    if (!plain(*t)) t = &kept.add(*t);
     pointers.at[i] = (int64_t)(uintptr_t)t->data_ptr();
     counts.at[i] = t->numel();
   }
@@ -143,7 +146,7 @@ PyObject* do_pair(PyObject* params, PyObject* grads, PyObject* shapes, int64_t d
     if (!PyTuple_Check(shape) || !same_shape(p, shape))
       refuse(PyExc_ValueError, "AdamW: the parameters are not those of the state");
     on_device(p, device, what, i);
-    if (!p.is_contiguous())
+    if (!plain(p))
       refuse(PyExc_ValueError, "AdamW: parameter " + std::to_string(i) + " must be contiguous");
     to_types.at[i] = type_of(p, PyList_GET_ITEM(params, i), what);
     to.at[i] = (int64_t)(uintptr_t)p.data_ptr();
@@ -155,7 +158,7 @@ PyObject* do_pair(PyObject* params, PyObject* grads, PyObject* shapes, int64_t d
       refuse(PyExc_ValueError, "AdamW: gradient " + std::to_string(i) + " must be shaped like its parameter, on " +
                                    p.device().str());
     of_types.at[i] = type_of(*g, PyList_GET_ITEM(grads, i), what);
-    if (!g->is_contiguous()) g = &kept.add(*g);
+    if (!plain(*g)) g = &kept.add(*g);
     of.at[i] = (int64_t)(uintptr_t)g->data_ptr();
     counts.at[i] = p.numel();
   }

@@ -18,7 +18,6 @@ alone).  The arithmetic is float32; the kernels are ``gs_adamw_step``, ``gs_grad
 from __future__ import annotations
 
 from array import array
-from copy import copy
 from typing import Callable, Optional, Union
 
 import torch
@@ -203,7 +202,8 @@ class AdamWState:
         """A state of its own with the same moments in ``bits`` (32 or 8), to nearest."""
         if bits not in (32, 8):
             raise ValueError(f"AdamWState.convert: 32 or 8 bits, not {bits}")
-        to = copy(self)  # the layout and the powers are never written in place
+        to = AdamWState.__new__(AdamWState)
+        to.__dict__.update(self.__dict__)  # the layout and the powers are never written in place
         to.bits, to.norms = bits, None
         to.master_flat = None if self.master_flat is None else self.master_flat.clone()
         to._allocate(self.mu_flat.device, zero=False)
@@ -220,11 +220,11 @@ class AdamWState:
                 if getattr(self, name) is not None:
                     getattr(self, name).copy_(getattr(other, name))
         elif self.bits == 8:
-            _lib.call("gs_moments_encode", _lib.stream_handle(dev), self.size, _lib.ptr(other.mu_flat),
-                      _lib.ptr(other.nu_flat), _lib.ptr(self.mu_flat), _lib.ptr(self.nu_flat), _lib.ptr(self.fields))
+            _lib.call("gs_moments_encode", _lib.stream_handle(dev), self.size, *map(_address, (
+                other.mu_flat, other.nu_flat, self.mu_flat, self.nu_flat, self.fields)))
         else:
-            _lib.call("gs_moments_decode", _lib.stream_handle(dev), self.size, _lib.ptr(other.mu_flat),
-                      _lib.ptr(other.nu_flat), _lib.ptr(other.fields), _lib.ptr(self.mu_flat), _lib.ptr(self.nu_flat))
+            _lib.call("gs_moments_decode", _lib.stream_handle(dev), self.size, *map(_address, (
+                other.mu_flat, other.nu_flat, other.fields, self.mu_flat, self.nu_flat)))
 
     def state_dict(self) -> dict:
         """The state as a dict of tensors (the state's own) and plain values, for a checkpoint."""

@@ -279,6 +279,19 @@ def test_gradients_that_are_not_contiguous_or_missing(cuda):
     assert float(a.norms.per_tensor[3]) == 0.0 and not a.mu[3].any()
 
 
+def test_gradients_that_are_views_of_complex_values(cuda):
+    """The imaginary part of a conjugate: strided, and negated only when it is read."""
+    z = torch.randn(600, dtype=torch.complex64, device=cuda)
+    g = z.conj().imag
+    p, q = torch.ones(600, device=cuda), torch.ones(600, device=cuda)
+    opt = AdamW(1e-2)
+    opt.step(p, g, opt.init(p))
+    opt.step(q, -torch.view_as_real(z)[:, 1].contiguous(), opt.init(q))
+    assert torch.equal(p, q)
+    want = np.sqrt((np64(z.imag) ** 2).sum())
+    assert abs(float(grad_norms(g).total) - want) <= 4 * E * want
+
+
 def test_step_on_a_stream_of_the_callers(cuda):
     g = torch.randn(100_000, device=cuda)
     p, q = torch.ones(100_000, device=cuda), torch.ones(100_000, device=cuda)
