@@ -24,9 +24,7 @@
 
 namespace gs {
 
-constexpr int kMomBlock = 256;  // elements per block: one wave, four elements a lane
-
-typedef float floatx4 __attribute__((ext_vector_type(4)));
+constexpr int kMomBlock = GS_MOMENT_BLOCK;  // elements per block: one wave, four elements a lane
 
 // Maxima of x and of y over the wave, in every lane (unsigned order is that of non-negative
 // floats).  A lane without a source reads 0, so that each step is one instruction; the two
