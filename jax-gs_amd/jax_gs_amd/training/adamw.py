@@ -160,6 +160,7 @@ class AdamWState:
         self.size = at
         self._offsets = array("q", self.offsets).tobytes()
         self.mu_flat = self.nu_flat = self.fields = self.master_flat = self.powers = None
+        self._powers_stream: Optional[int] = None  # that the powers were allocated on
         self.count = 0
         self.norms: Optional[GradNorms] = None
 
@@ -168,6 +169,10 @@ class AdamWState:
         dtype = torch.float32 if self.bits == 32 else torch.uint8
         self.mu_flat, self.nu_flat = (new((self.size,), dtype=dtype, device=dev) for _ in range(2))
         self.fields = new((self.size // BLOCK, 2), dtype=torch.uint8, device=dev) if self.bits == 8 else None
+
+    def _set_powers(self, powers: torch.Tensor) -> None:
+        """Take over powers that were allocated on the current stream."""
+        self.powers, self._powers_stream = powers, _lib.stream_handle(powers.device).value
 
     def _views(self, flat):
         return _like(self.keys, [flat[o:o + n].view(s) for o, n, s in zip(self.offsets, self.counts, self.shapes)])
@@ -302,7 +307,7 @@ class AdamW:
         state = self._state(params, self.moment_bits)
         ps = _tensors(params)
         state._allocate(ps[0].device, zero=True)
-        state.powers = self._powers(0, ps[0].device)
+        state._set_powers(self._powers(0, ps[0].device))
         self._masters(state, ps, None)
         return state
 
@@ -318,7 +323,8 @@ class AdamW:
                 raise ValueError("AdamW.restore: the moments are not those of the parameters")
             for o, n, x in zip(full.offsets, full.counts, given):
                 flat[o:o + n].copy_(x.detach().reshape(-1))
-        full.count, full.powers = int(count), self._powers(int(count), ps[0].device)
+        full.count = int(count)
+        full._set_powers(self._powers(full.count, ps[0].device))
         state = full if self.moment_bits == 32 else full.convert(8)
         self._masters(state, ps, master)
         return state
@@ -333,7 +339,8 @@ class AdamW:
         for name in ("mu_flat", "nu_flat", "fields"):
             if getattr(state, name) is not None:
                 getattr(state, name).copy_(d[name])
-        state.count, state.powers = int(d["count"]), d["powers"].to(device=dev, dtype=torch.float64, copy=True)
+        state.count = int(d["count"])
+        state._set_powers(d["powers"].to(device=dev, dtype=torch.float64, copy=True))
         if d["master_flat"] is not None:
             state.master_flat = d["master_flat"].to(device=dev, dtype=torch.float32, copy=True)
         return state
@@ -364,11 +371,16 @@ class AdamW:
         decays = array("d", self._each(self.decay, state, "weight_decay"))
         powers = torch.empty_like(state.powers)
         key = (self.seed * 0x85EBCA6B + (state.count + 1) * 0xC2B2AE3D + 0x27D4EB2F) & 0xFFFFFFFF
-        _lib.call("gs_adamw_step", _lib.stream_handle(dev), k, to, to_types, of, of_types, state._offsets, counts,
+        stream = _lib.stream_handle(dev)
+        _lib.call("gs_adamw_step", stream, k, to, to_types, of, of_types, state._offsets, counts,
                   lens, rates.tobytes(), decays.tobytes(), state.bits, state.size, state.mu_flat.data_ptr(),
                   state.nu_flat.data_ptr(), _address(state.fields), _address(state.master_flat), _address(act), rows,
                   _address(scale), state.powers.data_ptr(), powers.data_ptr(), self.b1, self.b2, self.eps, key)
-        state.powers = powers
+        if stream.value != state._powers_stream:
+            # read here, and about to be let go of: whoever the allocator gives them to on the stream
+            # that they come from waits for this step
+            state.powers.record_stream(torch.cuda.current_stream(dev))
+        state.powers, state._powers_stream = powers, stream.value
         state.count += 1
         return state
 

@@ -1,0 +1,79 @@
+"""What AdamW hands to the native step, on the host: the device calls are recorded, not made."""
+import ctypes
+
+import pytest
+import torch
+
+from jax_gs_amd import _lib
+from jax_gs_amd.training.adamw import AdamW, AdamWState
+
+
+class Recorder:
+    """Stands in for the native library and for streams: keeps the arguments of every call, and which
+    memory was recorded on which stream."""
+
+    def __init__(self, monkeypatch):
+        self.calls, self.recorded, self.stream = [], [], 0
+        monkeypatch.setattr(_lib, "call", lambda name, *args: self.calls.append((name, args)))
+        monkeypatch.setattr(_lib, "stream_handle", lambda device: ctypes.c_void_p(self.stream))
+        monkeypatch.setattr(_lib, "tensors", lambda: self)
+        monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: self.stream)
+        monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: self.recorded.append((t.data_ptr(), s)))
+
+    @staticmethod
+    def pair(ps, gs, shapes, device):
+        return b"", b"", b"", b"", b"", None
+
+    def __getattr__(self, name):  # whatever else the list module offers
+        return lambda *args: None
+
+    def steps(self):
+        return [args for name, args in self.calls if name == "gs_adamw_step"]
+
+
+def host_state(opt, shapes=((300,), (7,))):
+    state = AdamWState(None, shapes, opt.moment_bits)
+    state._allocate(torch.device("cpu"), zero=True)
+    state._set_powers(opt._powers(0, torch.device("cpu")))
+    return state
+
+
+POWERS, NEXT = 20, 21  # places of powers and powers_next among gs_adamw_step's arguments
+
+
+def test_powers_are_not_handed_back_while_another_stream_reads_them(monkeypatch):
+    """A step on another stream than the one its powers were allocated on: their memory is recorded on the
+    step's stream, so that the allocator's next user waits for it.  On one stream nothing is to be done."""
+    native = Recorder(monkeypatch)
+    opt = AdamW(1e-3)
+    state = host_state(opt)
+    ps = [torch.zeros(s) for s in state.shapes]
+    held, want, owner = [], [], 0
+    for stream in (0, 0, 64, 64, 64, 0, 96, 96):
+        native.stream = stream
+        held.append(state.powers)  # so that an address cannot come back
+        if stream != owner:
+            want.append((state.powers.data_ptr(), stream))
+        owner = stream
+        opt.step(ps, ps, state)
+    assert native.recorded == want and len(want) == 3
+    args = native.steps()
+    assert [a[NEXT] for a in args[:-1]] == [a[POWERS] for a in args[1:]]
+    assert state.powers.data_ptr() == args[-1][NEXT]
+
+
+def test_powers_of_a_converted_state(monkeypatch):
+    """Two states share the powers until each steps; neither step writes what the other reads."""
+    native = Recorder(monkeypatch)
+    opt = AdamW(1e-3)
+    a = host_state(opt)
+    native.stream = 64
+    b = a.convert(8)
+    ps = [torch.zeros(s) for s in a.shapes]
+    held, shared = [a.powers], a.powers.data_ptr()
+    for s in (a, b, a, b):
+        opt.step(ps, ps, s)
+        held.append(s.powers)
+    args = native.steps()
+    assert args[0][POWERS] == args[1][POWERS] == shared and len({x[NEXT] for x in args} | {shared}) == 5
+    assert native.recorded == [(shared, 64), (shared, 64)]

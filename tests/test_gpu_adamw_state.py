@@ -1,0 +1,53 @@
+"""AdamW's state: streams, checkpoints, masters, and what a step leaves alone."""
+import numpy as np
+import pytest
+import torch
+
+from jax_gs_amd.training.adamw import AdamW
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_steps_on_a_stream_while_another_allocates(cuda, bits):
+    """The state is made on one stream and stepped on another, while the first allocates and fills arrays of
+    the powers' size: the bits of a run on one stream."""
+    n = 4_000_000
+    gen = torch.Generator(device=cuda).manual_seed(0)
+    p = torch.randn(n, generator=gen, device=cuda)
+    g = torch.randn(n, generator=gen, device=cuda)
+    q = p.clone()
+    opt = AdamW(1e-2, weight_decay=0.1, moment_bits=bits, max_grad_norm=1.0)
+    a, b = opt.init(p), opt.init(q)
+    for _ in range(8):
+        opt.step(p, g, a)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    filled = []
+    for _ in range(8):
+        with torch.cuda.stream(side):
+            opt.step(q, g, b)
+        filled += [torch.full((4,), 0.5, dtype=torch.float64, device=cuda) for _ in range(16)]
+        del filled[:-8]
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(a.powers, b.powers) and a.count == b.count == 8
+    np.testing.assert_allclose(a.powers.cpu().numpy()[:2], [0.9 ** 8, 0.999 ** 8], rtol=1e-14)
+    assert torch.equal(p, q) and torch.equal(a.mu_flat, b.mu_flat) and torch.equal(a.nu_flat, b.nu_flat)
+
+
+def test_a_converted_state_goes_on_by_itself(cuda):
+    """Steps of the one leave the other's powers, which were the same."""
+    g = torch.ones(1000, device=cuda)
+    opt = AdamW(1e-2)
+    p = torch.zeros(1000, device=cuda)
+    a = opt.init(p)
+    opt.step(p, g, a)
+    b = a.convert(8)
+    q = p.clone()
+    for _ in range(3):
+        opt.step(p, g, a)
+    np.testing.assert_allclose(b.powers.cpu().numpy()[:2], [0.9, 0.999], rtol=1e-15)
+    opt.step(q, g, b)
+    np.testing.assert_allclose(b.powers.cpu().numpy()[:2], [0.9 ** 2, 0.999 ** 2], rtol=1e-15)
+    np.testing.assert_allclose(a.powers.cpu().numpy()[:2], [0.9 ** 4, 0.999 ** 4], rtol=1e-14)
