@@ -137,6 +137,14 @@ def grad_norms(grads, max_norm: Optional[float] = None, active_mask=None, grad_s
     return _norms(dev, len(gs), pointers, types, counts, mask, max_norm, _scalar(grad_scale, dev, "grad_norms"))
 
 
+def _load(own: torch.Tensor, d: dict, name: str) -> torch.Tensor:
+    """A checkpoint's array into the state's own, which the kernels take to be whole."""
+    given = d[name]
+    if not isinstance(given, torch.Tensor) or given.shape != own.shape:
+        raise ValueError(f"AdamW.load_state_dict: {name} must be a tensor of shape {tuple(own.shape)}")
+    return own.copy_(given)
+
+
 class AdamWState:
     """Moments and step count of one model's parameters.
 
@@ -331,18 +339,21 @@ class AdamW:
 
     def load_state_dict(self, params, d: dict) -> AdamWState:
         """The state of a checkpoint (``AdamWState.state_dict``) for these parameters."""
-        state = self._state(params, int(d["bits"]))
+        bits = int(d["bits"])
+        if bits not in (32, 8):
+            raise ValueError(f"AdamW.load_state_dict: moments in 32 or 8 bits, not {bits}")
+        state = self._state(params, bits)
         dev = _tensors(params)[0].device
         if [tuple(s) for s in d["shapes"]] != [tuple(s) for s in state.shapes]:
             raise ValueError("AdamW.load_state_dict: the checkpoint is of other tensors")
         state._allocate(dev, zero=True)
         for name in ("mu_flat", "nu_flat", "fields"):
             if getattr(state, name) is not None:
-                getattr(state, name).copy_(d[name])
+                _load(getattr(state, name), d, name)
         state.count = int(d["count"])
-        state._set_powers(d["powers"].to(device=dev, dtype=torch.float64, copy=True))
+        state._set_powers(_load(torch.empty((4,), dtype=torch.float64, device=dev), d, "powers"))
         if d["master_flat"] is not None:
-            state.master_flat = d["master_flat"].to(device=dev, dtype=torch.float32, copy=True)
+            state.master_flat = _load(torch.empty((state.size,), dtype=torch.float32, device=dev), d, "master_flat")
         return state
 
     def lr_at(self, lr: LearningRate, count: int) -> float:

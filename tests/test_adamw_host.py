@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from jax_gs_amd import _lib
+from jax_gs_amd.training import adamw
 from jax_gs_amd.training.adamw import AdamW, AdamWState
 
 
@@ -77,3 +78,58 @@ def test_powers_of_a_converted_state(monkeypatch):
     args = native.steps()
     assert args[0][POWERS] == args[1][POWERS] == shared and len({x[NEXT] for x in args} | {shared}) == 5
     assert native.recorded == [(shared, 64), (shared, 64)]
+
+
+@pytest.fixture
+def on_host(monkeypatch):
+    """States may be made of host tensors."""
+    native = Recorder(monkeypatch)
+    monkeypatch.setattr(adamw, "_device", lambda t, what: t.device)
+    native.gather = lambda ts, device, what: (b"", b"", b"", None)
+    return native
+
+
+def checkpoint(opt, params):
+    state = opt.init(params)
+    return {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in state.state_dict().items()}
+
+
+@pytest.mark.parametrize("bits, name, length", [
+    (32, "mu_flat", 1), (32, "nu_flat", 511), (32, "powers", 3), (32, "powers", 1), (32, "master_flat", 511), (32, "master_flat", 1),
+    (8, "mu_flat", 513), (8, "nu_flat", 1), (8, "powers", 8), (8, "master_flat", 513), (8, "fields", 1)])
+def test_buffers_of_another_length_are_not_loaded(on_host, bits, name, length):
+    """The native step takes their addresses alone: a short one would be read and written out of range."""
+    params = [torch.zeros(300, dtype=torch.bfloat16)]
+    opt = AdamW(1e-3, moment_bits=bits, master_weights=True)
+    saved = checkpoint(opt, params)
+    assert saved[name].shape[0] != length
+    opt.load_state_dict(params, saved)
+    bad = torch.zeros((length, *saved[name].shape[1:]), dtype=saved[name].dtype)
+    with pytest.raises(ValueError, match=name):
+        opt.load_state_dict(params, {**saved, name: bad})
+
+
+def test_a_checkpoint_without_a_buffer_is_refused(on_host):
+    params = [torch.zeros(300)]
+    opt = AdamW(1e-3, moment_bits=8)
+    saved = checkpoint(opt, params)
+    for name in ("mu_flat", "nu_flat", "fields", "powers"):
+        with pytest.raises(ValueError, match=name):
+            opt.load_state_dict(params, {**saved, name: None})
+    with pytest.raises(ValueError, match="32 or 8"):
+        opt.load_state_dict(params, {**saved, "bits": 16})
+
+
+def test_loaded_buffers_are_whole_and_the_states_own(on_host):
+    """Strided and lazily negated tensors of the right length are loaded as their values."""
+    params = [torch.zeros(300, dtype=torch.float16)]
+    opt = AdamW(1e-3, master_weights=True)
+    saved = checkpoint(opt, params)
+    z = torch.complex(torch.zeros(512), torch.arange(512.0))
+    saved["master_flat"] = z.conj().imag
+    saved["mu_flat"] = torch.arange(1024.0)[::2]
+    state = opt.load_state_dict(params, saved)
+    for t, want in ((state.master_flat, -torch.arange(512.0)), (state.mu_flat, torch.arange(0.0, 1024.0, 2.0))):
+        assert t.is_contiguous() and not t.is_neg() and torch.equal(t, want)
+    state.powers.fill_(7.0)
+    assert not (saved["powers"] == 7.0).any()
