@@ -22,13 +22,11 @@
 // 2.1M Gaussians (124M elements, 40 % of the rows masked) in 32 bits 487 us; 3M (177M, 20 %
 // masked) in 8 bits 462 us.  The smallest call takes 4.4 us, five dependent reads.
 #include "gs_moments.h"
+#include "gs_pieces.h"
 #include "gs_rows.h"
 
 namespace gs {
 namespace {
-
-constexpr int kStepTensors = 76;   // per launch: the argument block stays below 4 KiB
-constexpr int kStepChunk = 1024;   // elements per workgroup
 
 struct StepTensor {
   void* param;
@@ -41,7 +39,7 @@ struct StepTensor {
   int kind;       // parameter type * 6 + gradient type * 2 + master
 };
 
-// As it is passed: one record per tensor, which a wave reads from one or two cache lines (arrays
+// As it is passed: one record per tensor (per 2^30 elements of one), which a wave reads from one or two cache lines (arrays
 // per field, ten lines, cost a tenth of the whole step in 8 bits: 158 -> 172 us).
 struct StepRecord {
   void* param;
@@ -53,12 +51,12 @@ struct StepRecord {
   float lr, decay;
   uint8_t last;     // elements of the last block, less one
   uint8_t kind;
-  uint16_t unused;
+  uint16_t piece;   // the record's workgroups begin at piece * kPieceGroups of the tensor
 };
 
 struct StepArgs {
   StepRecord t[kStepTensors];
-  uint32_t begin[kStepTensors];  // first workgroup
+  uint32_t begin[kStepTensors];  // first workgroup of each record
   int32_t n;
   uint32_t groups;
   void* mu;
@@ -274,7 +272,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(
   // their way (3M Gaussians 784 -> 764 us); in 32 bits, where more of them at once crowd the
   // memory (35M bfloat16 weights with masters 164 us asked here, 189 asked there), before.
   if (!k8 && !is_finite(scale)) return;
-  int k = -1;  // the last tensor that begins at or before this workgroup
+  int k = -1;  // the last record that begins at or before this workgroup
   for (int i = 0; i < A.n; i += 64) {
     const int q = i + (int)(threadIdx.x & 63u);
     k += __popcll(__ballot(q < A.n && b >= A.begin[min(q, kStepTensors - 1)]));
@@ -290,8 +288,8 @@ __global__ __launch_bounds__(256) void adamw_kernel(
                      q.lr,
                      q.decay,
                      q.kind};
-  const int64_t base =
-      (int64_t)(b - A.begin[k]) * kStepChunk + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) * kMomBlock;
+  const int64_t base = (q.piece * kPieceGroups + (b - A.begin[k])) * kStepChunk +
+                       __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) * kMomBlock;
   if (base >= t.count) return;  // the wave's block is past the end
   if (t.count - base < kMomBlock) {
     step_block<k8, kMask, false, PartBlock>(A, t, base, scale, r1, r2);
@@ -446,17 +444,14 @@ extern "C" int gs_adamw_step(void* stream, int num, void* const* params, const i
   // with four), and under a mask, whose loads come first (124M, 40 % off: 489 us, 502 with four).
   const unsigned lds = stream_all && moment_bits == 32 && !active ? 40960 : 0;
   // always one launch, so that the powers move on; further ones take what does not fit it
-  int some = 0, i = 0;
-  for (int j = 0; j < num; ++j) some += grads[j] && counts[j];
-  const int launches = (some + kStepTensors - 1) / kStepTensors;
-  const int each = launches > 0 ? (some + launches - 1) / launches : 0;
+  StepPieces pieces(num, grads, counts);
   do {
-    int k = 0;
+    StepPiece out[kStepTensors];
     int64_t groups = 0;
-    for (; i < num && k < each; ++i) {
-      if (!grads[i] || counts[i] == 0) continue;
-      const int64_t more = (counts[i] + kStepChunk - 1) / kStepChunk;
-      if (k > 0 && groups + more > 0x7fffffff) break;
+    A.n = pieces.next(out, groups);
+    A.groups = (uint32_t)groups;
+    for (int k = 0; k < A.n; ++k) {
+      const int i = out[k].tensor;
       const int64_t blocks = (counts[i] + kMomBlock - 1) / kMomBlock;
       StepRecord& t = A.t[k];
       t.param = params[i];
@@ -464,22 +459,19 @@ extern "C" int gs_adamw_step(void* stream, int num, void* const* params, const i
       t.at = (uint32_t)(offsets[i] / kMomBlock);
       t.blocks = (uint32_t)blocks;
       t.last = (uint8_t)(counts[i] - (blocks - 1) * kMomBlock - 1);
+      t.piece = (uint16_t)out[k].piece;
       t.row_len = active ? (uint32_t)row_lens[i] : 1u;
       t.magic = row_magic(t.row_len);
       t.lr = (float)lrs[i];
       t.decay = (float)decays[i];
       t.kind = (uint8_t)(param_types[i] * 6 + grad_types[i] * 2 + (param_types[i] != GS_TYPE_F32 && master ? 1 : 0));
-      A.begin[k++] = (uint32_t)groups;
-      groups += more;
+      A.begin[k] = (uint32_t)out[k].begin;
     }
-    A.n = k;
-    A.groups = (uint32_t)groups;
     const dim3 grid((unsigned)(groups > 0 ? groups : 1));
     hipLaunchKernelGGL(kernel, grid, dim3(256), lds, s, A, grad_scale, powers, powers_next);
     GS_LAUNCH_CHECK("adamw_kernel");
     powers_next = nullptr;
-    while (i < num && (!grads[i] || counts[i] == 0)) ++i;
-  } while (i < num);
+  } while (!pieces.done());
   return GS_OK;
 }
 
@@ -493,9 +485,13 @@ extern "C" int gs_moments_encode(void* stream, int64_t state_size, const float* 
              "gs_moments_encode: the state's arrays must be 16-byte aligned");
   const int64_t blocks = state_size / kMomBlock;
   auto* kernel = state_size * 10 >= kStreamBytes ? moments_encode_kernel<true> : moments_encode_kernel<false>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)div_up(blocks, 4)), dim3(256), 0, (hipStream_t)stream,
-                     blocks, mu, nu, mu8, nu8, fields);
-  GS_LAUNCH_CHECK("moments_encode_kernel");
+  for (int64_t first = 0, here; first < blocks; first += here) {
+    here = conversion_blocks(first, blocks);
+    const int64_t at = first * kMomBlock;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)div_up(here, 4)), dim3(256), 0, (hipStream_t)stream, here,
+                       mu + at, nu + at, mu8 + at, nu8 + at, fields + 2 * first);
+    GS_LAUNCH_CHECK("moments_encode_kernel");
+  }
   return GS_OK;
 }
 
@@ -509,8 +505,12 @@ extern "C" int gs_moments_decode(void* stream, int64_t state_size, const uint8_t
              "gs_moments_decode: the state's arrays must be 16-byte aligned");
   const int64_t blocks = state_size / kMomBlock;
   auto* kernel = state_size * 10 >= kStreamBytes ? moments_decode_kernel<true> : moments_decode_kernel<false>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)div_up(blocks, 4)), dim3(256), 0, (hipStream_t)stream,
-                     blocks, mu8, nu8, fields, mu, nu);
-  GS_LAUNCH_CHECK("moments_decode_kernel");
+  for (int64_t first = 0, here; first < blocks; first += here) {
+    here = conversion_blocks(first, blocks);
+    const int64_t at = first * kMomBlock;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)div_up(here, 4)), dim3(256), 0, (hipStream_t)stream, here,
+                       mu8 + at, nu8 + at, fields + 2 * first, mu + at, nu + at);
+    GS_LAUNCH_CHECK("moments_decode_kernel");
+  }
   return GS_OK;
 }
