@@ -304,10 +304,17 @@ class AdamW:
         return state
 
     def _masters(self, state: AdamWState, ps, master) -> None:
-        if not self.master_weights or all([p.dtype == torch.float32 for p in ps]):
+        if all([p.dtype == torch.float32 for p in ps]):
             return
+        if not self.master_weights:
+            if master is not None:
+                raise ValueError("AdamW.restore: masters given to an optimizer that keeps none (master_weights)")
+            return
+        given = ps if master is None else _tensors(master, state.keys)
+        if [x.numel() for x in given] != state.counts:
+            raise ValueError("AdamW.restore: the masters are not those of the parameters")
         state.master_flat = torch.zeros((state.size,), dtype=torch.float32, device=ps[0].device)
-        for o, n, x in zip(state.offsets, state.counts, ps if master is None else _tensors(master, state.keys)):
+        for o, n, x in zip(state.offsets, state.counts, given):
             state.master_flat[o:o + n].copy_(x.detach().reshape(-1))
 
     def init(self, params) -> AdamWState:

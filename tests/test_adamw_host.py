@@ -133,3 +133,19 @@ def test_loaded_buffers_are_whole_and_the_states_own(on_host):
         assert t.is_contiguous() and not t.is_neg() and torch.equal(t, want)
     state.powers.fill_(7.0)
     assert not (saved["powers"] == 7.0).any()
+
+
+def test_masters_must_be_those_of_the_parameters(on_host):
+    """Too few of them, or one value for a whole tensor, would leave weights to be computed from zeros or from
+    that value."""
+    params = [torch.ones(300, dtype=torch.bfloat16), torch.ones(7, dtype=torch.bfloat16)]
+    zeros = [torch.zeros(300), torch.zeros(7)]
+    opt = AdamW(1e-3, master_weights=True)
+    good = [torch.full((300,), 1.001), torch.full((7,), 0.999)]
+    state = opt.restore(params, zeros, zeros, 3, master=good)
+    assert all(torch.equal(a, b) for a, b in zip(state.master, good))
+    for bad in (good[:1], [good[0], good[1][:1]], [good[0], torch.ones(())], good + good, [good[0], torch.ones(8)]):
+        with pytest.raises(ValueError, match="masters are not those"):
+            opt.restore(params, zeros, zeros, 3, master=bad)
+    with pytest.raises(ValueError, match="keeps none"):
+        AdamW(1e-3).restore(params, zeros, zeros, 3, master=good)
