@@ -345,7 +345,8 @@ class AdamW:
         return state
 
     def load_state_dict(self, params, d: dict) -> AdamWState:
-        """The state of a checkpoint (``AdamWState.state_dict``) for these parameters."""
+        """The state of a checkpoint (``AdamWState.state_dict``) for these parameters: with its bits and its
+        master weights.  Where it has none and the optimizer keeps them, they are the parameters' values."""
         bits = int(d["bits"])
         if bits not in (32, 8):
             raise ValueError(f"AdamW.load_state_dict: moments in 32 or 8 bits, not {bits}")
@@ -361,6 +362,8 @@ class AdamW:
         state._set_powers(_load(torch.empty((4,), dtype=torch.float64, device=dev), d, "powers"))
         if d["master_flat"] is not None:
             state.master_flat = _load(torch.empty((state.size,), dtype=torch.float32, device=dev), d, "master_flat")
+        else:
+            self._masters(state, _tensors(params), None)
         return state
 
     def lr_at(self, lr: LearningRate, count: int) -> float:

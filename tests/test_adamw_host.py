@@ -149,3 +149,23 @@ def test_masters_must_be_those_of_the_parameters(on_host):
             opt.restore(params, zeros, zeros, 3, master=bad)
     with pytest.raises(ValueError, match="keeps none"):
         AdamW(1e-3).restore(params, zeros, zeros, 3, master=good)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_masters_of_a_checkpoint_without_any(on_host, bits):
+    """An optimizer that keeps masters makes them from the parameters, as init does; one that keeps none goes on
+    with those that a checkpoint has."""
+    params = [torch.randn(300).to(torch.bfloat16), torch.randn(7), torch.zeros(0, dtype=torch.float16)]
+    without, keeps = AdamW(1e-3, moment_bits=bits), AdamW(1e-3, moment_bits=bits, master_weights=True)
+    saved = checkpoint(without, params)
+    assert saved["master_flat"] is None
+    state = keeps.load_state_dict(params, saved)
+    assert state.master_flat is not None and torch.equal(state.master_flat, keeps.init(params).master_flat)
+    assert torch.equal(state.master[0], params[0].float())
+    assert without.load_state_dict(params, saved).master_flat is None
+    saved = checkpoint(keeps, params)
+    saved["master_flat"] += 2.0 ** -12
+    for opt in (keeps, without):
+        assert torch.equal(opt.load_state_dict(params, saved).master_flat, saved["master_flat"])
+    full = [p.float() for p in params]
+    assert keeps.load_state_dict(full, checkpoint(keeps, full)).master_flat is None
