@@ -101,7 +101,7 @@ def _scalar(grad_scale, dev, what: str):
         return torch.full((), float(grad_scale), device=dev)
     if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != dev:
         raise ValueError(f"{what}: grad_scale must be one float32 on {dev}")
-    return grad_scale
+    return grad_scale.resolve_neg()
 
 
 def _address(t: Optional[torch.Tensor]):

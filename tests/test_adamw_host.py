@@ -1,5 +1,6 @@
 """What AdamW hands to the native step, on the host: the device calls are recorded, not made."""
 import ctypes
+from array import array
 
 import pytest
 import torch
@@ -23,7 +24,8 @@ class Recorder:
 
     @staticmethod
     def pair(ps, gs, shapes, device):
-        return b"", b"", b"", b"", b"", None
+        counts = array("q", [p.numel() for p in ps]).tobytes()
+        return b"", b"", b"", b"", counts, None
 
     def __getattr__(self, name):  # whatever else the list module offers
         return lambda *args: None
@@ -169,3 +171,23 @@ def test_masters_of_a_checkpoint_without_any(on_host, bits):
         assert torch.equal(opt.load_state_dict(params, saved).master_flat, saved["master_flat"])
     full = [p.float() for p in params]
     assert keeps.load_state_dict(full, checkpoint(keeps, full)).master_flat is None
+
+
+SCALE = 19  # place of grad_scale among gs_adamw_step's arguments
+
+
+def test_a_lazily_negated_scale_is_handed_on_as_its_value(on_host):
+    """The imaginary part of a conjugate is float32 and reads as minus what lies in memory."""
+    opt = AdamW(1e-3)
+    ps = [torch.zeros(300)]
+    state = opt.init(ps)
+    scale = torch.tensor(complex(0.0, -0.5), dtype=torch.complex64).conj().imag
+    assert scale.is_neg() and float(scale) == 0.5
+    seen = []
+    call = _lib.call
+    _lib.call = lambda name, *args: (call(name, *args), seen.append(ctypes.c_float.from_address(args[SCALE]).value))
+    try:
+        opt.step(ps, ps, state, grad_scale=scale)
+    finally:
+        _lib.call = call
+    assert seen == [0.5]
