@@ -381,6 +381,7 @@ class AdamW:
         mask = None if active_mask is None else _mask(active_mask, ps, dev, "AdamW")
         act, rows, lens = mask or (None, 0, None)
         scale = _scalar(grad_scale, dev, "AdamW")
+        state.norms = None
         if self.max_grad_norm is not None:
             state.norms = _norms(dev, k, of, of_types, counts, mask, self.max_grad_norm, scale)
             scale = state.norms.scale

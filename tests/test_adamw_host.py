@@ -191,3 +191,14 @@ def test_a_lazily_negated_scale_is_handed_on_as_its_value(on_host):
     finally:
         _lib.call = call
     assert seen == [0.5]
+
+
+def test_norms_are_those_of_the_last_step(on_host):
+    """A step that takes no norm leaves none behind from an earlier one."""
+    clips, plain = AdamW(1e-3, max_grad_norm=1.0), AdamW(1e-3)
+    ps = [torch.zeros(300)]
+    state = clips.init(ps)
+    clips.step(ps, ps, state)
+    assert state.norms is not None
+    plain.step(ps, ps, state)
+    assert state.norms is None
