@@ -130,7 +130,17 @@ struct WholeBlock {
     if (kMaster) load4<kStream>(master + l4, w);
     else load4<kStream>((const P*)param + l4, w);
   }
-  __device__ void store(uint32_t l4, const float (&w)[4]) const {
+  // on: which of the four to store.  Without masters the others are what was read from there.
+  __device__ void store(uint32_t l4, const float (&w)[4], uint32_t on) const {
+    if (kMaster && on != 15u) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (on >> j & 1u) {
+          param[l4 + j] = (P)w[j];
+          master[l4 + j] = w[j];
+        }
+      return;
+    }
     if (kStream && stream_params) {
       asm volatile("");  // keeps the compiler from merging the two stores into one of the second kind
       store4<true>(param + l4, w);
@@ -180,10 +190,10 @@ struct PartBlock {
       w[j] = j < k ? value(b[j], master ? GS_TYPE_F32 : ptype) : 0.0f;
     }
   }
-  __device__ void store(uint32_t l4, const float (&w)[4]) const {
+  __device__ void store(uint32_t l4, const float (&w)[4], uint32_t on) const {
     const int k = n(l4);
     for (int j = 0; j < 4; ++j) {
-      if (j >= k) continue;
+      if (j >= k || !(on >> j & 1u)) continue;
       const int64_t i = base + l4 + j;
       if (ptype == GS_TYPE_F32) ((float*)param)[i] = w[j];
       else if (ptype == GS_TYPE_BF16) ((__bf16*)param)[i] = (__bf16)w[j];
@@ -236,7 +246,7 @@ __device__ inline void step_block(const StepArgs& A, const StepTensor& t, int64_
     const float y = w[j] - t.lr * (u + t.decay * w[j]);
     w[j] = !kMask || (on >> j & 1u) ? y : w[j];
   }
-  if (!kMask || on) io.store(l4, w);
+  if (!kMask || on) io.store(l4, w, on);
   if (k8) {
     uint32_t h[4];
 #pragma unroll

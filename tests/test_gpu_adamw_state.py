@@ -51,3 +51,22 @@ def test_a_converted_state_goes_on_by_itself(cuda):
     opt.step(q, g, b)
     np.testing.assert_allclose(b.powers.cpu().numpy()[:2], [0.9 ** 2, 0.999 ** 2], rtol=1e-15)
     np.testing.assert_allclose(a.powers.cpu().numpy()[:2], [0.9 ** 4, 0.999 ** 4], rtol=1e-14)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows, row", [(400, 1), (333, 3), (100, 2), (9, 301), (7, 4)])
+def test_masked_rows_keep_what_the_program_wrote(cuda, bits, dtype, rows, row):
+    """Half parameters with masters: a program writes its tensor, not the masters.  Rows whose mask is off keep what
+    it wrote, whoever their neighbours are, and their masters stay too; the others follow their masters."""
+    gen = torch.Generator(device=cuda).manual_seed(rows)
+    p = torch.randn(rows, row, generator=gen, device=cuda).to(dtype)
+    on = torch.rand(rows, generator=gen, device=cuda) < 0.5
+    on[:2] = torch.tensor([True, False], device=cuda)
+    opt = AdamW(1e-2, moment_bits=bits, master_weights=True)
+    state = opt.init([p])
+    p.fill_(3.0)
+    master = state.master[0].clone()
+    opt.step([p], [torch.ones(rows, row, device=cuda).to(dtype)], state, active_mask=on)
+    assert bool((p[~on] == 3.0).all()) and torch.equal(state.master[0][~on], master[~on])
+    assert torch.equal(p[on], state.master[0][on].to(dtype)) and not bool((state.master[0][on] == master[on]).any())
