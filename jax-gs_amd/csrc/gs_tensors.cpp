@@ -5,6 +5,7 @@
 //
 //   gather(tensors, device, what)                  -> (pointers, types, counts, kept)
 //   pair(params, grads, shapes, device)            -> (to, to_types, of, of_types, counts, kept)
+//   written(tensors, grads)                        -> None: marks as modified in place what a call wrote
 //
 // The first three (five) are bytes objects holding int64 pointers, int32 types and int64 element
 // counts.  A None among the tensors (gradients) has pointer 0 and count 0.  A tensor that is not
@@ -170,6 +171,20 @@ PyObject* do_pair(PyObject* params, PyObject* grads, PyObject* shapes, int64_t d
                        counts.release(), kept.release());
 }
 
+// The kernels write through addresses: autograd, which has to refuse a backward pass over values that
+// it saved and that are no longer there, is told of it.  Entry i takes no part where it, or the list of
+// gradients' entry i, is None; tensors of inference mode count no versions.
+PyObject* do_written(PyObject* tensors, PyObject* grads) {
+  const Py_ssize_t n = PyList_GET_SIZE(tensors);
+  if (grads && n != PyList_GET_SIZE(grads)) refuse(PyExc_ValueError, "written: lists of different lengths");
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    if (PyList_GET_ITEM(tensors, i) == Py_None || (grads && PyList_GET_ITEM(grads, i) == Py_None)) continue;
+    const at::Tensor& t = tensor_at(tensors, i, "written");
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  }
+  Py_RETURN_NONE;
+}
+
 template <class F>
 PyObject* guarded(F f) {
   try {
@@ -198,8 +213,15 @@ PyObject* pair(PyObject*, PyObject* args) {
   return guarded([&] { return do_pair(params, grads, shapes, device); });
 }
 
+PyObject* written(PyObject*, PyObject* args) {
+  PyObject *tensors, *grads = nullptr;
+  if (!PyArg_ParseTuple(args, "O!|O!", &PyList_Type, &tensors, &PyList_Type, &grads)) return nullptr;
+  return guarded([&] { return do_written(tensors, grads); });
+}
+
 PyMethodDef methods[] = {{"gather", gather, METH_VARARGS, "Pointers, types and counts of a list of tensors."},
                          {"pair", pair, METH_VARARGS, "The same of parameters and their gradients."},
+                         {"written", written, METH_VARARGS, "Marks tensors as modified in place."},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensors", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

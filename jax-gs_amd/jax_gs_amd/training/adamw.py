@@ -182,6 +182,9 @@ class AdamWState:
         """Take over powers that were allocated on the current stream."""
         self.powers, self._powers_stream = powers, _lib.stream_handle(powers.device).value
 
+    def _written(self) -> None:
+        _lib.tensors().written([self.mu_flat, self.nu_flat, self.fields, self.master_flat])
+
     def _views(self, flat):
         return _like(self.keys, [flat[o:o + n].view(s) for o, n, s in zip(self.offsets, self.counts, self.shapes)])
 
@@ -238,6 +241,7 @@ class AdamWState:
         else:
             _lib.call("gs_moments_decode", _lib.stream_handle(dev), self.size, *map(_address, (
                 other.mu_flat, other.nu_flat, other.fields, self.mu_flat, self.nu_flat)))
+        self._written()
 
     def state_dict(self) -> dict:
         """The state as a dict of tensors (the state's own) and plain values, for a checkpoint."""
@@ -370,7 +374,8 @@ class AdamW:
         return float(lr(count)) if callable(lr) else float(lr)
 
     def step(self, params, grads, state: AdamWState, active_mask=None, grad_scale=None) -> AdamWState:
-        """Update the parameters, the moments and the count in place; returns the state.
+        """Update the parameters, the moments and the count in place; returns the state.  As after any
+        in-place operation, autograd refuses a backward pass that needs the values from before.
 
         ``grad_scale`` (one float32 on the device, or a number) multiplies the gradients; when it
         is not finite nothing changes.  Rows whose ``active_mask`` entry is False keep their
@@ -398,6 +403,8 @@ class AdamW:
                   lens, rates.tobytes(), decays.tobytes(), state.bits, state.size, state.mu_flat.data_ptr(),
                   state.nu_flat.data_ptr(), _address(state.fields), _address(state.master_flat), _address(act), rows,
                   _address(scale), state.powers.data_ptr(), powers.data_ptr(), self.b1, self.b2, self.eps, key)
+        _lib.tensors().written(ps, gs)
+        state._written()
         if stream.value != state._powers_stream:
             # read here, and about to be let go of: whoever the allocator gives them to on the stream
             # that they come from waits for this step

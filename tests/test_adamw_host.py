@@ -202,3 +202,57 @@ def test_norms_are_those_of_the_last_step(on_host):
     assert state.norms is not None
     plain.step(ps, ps, state)
     assert state.norms is None
+
+
+@pytest.fixture
+def counting(on_host, module=_lib.tensors):
+    """The module that tells autograd of what was written is the built one."""
+    on_host.written = module().written
+    return on_host
+
+
+def test_autograd_knows_that_a_step_writes(counting):
+    """A graph that saved a parameter's or a master's values from before the step gives no gradient from those after
+    it; one that saved a tensor without a gradient in the step goes on."""
+    opt = AdamW(1e-3, master_weights=True)
+    ps = [torch.randn(300, requires_grad=True), torch.randn(7, requires_grad=True), torch.randn(9).to(torch.bfloat16)]
+    state = opt.init([p.detach() for p in ps])
+    first, second = (ps[0] * ps[0]).sum(), (ps[1] * ps[1]).sum()
+    scale = torch.ones((), requires_grad=True)
+    third = (state.master[2] * scale).sum()
+    opt.step(ps, [torch.zeros(300), None, torch.zeros(9)], state)
+    for y in (first, third):
+        with pytest.raises(RuntimeError, match="inplace operation"):
+            y.backward()
+    second.backward()
+    assert torch.equal(ps[1].grad, 2.0 * ps[1].detach())
+
+
+def test_versions_of_what_a_step_writes(counting):
+    opt = AdamW(1e-3, moment_bits=8)
+    ps = [torch.zeros(300), torch.zeros(7)]
+    state = opt.init(ps)
+    count = lambda: [t._version for t in (*ps, state.mu_flat, state.nu_flat, state.fields)]  # noqa: E731
+    before = count()
+    opt.step(ps, [ps[0], None], state)
+    assert [a - b for a, b in zip(count(), before)] == [1, 0, 1, 1, 1]
+    before = count()
+    state.set_moments(AdamW(1e-3).init(ps))
+    assert [a > b for a, b in zip(count(), before)] == [False, False, True, True, True]
+    with torch.inference_mode():
+        qs = [torch.zeros(300), torch.zeros(7)]
+    opt.step(qs, qs, opt.init(qs))  # they count none
+
+
+def test_a_refused_step_writes_nothing(counting, monkeypatch):
+    opt = AdamW(1e-3)
+    ps = [torch.zeros(300)]
+    state = opt.init(ps)
+
+    def refuse(name, *args):
+        raise ValueError("refused")
+
+    monkeypatch.setattr(_lib, "call", refuse)
+    with pytest.raises(ValueError, match="refused"):
+        opt.step(ps, ps, state)
+    assert ps[0]._version == 0 and state.count == 0

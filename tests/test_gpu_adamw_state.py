@@ -70,3 +70,19 @@ def test_masked_rows_keep_what_the_program_wrote(cuda, bits, dtype, rows, row):
     opt.step([p], [torch.ones(rows, row, device=cuda).to(dtype)], state, active_mask=on)
     assert bool((p[~on] == 3.0).all()) and torch.equal(state.master[0][~on], master[~on])
     assert torch.equal(p[on], state.master[0][on].to(dtype)) and not bool((state.master[0][on] == master[on]).any())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_graph_from_before_the_step_is_refused(cuda, bits):
+    """A graph that saved a parameter would give its gradient with the values after the step."""
+    p, q = (torch.randn(1000, device=cuda, requires_grad=True) for _ in range(2))
+    opt = AdamW(1e-2, moment_bits=bits, max_grad_norm=1.0)
+    state = opt.init([p, q])
+    loss, other = (p * p).sum(), (q * q).sum()
+    opt.step([p, q], [torch.ones_like(p), None], state)
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        loss.backward()
+    other.backward()
+    assert torch.equal(q.grad, 2.0 * q.detach())
+    (p * p).sum().backward()
+    assert torch.equal(p.grad, 2.0 * p.detach())
