@@ -198,3 +198,8 @@ def stream_handle(device: torch.device):
     if _raw_stream is not None and device.index is not None:
         return ctypes.c_void_p(_raw_stream(device.index))
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def capturing(device: torch.device) -> bool:
+    """Whether the calls made now go into a graph instead of running."""
+    return device.type == "cuda" and torch.cuda.is_current_stream_capturing()

@@ -382,6 +382,9 @@ class AdamW:
         parameters and take a zero gradient, whatever theirs holds."""
         ps, gs = _tensors(params, state.keys), _tensors(grads, state.keys)
         k, dev = len(ps), state.mu_flat.device
+        if _lib.capturing(dev):
+            # replays would read powers that the state has let go of, and repeat one step's t and random bits
+            raise RuntimeError("AdamW: a step cannot be captured into a graph")
         to, to_types, of, of_types, counts, kept = _lib.tensors().pair(ps, gs, state.shapes, dev.index)
         mask = None if active_mask is None else _mask(active_mask, ps, dev, "AdamW")
         act, rows, lens = mask or (None, 0, None)

@@ -256,3 +256,16 @@ def test_a_refused_step_writes_nothing(counting, monkeypatch):
     with pytest.raises(ValueError, match="refused"):
         opt.step(ps, ps, state)
     assert ps[0]._version == 0 and state.count == 0
+
+
+def test_a_step_under_graph_capture_is_refused(on_host, monkeypatch):
+    """A captured step holds the addresses of the powers that the state lets go of, one t and one rounding key."""
+    opt = AdamW(1e-3, max_grad_norm=1.0)
+    ps = [torch.zeros(300)]
+    state = opt.init(ps)
+    powers = state.powers
+    made = len(on_host.calls)
+    monkeypatch.setattr(_lib, "capturing", lambda device: True, raising=False)
+    with pytest.raises(RuntimeError, match="captured"):
+        opt.step(ps, ps, state)
+    assert len(on_host.calls) == made and state.powers is powers and state.count == 0 and state.norms is None

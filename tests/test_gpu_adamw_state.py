@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 import torch
 
-from jax_gs_amd.training.adamw import AdamW
+from jax_gs_amd.training.adamw import AdamW, grad_norms
 
 pytestmark = pytest.mark.gpu
 
@@ -86,3 +86,31 @@ def test_a_graph_from_before_the_step_is_refused(cuda, bits):
     assert torch.equal(q.grad, 2.0 * q.detach())
     (p * p).sum().backward()
     assert torch.equal(p.grad, 2.0 * p.detach())
+
+
+def test_a_step_is_not_captured_but_the_norms_are(cuda):
+    """The refusal under a real capture leaves the state as it was; gradient norms are replayed."""
+    p = torch.zeros(5000, device=cuda)
+    g = torch.randn(5000, device=cuda)
+    opt = AdamW(1e-2)
+    state = opt.init([p])
+    opt.step([p], [g], state)
+    grad_norms([g], max_norm=1.0)
+    before = p.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norms = grad_norms([g], max_norm=1.0)
+        with pytest.raises(RuntimeError, match="captured"):
+            opt.step([p], [g], state)
+    assert state.count == 1
+    for k in (1.0, 3.0, 0.5):
+        g.normal_().mul_(k)
+        graph.replay()
+        want = grad_norms([g], max_norm=1.0)
+        torch.cuda.synchronize()
+        assert torch.equal(norms.total, want.total) and torch.equal(norms.scale, want.scale)
+    assert torch.equal(p, before)
+    opt.step([p], [g], state)
+    assert state.count == 2 and not torch.equal(p, before)
+    np.testing.assert_allclose(state.powers.cpu().numpy()[:2], [0.9 ** 2, 0.999 ** 2], rtol=1e-14)
