@@ -235,12 +235,15 @@ class AdamWState:
             for name in ("mu_flat", "nu_flat", "fields"):
                 if getattr(self, name) is not None:
                     getattr(self, name).copy_(getattr(other, name))
-        elif self.bits == 8:
-            _lib.call("gs_moments_encode", _lib.stream_handle(dev), self.size, *map(_address, (
-                other.mu_flat, other.nu_flat, self.mu_flat, self.nu_flat, self.fields)))
         else:
-            _lib.call("gs_moments_decode", _lib.stream_handle(dev), self.size, *map(_address, (
-                other.mu_flat, other.nu_flat, other.fields, self.mu_flat, self.nu_flat)))
+            mu, nu, fields = other.mu_flat, other.nu_flat, other.fields
+            if mu.device != dev:  # the kernels take addresses of their own device
+                mu, nu, fields = (None if x is None else x.to(dev) for x in (mu, nu, fields))
+            s = _lib.stream_handle(dev)
+            if self.bits == 8:
+                _lib.call("gs_moments_encode", s, self.size, *map(_address, (mu, nu, self.mu_flat, self.nu_flat, self.fields)))
+            else:
+                _lib.call("gs_moments_decode", s, self.size, *map(_address, (mu, nu, fields, self.mu_flat, self.nu_flat)))
         self._written()
 
     def state_dict(self) -> dict:

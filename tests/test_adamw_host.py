@@ -269,3 +269,23 @@ def test_a_step_under_graph_capture_is_refused(on_host, monkeypatch):
     with pytest.raises(RuntimeError, match="captured"):
         opt.step(ps, ps, state)
     assert len(on_host.calls) == made and state.powers is powers and state.count == 0 and state.norms is None
+
+
+@pytest.mark.parametrize("bits, entry", [(32, "gs_moments_decode"), (8, "gs_moments_encode")])
+def test_moments_of_a_state_on_another_device(on_host, monkeypatch, bits, entry):
+    """The conversions take addresses of their own device: another device's moments are brought over first."""
+    ps = [torch.zeros(300)]
+    state, other = AdamW(1e-3, moment_bits=bits).init(ps), AdamW(1e-3, moment_bits=40 - bits).init(ps)
+    names = ["mu_flat", "nu_flat"] + (["fields"] if other.bits == 8 else [])
+    brought = {}
+    for name in names:
+        here = getattr(other, name)
+        there = torch.empty_like(here, device="meta")
+        setattr(other, name, there)
+        brought[id(there)] = here
+    to = torch.Tensor.to
+    monkeypatch.setattr(torch.Tensor, "to", lambda t, *a: brought[id(t)] if t.is_meta else to(t, *a))
+    state.set_moments(other)
+    name, args = on_host.calls[-1]
+    assert name == entry
+    assert list(args[2:2 + len(names)]) == [t.data_ptr() for t in brought.values()] and all(args[2:])
