@@ -5,7 +5,7 @@
 //
 //   gather(tensors, device, what)                  -> (pointers, types, counts, kept)
 //   pair(params, grads, shapes, device)            -> (to, to_types, of, of_types, counts, kept)
-//   written(tensors, grads)                        -> None: marks as modified in place what a call wrote
+//   written(tensors, grads, others)                -> None: marks as modified in place what a call wrote
 //
 // The first three (five) are bytes objects holding int64 pointers, int32 types and int64 element
 // counts.  A None among the tensors (gradients) has pointer 0 and count 0.  A tensor that is not
@@ -172,16 +172,19 @@ PyObject* do_pair(PyObject* params, PyObject* grads, PyObject* shapes, int64_t d
 }
 
 // The kernels write through addresses: autograd, which has to refuse a backward pass over values that
-// it saved and that are no longer there, is told of it.  Entry i takes no part where it, or the list of
-// gradients' entry i, is None; tensors of inference mode count no versions.
-PyObject* do_written(PyObject* tensors, PyObject* grads) {
-  const Py_ssize_t n = PyList_GET_SIZE(tensors);
-  if (grads && n != PyList_GET_SIZE(grads)) refuse(PyExc_ValueError, "written: lists of different lengths");
-  for (Py_ssize_t i = 0; i < n; ++i) {
-    if (PyList_GET_ITEM(tensors, i) == Py_None || (grads && PyList_GET_ITEM(grads, i) == Py_None)) continue;
-    const at::Tensor& t = tensor_at(tensors, i, "written");
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-  }
+// it saved and that are no longer there, is told of it.  Tensors without a gradient take no part, nor
+// does a None among the others; tensors of inference mode count no versions.
+void mark(PyObject* list, Py_ssize_t i) {
+  const at::Tensor& t = tensor_at(list, i, "written");
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+PyObject* do_written(PyObject* tensors, PyObject* grads, PyObject* others) {
+  if (PyList_GET_SIZE(tensors) != PyList_GET_SIZE(grads)) refuse(PyExc_ValueError, "written: lists of different lengths");
+  for (Py_ssize_t i = 0; i < PyList_GET_SIZE(tensors); ++i)
+    if (PyList_GET_ITEM(grads, i) != Py_None) mark(tensors, i);
+  for (Py_ssize_t i = 0; i < PyList_GET_SIZE(others); ++i)
+    if (PyList_GET_ITEM(others, i) != Py_None) mark(others, i);
   Py_RETURN_NONE;
 }
 
@@ -214,9 +217,9 @@ PyObject* pair(PyObject*, PyObject* args) {
 }
 
 PyObject* written(PyObject*, PyObject* args) {
-  PyObject *tensors, *grads = nullptr;
-  if (!PyArg_ParseTuple(args, "O!|O!", &PyList_Type, &tensors, &PyList_Type, &grads)) return nullptr;
-  return guarded([&] { return do_written(tensors, grads); });
+  PyObject *tensors, *grads, *others;
+  if (!PyArg_ParseTuple(args, "O!O!O!", &PyList_Type, &tensors, &PyList_Type, &grads, &PyList_Type, &others)) return nullptr;
+  return guarded([&] { return do_written(tensors, grads, others); });
 }
 
 PyMethodDef methods[] = {{"gather", gather, METH_VARARGS, "Pointers, types and counts of a list of tensors."},

@@ -182,9 +182,6 @@ class AdamWState:
         """Take over powers that were allocated on the current stream."""
         self.powers, self._powers_stream = powers, _lib.stream_handle(powers.device).value
 
-    def _written(self) -> None:
-        _lib.tensors().written([self.mu_flat, self.nu_flat, self.fields, self.master_flat])
-
     def _views(self, flat):
         return _like(self.keys, [flat[o:o + n].view(s) for o, n, s in zip(self.offsets, self.counts, self.shapes)])
 
@@ -244,7 +241,7 @@ class AdamWState:
                 _lib.call("gs_moments_encode", s, self.size, *map(_address, (mu, nu, self.mu_flat, self.nu_flat, self.fields)))
             else:
                 _lib.call("gs_moments_decode", s, self.size, *map(_address, (mu, nu, fields, self.mu_flat, self.nu_flat)))
-        self._written()
+        _lib.tensors().written([], [], [self.mu_flat, self.nu_flat, self.fields])
 
     def state_dict(self) -> dict:
         """The state as a dict of tensors (the state's own) and plain values, for a checkpoint."""
@@ -388,7 +385,8 @@ class AdamW:
         if _lib.capturing(dev):
             # replays would read powers that the state has let go of, and repeat one step's t and random bits
             raise RuntimeError("AdamW: a step cannot be captured into a graph")
-        to, to_types, of, of_types, counts, kept = _lib.tensors().pair(ps, gs, state.shapes, dev.index)
+        native = _lib.tensors()
+        to, to_types, of, of_types, counts, kept = native.pair(ps, gs, state.shapes, dev.index)
         mask = None if active_mask is None else _mask(active_mask, ps, dev, "AdamW")
         act, rows, lens = mask or (None, 0, None)
         scale = _scalar(grad_scale, dev, "AdamW")
@@ -409,8 +407,7 @@ class AdamW:
                   lens, rates.tobytes(), decays.tobytes(), state.bits, state.size, state.mu_flat.data_ptr(),
                   state.nu_flat.data_ptr(), _address(state.fields), _address(state.master_flat), _address(act), rows,
                   _address(scale), state.powers.data_ptr(), powers.data_ptr(), self.b1, self.b2, self.eps, key)
-        _lib.tensors().written(ps, gs)
-        state._written()
+        native.written(ps, gs, [state.mu_flat, state.nu_flat, state.fields, state.master_flat])
         if stream.value != state._powers_stream:
             # read here, and about to be let go of: whoever the allocator gives them to on the stream
             # that they come from waits for this step
