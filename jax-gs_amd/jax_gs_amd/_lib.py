@@ -202,4 +202,7 @@ def stream_handle(device: torch.device):
 
 def capturing(device: torch.device) -> bool:
     """Whether the calls made now go into a graph instead of running."""
-    return device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+    # the default stream, handle 0, cannot be captured: 0.1 us instead of 0.3
+    if device.index is None or (_raw_stream is not None and _raw_stream(device.index) == 0):
+        return False
+    return torch.cuda.is_current_stream_capturing()

@@ -101,7 +101,7 @@ def _scalar(grad_scale, dev, what: str):
         return torch.full((), float(grad_scale), device=dev)
     if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != dev:
         raise ValueError(f"{what}: grad_scale must be one float32 on {dev}")
-    return grad_scale.resolve_neg()
+    return grad_scale.resolve_neg() if grad_scale.is_neg() else grad_scale
 
 
 def _address(t: Optional[torch.Tensor]):
@@ -220,28 +220,32 @@ class AdamWState:
         to.bits, to.norms = bits, None
         to.master_flat = None if self.master_flat is None else self.master_flat.clone()
         to._allocate(self.mu_flat.device, zero=False)
-        to.set_moments(self)
+        to._take(self.bits, self.mu_flat, self.nu_flat, self.fields)
         return to
 
     def set_moments(self, other: "AdamWState") -> None:
         """Take over another state's moments (of the same tensors), to nearest."""
         if other.shapes != self.shapes:
             raise ValueError("AdamWState.set_moments: states of different tensors")
-        dev = self.mu_flat.device
-        if self.bits == other.bits:
-            for name in ("mu_flat", "nu_flat", "fields"):
-                if getattr(self, name) is not None:
-                    getattr(self, name).copy_(getattr(other, name))
-        else:
-            mu, nu, fields = other.mu_flat, other.nu_flat, other.fields
-            if mu.device != dev:  # the kernels take addresses of their own device
-                mu, nu, fields = (None if x is None else x.to(dev) for x in (mu, nu, fields))
-            s = _lib.stream_handle(dev)
-            if self.bits == 8:
-                _lib.call("gs_moments_encode", s, self.size, *map(_address, (mu, nu, self.mu_flat, self.nu_flat, self.fields)))
-            else:
-                _lib.call("gs_moments_decode", s, self.size, *map(_address, (mu, nu, fields, self.mu_flat, self.nu_flat)))
+        given, dev = (other.mu_flat, other.nu_flat, other.fields), self.mu_flat.device
+        if other.mu_flat.device != dev:  # the kernels take addresses of their own device
+            given = [None if x is None else x.to(dev) for x in given]
+        self._take(other.bits, *given)
         _lib.tensors().written([], [], [self.mu_flat, self.nu_flat, self.fields])
+
+    def _take(self, bits: int, mu, nu, fields) -> None:
+        """Moments in ``bits`` on this device, laid out as these, into this state's."""
+        dev = self.mu_flat.device
+        if self.bits == bits:
+            for own, given in ((self.mu_flat, mu), (self.nu_flat, nu), (self.fields, fields)):
+                if own is not None:
+                    own.copy_(given)
+        elif self.bits == 8:
+            _lib.call("gs_moments_encode", _lib.stream_handle(dev), self.size, *map(_address, (
+                mu, nu, self.mu_flat, self.nu_flat, self.fields)))
+        else:
+            _lib.call("gs_moments_decode", _lib.stream_handle(dev), self.size, *map(_address, (
+                mu, nu, fields, self.mu_flat, self.nu_flat)))
 
     def state_dict(self) -> dict:
         """The state as a dict of tensors (the state's own) and plain values, for a checkpoint."""
