@@ -12,7 +12,7 @@ import pytest
 import torch
 
 import adamw_reference as ref
-from jax_gs_amd.training.adamw import AdamW
+from jax_gs_amd.training.adamw import AdamW, grad_norms
 from test_gpu_adamw import SIZES, TYPES, check32, check8, rows_like, run32, tensors, weights_close
 
 pytestmark = pytest.mark.gpu
@@ -304,3 +304,23 @@ def test_both_entries_of_the_training_step_are_one_path(cuda, monkeypatch):
         trainer.train_step(state, tgt, w2c, static, opt, sh_degree=3, fused=fused)
         assert state.opt_state.count == 1
     assert len(taken) == 2
+
+
+def test_a_norm_beyond_float32_still_clips(cuda):
+    """The sums are float64: 100 gradients of 2e38 have the norm 2e39, which float32 does not hold, and a factor of
+    5e-40, which it holds to half of 2^-149.  The step is made; gradients that are not finite make none."""
+    g = torch.full((100,), 2e38, device=cuda)
+    norms = grad_norms([g], max_norm=1.0)
+    assert float(norms.total) == float("inf") == float(norms.per_tensor[0])
+    want = 1.0 / (float(g[0].double()) * 10.0)
+    assert abs(float(norms.scale.double()) - want) <= 2.0 ** -150
+    p = torch.zeros(100, device=cuda)
+    opt = AdamW(1e-2, max_grad_norm=1.0)
+    state = opt.init([p])
+    opt.step([p], [g], state)
+    # g * scale: half of 2^-149 of 5e-40, 1.5e-6, and one rounding; three more in m
+    np.testing.assert_allclose(np64(state.mu[0]), 0.1 * np64(g) * want, rtol=2e-6)
+    before = p.clone()
+    g[3] = float("inf")
+    opt.step([p], [g], state)
+    assert torch.equal(p, before) and bool(p.lt(0).all()) and torch.isnan(state.norms.scale)
