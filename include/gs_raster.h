@@ -534,7 +534,8 @@ size_t gs_grad_norms_workspace_size(int num, const int64_t* counts);
 /* The 2-norm of each of num gradients (norms[num], may be NULL) and out[2] = {the norm of them
  * all, the factor that clips}: s min(1, max_norm / (norm + 1e-6)) with s = grad_scale[0] (device
  * scalar, NULL for 1; the norms are those of s times the gradients), s itself when max_norm <= 0,
- * NaN when the norm is not finite.  grads, grad_types (GS_TYPE_*), counts and row_lens are host
+ * NaN when a gradient or s is not finite.  (A norm beyond float32's range is returned as infinity;
+ * the factor, from the float64 norm, is then finite.)  grads, grad_types (GS_TYPE_*), counts and row_lens are host
  * arrays, grads of device pointers aligned to their type.  With active (device, rows bytes) every
  * tensor has rows x row_lens[i] elements, and rows whose byte is 0 are left out whatever they
  * hold.  Sums are float64 in a fixed order.  workspace: 8-byte aligned. */
@@ -552,11 +553,12 @@ int gs_grad_norms(void* stream, int num, const void* const* grads, const int* gr
  * GS_MOMENT_BLOCK) on, each tensor in blocks of its own, in the order of the tensors.  moment_bits 32: mu, nu are float32 (m
  * and v), fields NULL.  moment_bits 8: mu, nu are bytes and fields holds two bytes per block
  * (see gs_moments_encode), rounded stochastically by a hash of the element's place and key,
- * which the caller changes from step to step.  Elements between tensors are left alone or
- * written as zero.  master (may be NULL): float32 weights of half-typed tensors, flat as the
+ * which the caller changes from step to step.  Elements between tensors must be zero, and stay so:
+ * they are read, and in 8 bits count towards their block's maximum.  master (may be NULL): float32 weights of half-typed tensors, flat as the
  * moments; they are updated and the tensor gets their rounded value.
  * powers (device, four doubles): b1^(t-1), b2^(t-1), 1 / (1 - b1^t), 1 / sqrt(1 - b2^t);
- * powers_next, another four, receives those of the next step.
+ * powers_next, another four, receives those of the next step.  (A graph that captures the call repeats it
+ * with the same powers, powers_next and key.)
  * Host arrays: params, grads (device pointers; a NULL gradient leaves tensor i alone),
  * param_types, grad_types, offsets, counts, row_lens (NULL without active), lrs, decays. */
 int gs_adamw_step(void* stream, int num, void* const* params, const int* param_types, const void* const* grads,

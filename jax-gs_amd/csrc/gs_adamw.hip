@@ -16,11 +16,12 @@
 // The tensor is found by one comparison per lane and a ballot.
 //
 // One pass over memory, which bounds it: 28 B an element with float32 everywhere, 16 B with 8-bit
-// moments; a large copy reaches 5.2 TB/s.  Measured: 59M float32 elements 260 us in 32 bits (6.3
+// moments; a large copy reaches 5.1 TB/s.  Measured: 59M float32 elements 260 us in 32 bits (6.3
 // TB/s), 152 us in 8 bits (6.2 TB/s; 257 vector instructions a wave, which would take 110 us by
 // themselves and are what bounds bfloat16 weights and gradients, 128 us for 10 B an element);
 // 2.1M Gaussians (124M elements, 40 % of the rows masked) in 32 bits 487 us; 3M (177M, 20 %
-// masked) in 8 bits 462 us.  The smallest call takes 4.4 us, five dependent reads.
+// masked) in 8 bits 462 us; 59M half weights and gradients without masters in 32 bits 203 us (6.4
+// TB/s, either type).  The smallest call takes 4.4 us, five dependent reads.
 #include "gs_moments.h"
 #include "gs_pieces.h"
 #include "gs_rows.h"

@@ -168,7 +168,7 @@ __device__ inline void encode_block(const float (&m)[4], const float (&r)[4], co
 }
 
 // Correctly rounded roots of four values v >= 0.  The hardware's reciprocal root and one
-// correction from the exact residual give the rounded root of every float from 2^-100 on (all
+// Newton step from the exact residual (s + (v - s^2) / (2 s), s = v times that) give the rounded root of every float from 2^-100 on (all
 // 1.9e9 of them compared with the compiler's sequence); a lane with smaller ones, whose residual
 // would underflow, or with one that is not finite takes that sequence.
 __device__ inline void roots4(const float (&v)[4], float (&r)[4]) {
@@ -189,9 +189,10 @@ __device__ inline void roots4(const float (&v)[4], float (&r)[4]) {
   }
 }
 
-// 32 hashed bits of an element's place in the state: a Weyl step, one multiplication by an
-// odd constant between two shifts.  key holds the seed and the step.  The element is block + j
-// with block a multiple of 256 that is the same for the wave and j < 256.
+// 32 hashed bits of an element's place in the state: a Weyl step by a prime near 2^32 over the
+// golden ratio, then one multiplication by an odd constant between two shifts, the usual finish of
+// integer hashes; the multipliers are known ones of such hashes.  key holds the seed and the step.
+// The element is block + j with block a multiple of 256 that is the same for the wave and j < 256.
 __device__ inline uint32_t place_hash(int64_t block, uint32_t j, uint32_t key) {
   const uint32_t x = (uint32_t)block + (uint32_t)((uint64_t)block >> 32) * 0x632be5abu;
   uint32_t h = j * 0x9e3779b1u + (x * 0x9e3779b1u + key);

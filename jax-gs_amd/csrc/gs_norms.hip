@@ -1,13 +1,15 @@
 // Norms of many gradients at once, and the factor that clips them, on gfx950.
 //
 //   n_k = |s| sqrt(sum_i g_ki^2),   n = sqrt(sum_k n_k^2),
-//   scale = s min(1, c / (n + 1e-6))   (s without c; NaN unless n is finite),
+//   scale = s min(1, c / (n + 1e-6))   (s without c; NaN unless the float64 n is finite, that is
+//                                       unless s and every gradient are),
 // s a device scalar (a loss scale's inverse) or 1.  Rows whose mask is 0 are left out, whatever
 // they hold.  Squares and sums are float64: no square of a float32 overflows or vanishes there,
 // and the order of the sums, which is fixed, does not show in the float32 results.
 //
-// Every workgroup sums one run of consecutive elements of one tensor (the runs' length is chosen
-// so that about 2048 of them cover all tensors) into one partial sum; a second launch of one
+// Every workgroup sums one run of consecutive elements of one tensor into one partial sum (runs are
+// the multiple of 8192 elements with which at most 2048 whole ones cover all tensors: for large lists
+// 1025 to 2048 of them); a second launch of one
 // workgroup adds the partial sums of each tensor and the tensors' sums.  Reading bounds the first:
 // 59M float32 44 us (5.3 TB/s), 148 bfloat16 tensors of 22M elements 13 us, 124M float32 under a
 // mask 110 us (150 us behind a step, whose dirty lines are written back meanwhile); the second

@@ -32,8 +32,8 @@ BLOCK = 256  # elements that share an exponent in 8 bits; each tensor's moments 
 
 
 class GradNorms:
-    """Device float32: ``total``, the norm of all gradients; ``per_tensor``, each one's; ``scale``,
-    the factor for the step."""
+    """Device float32: ``total``, the norm of all gradients; ``per_tensor``, each one's (infinite beyond
+    float32's range); ``scale``, the factor for the step."""
     __slots__ = ("_out", "_k")
 
     def __init__(self, out: torch.Tensor, k: int):
@@ -123,7 +123,8 @@ def _norms(dev, k: int, pointers: bytes, types: bytes, counts: bytes, mask, max_
 def grad_norms(grads, max_norm: Optional[float] = None, active_mask=None, grad_scale=None) -> GradNorms:
     """2-norms of grad_scale times the gradients, per tensor and of all, and the factor
     ``grad_scale * min(1, max_norm / (total + 1e-6))`` (``grad_scale`` without ``max_norm``),
-    NaN when the total is not finite, all on the device.  Rows where ``active_mask`` is False
+    NaN when a gradient or ``grad_scale`` is not finite, all on the device (the sums are float64, so
+    that a norm beyond float32's range still clips).  Rows where ``active_mask`` is False
     are left out, whatever they hold; ``None`` gradients count as empty."""
     if max_norm is not None and not max_norm > 0.0:
         raise ValueError(f"grad_norms: max_norm must be positive, not {max_norm}")
@@ -263,7 +264,7 @@ class AdamW:
     follow from ``seed``, the step and the element.  ``master_weights`` keeps float32 weights of
     half-typed parameters in the state.  With ``max_grad_norm`` every step takes the gradients'
     norm first (``state.norms``), scales them down to it, and leaves everything as it is when
-    it is not finite."""
+    some gradient is not finite."""
 
     def __init__(self, learning_rates, b1: float = 0.9, b2: float = 0.999, eps: float = 1e-8, weight_decay=0.0,
                  moment_bits: int = 32, master_weights: bool = False, max_grad_norm: Optional[float] = None,
@@ -336,7 +337,8 @@ class AdamW:
 
     def restore(self, params, mu, nu, count: int, master=None) -> AdamWState:
         """The state after ``count`` updates from first and second moments in 32 bits given
-        tensor by tensor (an ``AdamState``'s ``mu`` and ``nu``, for one)."""
+        tensor by tensor (an ``AdamState``'s ``mu`` and ``nu``, for one), and float32 masters if the
+        optimizer keeps them (the parameters' values where none are given)."""
         full = self._state(params, 32)
         ps = _tensors(params)
         full._allocate(ps[0].device, zero=True)

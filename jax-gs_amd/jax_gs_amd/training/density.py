@@ -78,7 +78,8 @@ def densify_and_prune(state: DensityState, generator: Optional[torch.Generator] 
     opt = state.opt_state
     if opt is not None:
         # 8-bit moments are moved in 32 bits: what they stand for comes back unchanged, but where a
-        # row that moved in has raised the exponent of its block
+        # row that moved in has raised the exponent of its block.  Both forms are live meanwhile: 10 B
+        # an element next to the 8 of moments in 32 bits
         wide = opt.convert(32) if getattr(opt, "bits", 32) == 8 else opt
         mu, nu = wide.mu, wide.nu
         moments = [mu[f] for f in FIELDS] + [nu[f] for f in FIELDS]

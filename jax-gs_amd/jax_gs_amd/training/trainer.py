@@ -65,8 +65,8 @@ def train_step(state, target_image, w2c, camera_static, optimizer, fast_tpu_rast
     rasterizer's VJP, then one kernel for the preprocessing VJP, the statistics and the
     Adam update (no parameter gradient reaches memory).  fused=False builds the same
     step from ``render``'s autograd, ``accumulate_from_extras`` and ``Adam.step``.  An
-    ``AdamW`` optimizer needs the gradients whole (their norm comes before the update) and
-    always takes that form; metrics["grad_norm"] is the norm it clipped."""
+    ``AdamW`` optimizer always takes that form (to clip, it needs the gradients whole; the one
+    kernel updates by ``Adam`` only); metrics["grad_norm"] is the norm it clipped."""
     W, H, fx, fy, cx, cy = camera_static
     params = state.gaussians
     dev = params.means.device
