@@ -118,31 +118,34 @@ __device__ inline void store_codes(void* p, int64_t at, uint32_t x) {
 // Whole blocks know their types, so that all loads are on their way before the first wait.
 template <bool kStream, class P, class G, bool kMaster>
 struct WholeBlock {
+  typedef P params __attribute__((ext_vector_type(4), aligned(sizeof(P))));
   const G* grad;
   P* param;
   float* master;
   bool stream_params;
+  params old;  // of a lane with masters and some of its four masked
   __device__ WholeBlock(const StepArgs& A, const StepTensor& t, int64_t base)
       : grad((const G*)t.grad + base), param((P*)t.param + base), master(A.master + t.at + base),
         stream_params(A.stream_params) {}
   __device__ int n(uint32_t) const { return 4; }
-  __device__ void load(uint32_t l4, float (&g)[4], float (&w)[4]) const {
+  // on: which of the four are not masked.
+  __device__ void load(uint32_t l4, float (&g)[4], float (&w)[4], uint32_t on) {
     load4<kStream>(grad + l4, g);
     if (kMaster) load4<kStream>(master + l4, w);
     else load4<kStream>((const P*)param + l4, w);
+    if (kMaster && on != 15u) old = *reinterpret_cast<const params*>(param + l4);
   }
-  // on: which of the four to store.  Without masters the others are what was read from there.
+  // The masked of the four are stored as what was read from there.  With masters that is one more
+  // read, which takes less than storing the others one by one (30M bfloat16 with masters, 40 % of the
+  // elements masked, 32 and 8 bits: 138 and 98 us, one by one 166 and 118).
   __device__ void store(uint32_t l4, const float (&w)[4], uint32_t on) const {
     if (kMaster && on != 15u) {
+      params v = old;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (on >> j & 1u) {
-          param[l4 + j] = (P)w[j];
-          master[l4 + j] = w[j];
-        }
-      return;
-    }
-    if (kStream && stream_params) {
+        if (on >> j & 1u) v[j] = (P)w[j];
+      *reinterpret_cast<params*>(param + l4) = v;
+    } else if (kStream && stream_params) {
       asm volatile("");  // keeps the compiler from merging the two stores into one of the second kind
       store4<true>(param + l4, w);
       asm volatile("");
@@ -180,7 +183,7 @@ struct PartBlock {
     if (type == GS_TYPE_BF16) return bits_to_float(x << 16);
     return (float)__builtin_bit_cast(_Float16, (uint16_t)x);
   }
-  __device__ void load(uint32_t l4, float (&g)[4], float (&w)[4]) const {
+  __device__ void load(uint32_t l4, float (&g)[4], float (&w)[4], uint32_t) const {
     uint32_t a[4], b[4];
     raw(grad, base, gtype == GS_TYPE_F32, l4, a);
     raw(master ? (const void*)master : param, master ? 0 : base, master || ptype == GS_TYPE_F32, l4, b);
@@ -211,7 +214,7 @@ __device__ inline void step_block(const StepArgs& A, const StepTensor& t, int64_
                                   double r2d) {
   const uint32_t l4 = (threadIdx.x & 63u) * 4u;
   const int64_t at = t.at + base;
-  const Block io(A, t, base);
+  Block io(A, t, base);
   float w[4] = {0.0f, 0.0f, 0.0f, 0.0f}, g[4] = {0.0f, 0.0f, 0.0f, 0.0f}, m[4], r[4], v[4];
   uint32_t m8 = 0, r8 = 0, f = 0;
   if (k8) {
@@ -224,7 +227,7 @@ __device__ inline void step_block(const StepArgs& A, const StepTensor& t, int64_
   }
   // masked rows: neither gradient nor parameter is read or written
   const uint32_t on = kMask ? rows_on<4>(A.active, t.magic, t.row_len, base, l4, io.n(l4)) : 15u;
-  if (!kMask || on) io.load(l4, g, w);
+  if (!kMask || on) io.load(l4, g, w, on);
   if (k8 && !is_finite(scale)) return;
   const float r1 = (float)r1d, r2 = (float)r2d;
   if (k8) {
