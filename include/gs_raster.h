@@ -92,7 +92,9 @@ const char* gs_last_error(void);
  * gs_preprocess_bwd_w2c take zeroed.  Added since, with every call of 14 as it was:
  * gs_composite_segments_size, gs_composite_segments_size_for, gs_composite_fwd_seg,
  * gs_composite_bwd_seg; gs_l1_ssim_loss, gs_l1_ssim_loss_bwd; gs_grad_norms_workspace_size, gs_grad_norms,
- * gs_adamw_step, gs_moments_encode, gs_moments_decode. */
+ * gs_adamw_step, gs_moments_encode, gs_moments_decode; gs_clip_grads, gs_take_rows, gs_move_rows,
+ * gs_moments_take, gs_moments_move_workspace_size, gs_moments_move, gs_best_rows_workspace_size,
+ * gs_best_rows, gs_densify_sources. */
 int gs_abi_version(void);
 
 /* Projection + covariance + SH colour for every Gaussian.
@@ -543,6 +545,13 @@ int gs_grad_norms(void* stream, int num, const void* const* grads, const int* gr
                   const int64_t* row_lens, const uint8_t* active, int64_t rows, double max_norm,
                   const float* grad_scale, void* workspace, size_t workspace_bytes, float* norms, float* out);
 
+/* gs_grad_norms, and every gradient times the factor out[1], in place, rounded once to its type;
+ * rows whose mask is 0 keep what they hold, and everything does when the factor is not finite.
+ * The gradients do not overlap. */
+int gs_clip_grads(void* stream, int num, void* const* grads, const int* grad_types, const int64_t* counts,
+                  const int64_t* row_lens, const uint8_t* active, int64_t rows, double max_norm,
+                  const float* grad_scale, void* workspace, size_t workspace_bytes, float* norms, float* out);
+
 /* One AdamW step, in place, of num tensors of any sizes and of types GS_TYPE_* (gradients of
  * types of their own).  Per element, g = s * gradient (0 in rows whose mask is 0),
  *   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,
@@ -578,6 +587,47 @@ int gs_moments_encode(void* stream, int64_t state_size, const float* mu, const f
 int gs_moments_decode(void* stream, int64_t state_size, const uint8_t* mu8, const uint8_t* nu8,
                       const uint8_t* fields, float* mu, float* nu);
 
+/* Rows of num tensors by one index: row i of out[k] is row index[i] of tensors[k], for an index
+ * outside [0, rows) the row fills[k] (device pointers, fills and any of them may be NULL: zeros).
+ * Rows are bytes: row_bytes[k] of them one after another, strides[k] from row to row of tensors[k];
+ * out[k] is 16-byte aligned, its count rows lie one behind the other, and out_bytes[k] >= count *
+ * row_bytes[k] (NULL: equal) are written, zeros behind the rows.  index: device, count entries of
+ * index_bits 32 or 64.  Outputs overlap nothing else. */
+int gs_take_rows(void* stream, int num, const void* const* tensors, const int64_t* row_bytes,
+                 const int64_t* strides, int64_t rows, void* const* out, const int64_t* out_bytes,
+                 const void* const* fills, const void* index, int index_bits, int64_t count);
+
+/* The same in place: row i of every tensor becomes its row index[i] where index[i] != i, the row
+ * fills[k] where index[i] < 0.  A source is a row that stays (index[index[i]] = index[i]); a row
+ * whose index asks for another, or for one beyond the rows, stays too and is counted in left[0]
+ * (device, may be NULL, added to).  The tensors do not overlap each other or the index. */
+int gs_move_rows(void* stream, int num, void* const* tensors, const int64_t* row_bytes, const int64_t* strides,
+                 int64_t rows, const void* const* fills, const void* index, int index_bits, int32_t* left);
+
+/* gs_take_rows of moments in 8 bits (gs_moments_encode's arrays): tensor k has rows of row_lens[k]
+ * elements from offsets[k] on in the state of state_size elements and from out_offsets[k] on in the new one
+ * of out_size, both multiples of GS_MOMENT_BLOCK and tensors in order.  Blocks are encoded anew, to
+ * nearest even; elements of the last block behind the rows become zero, blocks between tensors are not written. */
+int gs_moments_take(void* stream, int num, const int64_t* row_lens, int64_t rows, const int64_t* offsets,
+                    int64_t state_size, const uint8_t* mu8, const uint8_t* nu8, const uint8_t* fields,
+                    const void* index, int index_bits, int64_t count, const int64_t* out_offsets,
+                    int64_t out_size, uint8_t* out_mu8, uint8_t* out_nu8, uint8_t* out_fields);
+
+/* gs_move_rows of moments in 8 bits; freed rows become zero.  workspace: 16-byte aligned, of
+ * gs_moments_move_workspace_size(state_size) bytes. */
+size_t gs_moments_move_workspace_size(int64_t state_size);
+int gs_moments_move(void* stream, int num, const int64_t* row_lens, int64_t rows, const int64_t* offsets,
+                    int64_t state_size, uint8_t* mu8, uint8_t* nu8, uint8_t* fields, const void* index,
+                    int index_bits, void* workspace, size_t workspace_bytes);
+
+/* The rows with the k largest of `rows` scores (of type GS_TYPE_*; NULL: all alike) among those
+ * whose byte of active (may be NULL) is not 0: out[k] holds their numbers, ascending, and -1 behind
+ * them where there are fewer.  Of equal scores the lowest rows come first; -0 equals +0, and NaN
+ * is below every number.  workspace: gs_best_rows_workspace_size(rows) bytes, 4-byte aligned. */
+size_t gs_best_rows_workspace_size(int64_t rows);
+int gs_best_rows(void* stream, int64_t rows, const void* scores, int type, const uint8_t* active, int64_t k,
+                 void* workspace, size_t workspace_bytes, int32_t* out);
+
 /* Workspace bytes of gs_densify_and_prune for a capacity of M Gaussians. */
 size_t gs_densify_workspace_size(int64_t capacity);
 
@@ -601,6 +651,12 @@ int gs_densify_and_prune(void* stream, int64_t capacity, int sh_k, float* means,
                          double grad_threshold, double min_opacity, double extent,
                          double max_screen_size, void* workspace, size_t workspace_bytes,
                          int32_t* counts);
+
+/* After gs_densify_and_prune with this workspace and counts (as given there): sources[i] is the slot
+ * whose rows slot i holds since, i itself unless it was filled -- the index of gs_move_rows for
+ * whatever else moves with the Gaussians. */
+int gs_densify_sources(void* stream, int64_t capacity, const void* workspace, size_t workspace_bytes,
+                       const int32_t* counts, int32_t* sources);
 
 /* opacities[i] = log(reset_value / (1 - reset_value)) where active[i] (in place).
  * Replaces jax_gs/training/density.py:69-93 (reset_opacities). */

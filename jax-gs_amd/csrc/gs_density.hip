@@ -178,6 +178,24 @@ __global__ __launch_bounds__(kDenBlock) void density_route_kernel(
   denom[i] = 0;
 }
 
+// Which Gaussian each slot holds the rows of after the moves: the source of a filled slot, else its own.
+// The flags and the workgroups' offsets are those that the routing used.
+__global__ __launch_bounds__(kDenBlock) void density_sources_kernel(
+    int64_t M, const uint8_t* __restrict__ flags, const int32_t* __restrict__ boff, const int32_t* __restrict__ ctl,
+    const int32_t* __restrict__ clone_src, const int32_t* __restrict__ split_src, int32_t* __restrict__ sources) {
+  __shared__ int wcnt[kDenBlock / 64];
+  const int64_t i = (int64_t)blockIdx.x * kDenBlock + threadIdx.x;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const bool is_empty = i < M && !(flags[i] & kAfter);
+  const uint64_t be = __ballot(is_empty);
+  if (lane == 0) wcnt[w] = __popcll(be);
+  __syncthreads();
+  const int r = boff[(int64_t)blockIdx.x * 4] + block_rank(is_empty, wcnt, 0, lane, w);
+  if (i >= M) return;
+  const int nc = ctl[0], ns = ctl[1];
+  sources[i] = !is_empty || r >= nc + ns ? (int32_t)i : r >= nc ? split_src[r - nc] : clone_src[r];
+}
+
 // Filled slot of rank r (the r-th empty slot) takes a copy of its source.  Work item
 // (r, j) copies value j of the slot's concatenated rows (every array, row after row),
 // so consecutive threads copy consecutive values of one row; the grid strides over
@@ -337,6 +355,22 @@ extern "C" int gs_densify_and_prune(void* stream, int64_t capacity, int sh_k, fl
   hipLaunchKernelGGL(density_split_kernel, dim3(1024), dim3(256), 0, s, means, scales, dest_slot, split_src, ctl,
                      noise, P.log16);
   GS_LAUNCH_CHECK("density_split_kernel");
+  return GS_OK;
+}
+
+extern "C" int gs_densify_sources(void* stream, int64_t capacity, const void* workspace, size_t workspace_bytes,
+                                  const int32_t* counts, int32_t* sources) {
+  GS_REQUIRE(capacity > 0 && capacity < ((int64_t)1 << 31), "gs_densify_sources: capacity out of range");
+  GS_REQUIRE(workspace && sources, "gs_densify_sources: NULL argument");
+  const DenLayout L = den_layout(capacity);
+  GS_REQUIRE(workspace_bytes >= L.total, "gs_densify_sources: workspace of %zu bytes, %zu needed", workspace_bytes,
+             L.total);
+  const char* ws = (const char*)workspace;
+  hipLaunchKernelGGL(density_sources_kernel, dim3((unsigned)L.nb), dim3(kDenBlock), 0, (hipStream_t)stream, capacity,
+                     (const uint8_t*)(ws + L.flags), (const int32_t*)(ws + L.bcount),
+                     counts ? counts : (const int32_t*)(ws + L.ctl), (const int32_t*)(ws + L.clone_src),
+                     (const int32_t*)(ws + L.split_src), sources);
+  GS_LAUNCH_CHECK("density_sources_kernel");
   return GS_OK;
 }
 

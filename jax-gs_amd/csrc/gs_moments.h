@@ -77,26 +77,34 @@ __device__ inline uint32_t moment_top(float x, int field, uint32_t noise) {
 __device__ inline uint32_t noise_hi(uint32_t h) { return __builtin_amdgcn_perm(0, h, 0x0c03020cu); }
 __device__ inline uint32_t noise_lo(uint32_t h) { return __builtin_amdgcn_perm(0, h, 0x0c01000cu); }
 
-// Four decoded values of the packed codes w of one lane; field as stored.  The signed code is the
-// machine's own 8-bit float (bias 7, the same "not finite" code).
-__device__ inline void decode_m4(uint32_t w, int field, float (&m)[4]) {
+// Four decoded values of the packed codes w of one lane; fields as stored, one for each value.  The
+// signed code is the machine's own 8-bit float (bias 7, the same "not finite" code).
+__device__ inline void decode_m4(uint32_t w, const int (&field)[4], float (&m)[4]) {
   const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
-  m[0] = ldexpf(a[0], field - 135);
-  m[1] = ldexpf(a[1], field - 135);
-  m[2] = ldexpf(b[0], field - 135);
-  m[3] = ldexpf(b[1], field - 135);
+  m[0] = ldexpf(a[0], field[0] - 135);
+  m[1] = ldexpf(a[1], field[1] - 135);
+  m[2] = ldexpf(b[0], field[2] - 135);
+  m[3] = ldexpf(b[1], field[3] - 135);
 }
-__device__ inline void decode_r4(uint32_t w, int field, float (&r)[4]) {
+__device__ inline void decode_r4(uint32_t w, const int (&field)[4], float (&r)[4]) {
   constexpr uint32_t mask = 255u << 19;
-  r[0] = ldexpf(bits_to_float((w << 19) & mask), field - 15);
-  r[1] = ldexpf(bits_to_float((w << 11) & mask), field - 15);
-  r[2] = ldexpf(bits_to_float((w << 3) & mask), field - 15);
-  r[3] = ldexpf(bits_to_float((w >> 5) & mask), field - 15);
+  r[0] = ldexpf(bits_to_float((w << 19) & mask), field[0] - 15);
+  r[1] = ldexpf(bits_to_float((w << 11) & mask), field[1] - 15);
+  r[2] = ldexpf(bits_to_float((w << 3) & mask), field[2] - 15);
+  r[3] = ldexpf(bits_to_float((w >> 5) & mask), field[3] - 15);
   if ((~w - 0x01010101u) & w & 0x80808080u) {  // some code is 255
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (((w >> (8 * j)) & 255u) == 255u) r[j] = bits_to_float(0x7fc00000u);
   }
+}
+__device__ inline void decode_m4(uint32_t w, int field, float (&m)[4]) {
+  const int f[4] = {field, field, field, field};
+  decode_m4(w, f, m);
+}
+__device__ inline void decode_r4(uint32_t w, int field, float (&r)[4]) {
+  const int f[4] = {field, field, field, field};
+  decode_r4(w, f, r);
 }
 
 // The top bytes of four words.

@@ -211,6 +211,52 @@ __global__ __launch_bounds__(1024) void grad_norms_total_kernel(int num, int par
   }
 }
 
+// Gradients times the factor, in place: the norms' runs, 16 bytes a lane, each product rounded once.
+// Masked rows keep what they hold.
+template <class G>
+__device__ inline void run_scale(G* __restrict__ g, const uint8_t* __restrict__ active, int32_t row_len, int64_t begin,
+                                 int64_t end, float f) {
+  constexpr int kVec = 16 / sizeof(G);
+  constexpr int kStep = 256 * kVec;
+  typedef G vec __attribute__((ext_vector_type(kVec), aligned(sizeof(G))));
+  const uint32_t l = threadIdx.x * kVec;
+  const uint64_t magic = active && row_len > 1 ? ~(uint64_t)0 / (uint32_t)row_len + 1 : 0;
+  for (int64_t base = begin; base < end; base += kStep) {
+    const int64_t left = end - base - l;
+    const int n = left >= kVec ? kVec : left > 0 ? (int)left : 0;
+    const uint32_t some = active ? rows_on<kVec>(active, magic, row_len, base, l, n) : (1u << n) - 1u;
+    if (some == 0) continue;
+    G* p = g + base + l;
+    if (some == (1u << kVec) - 1u) {
+      vec v = *reinterpret_cast<const vec*>(p);
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) v[j] = (G)((float)v[j] * f);
+      *reinterpret_cast<vec*>(p) = v;
+    } else {
+#pragma unroll
+      for (int j = 0; j < kVec; ++j)
+        if (some >> j & 1u) p[j] = (G)((float)p[j] * f);
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void grad_scale_kernel(NormArgs A, const float* __restrict__ factor) {
+  const uint32_t b = blockIdx.x;
+  const int lane = threadIdx.x & 63;
+  const float f = *factor;
+  if (b >= A.groups || f == 1.0f || !(fabsf(f) < __builtin_huge_valf())) return;
+  int k = -1;
+  for (int at = 0; at < A.n; at += 64) k += __popcll(__ballot(at + lane < A.n && b >= A.begin[min(at + lane, A.n - 1)]));
+  k = __builtin_amdgcn_readfirstlane(k);
+  const int64_t begin = (int64_t)(b - A.begin[k]) * A.run, count = A.count[k];
+  const int64_t end = begin + A.run < count ? begin + A.run : count;
+  const int type = A.type[k], row_len = A.row_len[k];
+  void* g = const_cast<void*>(A.grad[k]);
+  if (type == GS_TYPE_F32) run_scale((float*)g, A.active, row_len, begin, end, f);
+  else if (type == GS_TYPE_BF16) run_scale((__bf16*)g, A.active, row_len, begin, end, f);
+  else run_scale((_Float16*)g, A.active, row_len, begin, end, f);
+}
+
 }  // namespace
 }  // namespace gs
 
@@ -281,5 +327,36 @@ extern "C" int gs_grad_norms(void* stream, int num, const void* const* grads, co
   hipLaunchKernelGGL(grad_norms_total_kernel, dim3(1), dim3(1024), 0, s, num, (int)L.partials, group_log2, (const double*)ws,
                      (const int32_t*)(ws + L.first), (double*)(ws + L.sums), grad_scale, max_norm, norms, out);
   GS_LAUNCH_CHECK("grad_norms_total_kernel");
+  return GS_OK;
+}
+
+extern "C" int gs_clip_grads(void* stream, int num, void* const* grads, const int* grad_types, const int64_t* counts,
+                             const int64_t* row_lens, const uint8_t* active, int64_t rows, double max_norm,
+                             const float* grad_scale, void* workspace, size_t workspace_bytes, float* norms, float* out) {
+  GS_REQUIRE(max_norm > 0.0, "gs_clip_grads: the norm to clip to must be positive");
+  const int rc = gs_grad_norms(stream, num, grads, grad_types, counts, row_lens, active, rows, max_norm, grad_scale,
+                               workspace, workspace_bytes, norms, out);
+  if (rc != GS_OK) return rc;
+  const NormLayout L = norm_layout(num, counts);
+  NormArgs A{};
+  A.active = active;
+  A.run = L.run;
+  for (int i = 0; i < num;) {
+    int k = 0;
+    int64_t groups = 0;
+    for (; i < num && k < kNormTensors; ++i) {
+      A.grad[k] = grads[i];
+      A.count[k] = counts[i];
+      A.row_len[k] = active && counts[i] ? (int32_t)row_lens[i] : 1;
+      A.type[k] = (uint8_t)grad_types[i];
+      A.begin[k++] = (uint32_t)groups;
+      groups += (counts[i] + L.run - 1) / L.run;
+    }
+    if (groups == 0) continue;
+    A.n = k;
+    A.groups = (uint32_t)groups;
+    hipLaunchKernelGGL(grad_scale_kernel, dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, A, out + 1);
+    GS_LAUNCH_CHECK("grad_scale_kernel");
+  }
   return GS_OK;
 }

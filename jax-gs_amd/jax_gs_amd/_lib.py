@@ -6,6 +6,7 @@ has no CPU fallback.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -115,6 +116,15 @@ _SIGS = {
                       ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_uint32],
     "gs_moments_encode": [_P, _I64, _P, _P, _P, _P, _P],
     "gs_moments_decode": [_P, _I64, _P, _P, _P, _P, _P],
+    "gs_clip_grads": [_P, _I, _P, _P, _P, _P, _P, _I64, ctypes.c_double, _P, _P, _SZ, _P, _P],
+    "gs_take_rows": [_P, _I, _P, _P, _P, _I64, _P, _P, _P, _P, _I, _I64],
+    "gs_move_rows": [_P, _I, _P, _P, _P, _I64, _P, _P, _I, _P],
+    "gs_moments_take": [_P, _I, _P, _I64, _P, _I64, _P, _P, _P, _P, _I, _I64, _P, _I64, _P, _P, _P],
+    "gs_moments_move_workspace_size": [_I64],
+    "gs_moments_move": [_P, _I, _P, _I64, _P, _I64, _P, _P, _P, _P, _I, _P, _SZ],
+    "gs_best_rows_workspace_size": [_I64],
+    "gs_best_rows": [_P, _I64, _P, _I, _P, _I64, _P, _SZ, _P],
+    "gs_densify_sources": [_P, _I64, _P, _SZ, _P, _P],
     "gs_densify_accumulate": [_P, _I64, _P, _P, _P, _F, _F, _P, _P, _P, _P, _P, _P],
 }
 _RESTYPE = {"gs_last_error": ctypes.c_char_p, "gs_bin_workspace_size": _SZ, "gs_l1_ssim_workspace_size": _SZ,
@@ -122,7 +132,9 @@ _RESTYPE = {"gs_last_error": ctypes.c_char_p, "gs_bin_workspace_size": _SZ, "gs_
             "gs_bin_reference_workspace_size": _SZ, "gs_preprocess_bwd_w2c_workspace_size": _SZ,
             "gs_l1_ssim_window_workspace_size": _SZ,
             "gs_densify_workspace_size": _SZ, "gs_composite_segments_size": _SZ,
-            "gs_composite_segments_size_for": _SZ, "gs_grad_norms_workspace_size": _SZ, "gs_composite_l1_out_size": _I64}
+            "gs_composite_segments_size_for": _SZ, "gs_grad_norms_workspace_size": _SZ,
+            "gs_moments_move_workspace_size": _SZ, "gs_best_rows_workspace_size": _SZ,
+            "gs_composite_l1_out_size": _I64}
 
 _lib = None
 
@@ -198,6 +210,14 @@ def stream_handle(device: torch.device):
     if _raw_stream is not None and device.index is not None:
         return ctypes.c_void_p(_raw_stream(device.index))
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+_here = contextlib.nullcontext()
+
+
+def on(device: torch.device):
+    """`device` as the current one, to which launches and allocations go."""
+    return _here if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def capturing(device: torch.device) -> bool:

@@ -108,14 +108,15 @@ def _address(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-def _norms(dev, k: int, pointers: bytes, types: bytes, counts: bytes, mask, max_norm, scale) -> GradNorms:
+def _norms(dev, k: int, pointers: bytes, types: bytes, counts: bytes, mask, max_norm, scale,
+           entry: str = "gs_grad_norms") -> GradNorms:
     act, rows, lens = mask or (None, 0, None)
     nbytes = _lib.lib().gs_grad_norms_workspace_size(k, counts)
     # one allocation: the results, and from the next multiple of 8 bytes on the workspace
     head = (k + 3) // 2 * 2
     out = torch.empty((head + (nbytes + 3) // 4,), dtype=torch.float32, device=dev)
     at = out.data_ptr()
-    _lib.call("gs_grad_norms", _lib.stream_handle(dev), k, pointers, types, counts, lens, _address(act), rows,
+    _lib.call(entry, _lib.stream_handle(dev), k, pointers, types, counts, lens, _address(act), rows,
               0.0 if max_norm is None else float(max_norm), _address(scale), at + 4 * head, nbytes, at + 8, at)
     return GradNorms(out, k)
 
@@ -136,6 +137,28 @@ def grad_norms(grads, max_norm: Optional[float] = None, active_mask=None, grad_s
     pointers, types, counts, kept = _lib.tensors().gather(gs, dev.index, "grad_norms")
     mask = None if active_mask is None else _mask(active_mask, gs, dev, "grad_norms")
     return _norms(dev, len(gs), pointers, types, counts, mask, max_norm, _scalar(grad_scale, dev, "grad_norms"))
+
+
+def clip_grads_(grads, max_norm: float, active_mask=None, grad_scale=None) -> GradNorms:
+    """``grad_norms``, and every gradient multiplied in place by its factor, ``grad_scale * min(1, max_norm /
+    (total + 1e-6))``, rounded once to the gradient's type.  Rows where ``active_mask`` is False keep
+    what they hold, and where a gradient (of the other rows) or ``grad_scale`` is not finite all do: ``scale`` is NaN then.  For
+    optimizers that take no factor; ``AdamW(max_grad_norm=...)`` clips without writing the gradients."""
+    if not max_norm > 0.0:
+        raise ValueError(f"clip_grads_: max_norm must be positive, not {max_norm}")
+    gs = _tensors(grads)
+    first = next((g for g in gs if g is not None), None)
+    if first is None:
+        raise ValueError("clip_grads_: no gradients")
+    dev = _device(first, "clip_grads_")
+    native = _lib.tensors()
+    pointers, types, counts = native.dense(gs, dev.index, "clip_grads_", active_mask is not None)
+    mask = None if active_mask is None else _mask(active_mask, gs, dev, "clip_grads_")
+    with _lib.on(dev):
+        norms = _norms(dev, len(gs), pointers, types, counts, mask, max_norm, _scalar(grad_scale, dev, "clip_grads_"),
+                       "gs_clip_grads")
+    native.written([], [], gs)
+    return norms
 
 
 def _load(own: torch.Tensor, d: dict, name: str) -> torch.Tensor:
@@ -247,6 +270,78 @@ class AdamWState:
         else:
             _lib.call("gs_moments_decode", _lib.stream_handle(dev), self.size, *map(_address, (
                 mu, nu, fields, self.mu_flat, self.nu_flat)))
+
+    def _rows(self, what: str):
+        """(rows, elements per row of each tensor) of a state whose tensors have the same rows."""
+        rows = self.shapes[0][0] if len(self.shapes[0]) else None
+        if any([not len(s) or s[0] != rows for s in self.shapes]):
+            raise ValueError(f"AdamWState.{what}: the state's tensors do not have the same rows")
+        return rows, array("q", [s[1:].numel() for s in self.shapes])
+
+    def _row_views(self, flat, rows: int, lens):
+        """A flat array's tensors by their addresses and row bytes."""
+        at, size = flat.data_ptr(), flat.element_size()
+        return array("q", [at + o * size for o in self.offsets]).tobytes(), array("q", [n * size for n in lens]).tobytes()
+
+    def take_rows(self, index) -> "AdamWState":
+        """A state of its own for tensors whose row i is these tensors' row ``index[i]`` (``rows.take_rows``
+        of the parameters): moments and masters of those rows, zeros where ``index`` is no row's.  8-bit
+        moments are rounded to nearest where a new neighbour raises the exponent of their block."""
+        from .rows import _index
+
+        dev = self.mu_flat.device
+        index = _index(index, dev, "AdamWState.take_rows")
+        rows, lens = self._rows("take_rows")
+        count = index.numel()
+        to = AdamWState(self.keys, [(count, *s[1:]) for s in self.shapes], self.bits)
+        to.count, to.powers, to._powers_stream = self.count, self.powers, self._powers_stream
+        with _lib.on(dev):
+            to._allocate(dev, zero=False)
+            stream, of = _lib.stream_handle(dev), (index.data_ptr(), 8 * index.element_size(), count)
+            pairs = [(self.mu_flat, to.mu_flat), (self.nu_flat, to.nu_flat)] if self.bits == 32 else []
+            if self.master_flat is not None:
+                to.master_flat = torch.empty((to.size,), dtype=torch.float32, device=dev)
+                pairs.append((self.master_flat, to.master_flat))
+            if pairs:
+                k = len(pairs) * len(lens)
+                sources, bytes_ = zip(*[self._row_views(a, rows, lens) for a, _ in pairs])
+                outs = b"".join([to._row_views(b, count, lens)[0] for _, b in pairs])
+                padded = array("q", [-(-n // BLOCK) * BLOCK * 4 for n in to.counts]).tobytes() * len(pairs)
+                row_bytes = b"".join(bytes_)
+                _lib.call("gs_take_rows", stream, k, b"".join(sources), row_bytes, row_bytes, rows, outs, padded, None, *of)
+            if self.bits == 8:
+                _lib.call("gs_moments_take", stream, len(lens), lens.tobytes(), rows, self._offsets, self.size,
+                          *map(_address, (self.mu_flat, self.nu_flat, self.fields)), *of, to._offsets, to.size,
+                          *map(_address, (to.mu_flat, to.nu_flat, to.fields)))
+        return to
+
+    def move_rows_(self, index) -> "AdamWState":
+        """In place, the moments and masters of row i become those of row ``index[i]``, or zero where ``index``
+        is negative, as ``rows.move_rows_`` moves the parameters.  Returns the state."""
+        from .rows import _index
+
+        dev = self.mu_flat.device
+        index = _index(index, dev, "AdamWState.move_rows_")
+        rows, lens = self._rows("move_rows_")
+        if index.numel() != rows:
+            raise ValueError(f"AdamWState.move_rows_: {index.numel()} indices for {rows} rows")
+        with _lib.on(dev):
+            stream, bits = _lib.stream_handle(dev), 8 * index.element_size()
+            flats = [self.mu_flat, self.nu_flat] if self.bits == 32 else []
+            if self.master_flat is not None:
+                flats.append(self.master_flat)
+            if flats:
+                at, bytes_ = zip(*[self._row_views(x, rows, lens) for x in flats])
+                row_bytes = b"".join(bytes_)
+                _lib.call("gs_move_rows", stream, len(flats) * len(lens), b"".join(at), row_bytes, row_bytes, rows, None,
+                          index.data_ptr(), bits, None)
+            if self.bits == 8:
+                nbytes = _lib.lib().gs_moments_move_workspace_size(self.size)
+                ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+                _lib.call("gs_moments_move", stream, len(lens), lens.tobytes(), rows, self._offsets, self.size,
+                          *map(_address, (self.mu_flat, self.nu_flat, self.fields)), index.data_ptr(), bits, ws.data_ptr(), nbytes)
+        _lib.tensors().written([], [], [self.mu_flat, self.nu_flat, self.fields, self.master_flat])
+        return self
 
     def state_dict(self) -> dict:
         """The state as a dict of tensors (the state's own) and plain values, for a checkpoint."""

@@ -20,6 +20,7 @@ from .. import _lib
 from ..core.gaussians import Gaussians
 from .adamw import AdamW, AdamWState
 from .optimizer import FIELDS, Adam, AdamState
+from .rows import best_rows, take_rows
 
 
 @dataclass
@@ -62,10 +63,13 @@ def init_density_state(gaussians: Gaussians, optimizer: Union[Adam, AdamW, None]
 
 def densify_and_prune(state: DensityState, generator: Optional[torch.Generator] = None, densify_enabled: bool = True,
                       grad_threshold: float = 0.0002, min_opacity: float = 0.005, extent: float = 5.0,
-                      max_screen_size: int = 512, noise: Optional[torch.Tensor] = None) -> DensityState:
+                      max_screen_size: int = 512, noise: Optional[torch.Tensor] = None,
+                      sources: bool = False) -> DensityState:
     """density.py:98-211 in place; returns the state.  ``noise`` ([M, 3] standard normal)
     overrides the draws from ``generator``.  state.last_counts (int32 [5] on the device):
-    clones, splits, pruned, available slots, densified."""
+    clones, splits, pruned, available slots, densified.  With ``sources``,
+    state.last_sources (int32 [M]) is the index by which ``rows.move_rows_`` moves what
+    else a program keeps for each Gaussian: the slot that each slot's rows came from."""
     g = state.gaussians
     M = g.means.shape[0]
     dev = g.means.device
@@ -76,12 +80,10 @@ def densify_and_prune(state: DensityState, generator: Optional[torch.Generator] 
         raise ValueError(f"densify_and_prune: noise must be [{M}, 3]")
     moments = []
     opt = state.opt_state
-    if opt is not None:
-        # 8-bit moments are moved in 32 bits: what they stand for comes back unchanged, but where a
-        # row that moved in has raised the exponent of its block.  Both forms are live meanwhile: 10 B
-        # an element next to the 8 of moments in 32 bits
-        wide = opt.convert(32) if getattr(opt, "bits", 32) == 8 else opt
-        mu, nu = wide.mu, wide.nu
+    # 8-bit moments follow the other arrays by the index of sources
+    after = opt is not None and getattr(opt, "bits", 32) == 8
+    if opt is not None and not after:
+        mu, nu = opt.mu, opt.nu
         moments = [mu[f] for f in FIELDS] + [nu[f] for f in FIELDS]
     for t in [getattr(g, f) for f in FIELDS] + moments:
         if t.dtype != torch.float32 or not t.is_contiguous() or t.shape[0] != M:
@@ -96,10 +98,39 @@ def densify_and_prune(state: DensityState, generator: Optional[torch.Generator] 
               len(moments), mptr, _lib.ptr(state.active_mask), _lib.ptr(state.grad_accum), _lib.ptr(state.denom),
               _lib.ptr(state.max_radii), _lib.ptr(noise), int(bool(densify_enabled)), float(grad_threshold),
               float(min_opacity), float(extent), float(max_screen_size), _lib.ptr(ws), nbytes, _lib.ptr(counts))
-    if opt is not None and wide is not opt:
-        opt.set_moments(wide)
-    state.last_counts = counts
+    state.last_counts, state.last_sources = counts, None
+    if after or sources:
+        state.last_sources = torch.empty((M,), dtype=torch.int32, device=dev)
+        _lib.call("gs_densify_sources", _lib.stream_handle(dev), M, _lib.ptr(ws), nbytes, _lib.ptr(counts),
+                  _lib.ptr(state.last_sources))
+    if after:
+        opt.move_rows_(state.last_sources)
     return state
+
+
+def resize_density_state(state: DensityState, capacity: int, scores: Optional[torch.Tensor] = None) -> DensityState:
+    """A new state of another capacity with the active Gaussians in front, in their order, and what belongs to
+    them: moments, statistics.  Where more are active than fit, those with the highest ``scores``
+    ([M]; without it the opacities) stay.  Waits for the host once, for the number of active ones."""
+    g = state.gaussians
+    dev = g.means.device
+    if capacity < 1:
+        raise ValueError(f"resize_density_state: capacity {capacity}")
+    if scores is None:
+        scores = g.opacities.detach().reshape(-1)
+    with torch.no_grad():
+        index = best_rows(scores, capacity, active_mask=state.active_mask)
+        identity = torch.zeros((4,), dtype=torch.float32, device=dev)
+        identity[:1].fill_(1.0)  # padded quaternions, as init_density_state's
+        own = [getattr(g, f) for f in FIELDS] + [state.active_mask, state.grad_accum, state.denom, state.max_radii]
+        *fields, mask, accum, denom, radii = take_rows(own, index, [None, None, identity] + [None] * 6)
+        opt = state.opt_state
+        if isinstance(opt, AdamState):
+            opt = AdamState(mu=take_rows(opt.mu, index), nu=take_rows(opt.nu, index), count=opt.count)
+        elif opt is not None:
+            opt = opt.take_rows(index)
+        return DensityState(gaussians=Gaussians(*fields), opt_state=opt, active_mask=mask, num_active=int(mask.sum()),
+                            grad_accum=accum, denom=denom, max_radii=radii)
 
 
 def reset_opacities(state: DensityState, reset_val: float = 0.01) -> DensityState:

@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
-from typing import Callable, Dict, Union
+from typing import Callable, Dict, Optional, Union
 
 import numpy as np
 import torch
@@ -37,18 +37,24 @@ def exponential_decay(init_value: float, transition_steps: int, decay_rate: floa
 
 @dataclass
 class AdamState:
-    """First and second moments per array (zeros at init) and the step count."""
+    """First and second moments per array (zeros at init) and the step count; the norms of
+    the last step's gradients where they were clipped."""
     mu: Dict[str, torch.Tensor]
     nu: Dict[str, torch.Tensor]
     count: int = 0
+    norms: Optional[object] = None
 
 
 class Adam:
     """optax.adam per parameter array with its own learning rate (a float or a schedule
-    of the step count), b1 0.9, b2 0.999, eps 1e-8."""
+    of the step count), b1 0.9, b2 0.999, eps 1e-8.  With ``max_grad_norm`` every step first
+    brings the gradients down to that norm, in place (``adamw.clip_grads_``, state.norms)."""
 
     def __init__(self, learning_rates: Dict[str, LearningRate], b1: float = 0.9, b2: float = 0.999,
-                 eps: float = 1e-8):
+                 eps: float = 1e-8, max_grad_norm: Optional[float] = None):
+        if max_grad_norm is not None and not max_grad_norm > 0.0:
+            raise ValueError(f"Adam: max_grad_norm must be positive, not {max_grad_norm}")
+        self.max_grad_norm = max_grad_norm
         missing = [f for f in FIELDS if f not in learning_rates]
         if missing:
             raise ValueError(f"Adam: no learning rate for {missing}")
@@ -82,6 +88,11 @@ class Adam:
             act = as_bytes(torch.as_tensor(active_mask, device=dev))
             if act.numel() != n:
                 raise ValueError(f"Adam: active_mask has {act.numel()} entries for {n} Gaussians")
+        state.norms = None
+        if self.max_grad_norm is not None:
+            from .adamw import clip_grads_
+
+            state.norms = clip_grads_([a[1] for a in arrays], self.max_grad_norm, active_mask=act)
         k = len(arrays)
         P = ctypes.c_void_p * k
         _lib.call("gs_adam_step", _lib.stream_handle(dev), k, P(*[a[0].data_ptr() for a in arrays]),

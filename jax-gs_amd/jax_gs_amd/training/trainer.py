@@ -65,14 +65,14 @@ def train_step(state, target_image, w2c, camera_static, optimizer, fast_tpu_rast
     rasterizer's VJP, then one kernel for the preprocessing VJP, the statistics and the
     Adam update (no parameter gradient reaches memory).  fused=False builds the same
     step from ``render``'s autograd, ``accumulate_from_extras`` and ``Adam.step``.  An
-    ``AdamW`` optimizer always takes that form (to clip, it needs the gradients whole; the one
-    kernel updates by ``Adam`` only); metrics["grad_norm"] is the norm it clipped."""
+    ``AdamW`` optimizer, and an ``Adam`` that clips, always take that form (to clip, they need the gradients
+    whole; the one kernel updates by ``Adam`` only); metrics["grad_norm"] is the norm it clipped."""
     W, H, fx, fy, cx, cy = camera_static
     params = state.gaussians
     dev = params.means.device
     camera = Camera(int(W), int(H), float(fx), float(fy), float(cx), float(cy),
                     torch.as_tensor(w2c, dtype=torch.float32, device=dev), None)
-    if not fused or isinstance(optimizer, AdamW):
+    if not fused or isinstance(optimizer, AdamW) or getattr(optimizer, "max_grad_norm", None) is not None:
         return _train_step_autograd(state, target_image, camera, optimizer, fast_tpu_rasterizer, sh_degree)
     return _train_step_fused(state, target_image, camera, optimizer, sh_degree, fast_tpu_rasterizer)
 
