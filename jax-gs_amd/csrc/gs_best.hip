@@ -2,9 +2,14 @@
 //
 // A score's key is a 32-bit number in the order of the scores: 0 for NaN (below everything), -0 as +0.
 // The k-th largest key T is found digit by digit from the top (11, 11 and 10 bits; half types have 16
-// bits, in the upper digits): a histogram of the digit among the rows that agree with T so far, and the
-// bin in which the k-th falls.  Rows with a key above T are taken, and of those with T the first.  Counts are integers, so
-// the result does not depend on the order of the atomics.
+// bits, in the upper two digits): a histogram of the digit among the rows that agree with T so far, and the
+// bin in which the k-th falls.  Rows with a key above T are taken, and of those with T the first.  Counts are
+// integers, so the result does not depend on the order of the atomics.
+//
+// Few bytes move (3M half scores and their mask 9 MB, 1.3 us), so launches and their latency bound it.  Up to 16384
+// rows one workgroup does everything with its keys in registers.  Beyond, a launch for each digit, one that counts
+// what each workgroup takes and one that writes; the bin of a digit is found by every workgroup of the next launch for
+// itself, which reads 8 KiB but saves a launch.
 #include "gs_common.h"
 
 #include <algorithm>
@@ -13,25 +18,24 @@ namespace gs {
 namespace {
 
 constexpr int kBestBlock = 1024;
-constexpr int kBestGroups = 512;   // at most, for the passes over the scores
+constexpr int kBestRun = 8;        // consecutive rows a thread
+constexpr int kBestTile = kBestBlock * kBestRun;
+constexpr int kBestGroups = 512;   // at most
+constexpr int kBestOne = 2;        // tiles that one workgroup holds in registers
 constexpr int kBins = 2048;
+constexpr int kAlike = 3;          // in place of a type: no scores
 
 struct BestControl {
   uint32_t hist[3][kBins];
-  uint32_t prefix[4];   // T's digits before digit d, in place
-  uint32_t want[4];     // how many rows are still wanted among those that agree
+  uint32_t above[kBestGroups], equal[kBestGroups];  // rows above T and with T of each workgroup
 };
 
 struct BestArgs {
-  const void* scores;      // NULL: all alike
+  const void* scores;
   const uint8_t* active;
   int64_t n;
-  int64_t chunk;           // rows per workgroup, a multiple of kBestBlock
-  int type;
-  int digits;
+  int64_t tiles;  // per workgroup
   BestControl* ctl;
-  uint32_t* above;         // per workgroup: rows above T, rows with T (then: those before)
-  uint32_t* equal;
   int32_t* out;
   uint32_t k;
 };
@@ -42,48 +46,93 @@ __device__ inline uint32_t key_of(float x) {
   return (int32_t)b < 0 ? ~b : b | 0x80000000u;
 }
 
+// The key in the 16 bits of a half type (of either: sign, exponent, mantissa).
+template <int kType>
+__device__ inline uint32_t half_key(uint32_t b) {
+  constexpr uint32_t kInf = kType == GS_TYPE_BF16 ? 0x7f80u : 0x7c00u;
+  if ((b & 0x7fffu) > kInf) return 0;
+  if (b == 0x8000u) b = 0;
+  return ((b & 0x8000u) ? ~b & 0xffffu : b | 0x8000u) << 16;
+}
+
+template <int kType>
 __device__ inline uint32_t key_at(const BestArgs& A, int64_t i) {
-  if (!A.scores) return 1u;
-  if (A.type == GS_TYPE_F32) return key_of(((const float*)A.scores)[i]);
-  const uint32_t b = ((const uint16_t*)A.scores)[i];
-  if (A.type == GS_TYPE_BF16) return key_of(bits_to_float(b << 16)) & 0xffff0000u;
-  // float16: its 16 bits in their own order, in the upper half
-  const uint32_t c = b == 0x8000u ? 0u : b;
-  if ((c & 0x7fffu) > 0x7c00u) return 0;
-  return ((c & 0x8000u) ? ~c & 0xffffu : c | 0x8000u) << 16;
+  if constexpr (kType == kAlike) return 1u;
+  else if constexpr (kType == GS_TYPE_F32) return key_of(((const float*)A.scores)[i]);
+  else return half_key<kType>(((const uint16_t*)A.scores)[i]);
+}
+
+// The keys of the rows from i on and which of them count (bit by bit).
+template <int kType>
+__device__ inline uint32_t keys_at(const BestArgs& A, int64_t i, uint32_t (&key)[kBestRun]) {
+  typedef float f32x4 __attribute__((ext_vector_type(4), aligned(4)));
+  typedef uint16_t u16x8 __attribute__((ext_vector_type(8), aligned(2)));
+  typedef uint8_t u8x8 __attribute__((ext_vector_type(8), aligned(1)));
+  uint32_t on = 0;
+  if (i + kBestRun <= A.n) {
+    on = 255u;
+    if (A.active) {
+      const u8x8 a = *reinterpret_cast<const u8x8*>(A.active + i);
+      on = 0;
+#pragma unroll
+      for (int j = 0; j < kBestRun; ++j) on |= (uint32_t)(a[j] != 0) << j;
+    }
+    if constexpr (kType == GS_TYPE_F32) {
+      const f32x4 a = *reinterpret_cast<const f32x4*>((const float*)A.scores + i);
+      const f32x4 b = *reinterpret_cast<const f32x4*>((const float*)A.scores + i + 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        key[j] = key_of(a[j]);
+        key[j + 4] = key_of(b[j]);
+      }
+    } else if constexpr (kType == kAlike) {
+#pragma unroll
+      for (int j = 0; j < kBestRun; ++j) key[j] = 1u;
+    } else {
+      const u16x8 a = *reinterpret_cast<const u16x8*>((const uint16_t*)A.scores + i);
+#pragma unroll
+      for (int j = 0; j < kBestRun; ++j) key[j] = half_key<kType>(a[j]);
+    }
+    return on;
+  }
+#pragma unroll
+  for (int j = 0; j < kBestRun; ++j) {
+    key[j] = 0;
+    if (i + j < A.n && !(A.active && !A.active[i + j])) {
+      key[j] = key_at<kType>(A, i + j);
+      on |= 1u << j;
+    }
+  }
+  return on;
 }
 
 // digit d of a key: 11, 11, 10 bits
 __device__ inline int shift_of(int d) { return d == 0 ? 21 : d == 1 ? 10 : 0; }
+__device__ inline uint32_t bin_of(uint32_t key, int d) { return (key >> shift_of(d)) & (d == 2 ? 1023u : 2047u); }
+// whether the digits above digit d agree
+__device__ inline bool agrees(uint32_t key, uint32_t prefix, int d) {
+  return d == 0 || (key ^ prefix) >> (d == 1 ? 21 : 10) == 0;
+}
 
-__global__ __launch_bounds__(kBestBlock) void best_clear_kernel(BestControl* ctl, uint32_t k) {
-  for (int i = threadIdx.x; i < 3 * kBins; i += kBestBlock) (&ctl->hist[0][0])[i] = 0;
-  if (threadIdx.x == 0) {
-    ctl->prefix[0] = 0;
-    ctl->want[0] = k;
+// One row for each lane with `in`, into the histogram; the bin of the first such lane, which many may
+// share (scores that are zero), costs one atomic.
+__device__ inline void add_to(uint32_t* h, bool in, uint32_t bin) {
+  const uint64_t all = __ballot(in);
+  if (all == 0) return;
+  const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)bin, __builtin_ctzll(all));
+  const uint64_t same = __ballot(in && bin == first);
+  if (in) {
+    if (bin != first) atomicAdd(&h[bin], 1u);
+    else if ((threadIdx.x & 63) == __builtin_ctzll(same)) atomicAdd(&h[bin], (uint32_t)__popcll(same));
   }
 }
 
-__global__ __launch_bounds__(kBestBlock) void best_hist_kernel(BestArgs A, int d) {
-  __shared__ uint32_t h[kBins];
-  for (int i = threadIdx.x; i < kBins; i += kBestBlock) h[i] = 0;
-  __syncthreads();
-  const uint32_t prefix = A.ctl->prefix[d];
-  const int sh = shift_of(d), above = sh + (d == 2 ? 10 : 11);
-  const int64_t begin = blockIdx.x * A.chunk, end = min(begin + A.chunk, A.n);
-  for (int64_t i = begin + threadIdx.x; i < end; i += kBestBlock) {
-    if (A.active && !A.active[i]) continue;
-    const uint32_t key = key_at(A, i);
-    if (d > 0 && (key >> above) != (prefix >> above)) continue;
-    atomicAdd(&h[(key >> sh) & (d == 2 ? 1023u : 2047u)], 1u);
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < kBins; i += kBestBlock)
-    if (h[i]) atomicAdd(&A.ctl->hist[d][i], h[i]);
-}
+struct Sums {
+  uint32_t w[kBestBlock / 64];
+};
 
-// Inclusive sum over the workgroup's threads of x, in thread order.
-__device__ inline uint32_t block_scan(uint32_t x, uint32_t* w) {
+// Inclusive sum over the workgroup's threads of x, in thread order, and the sum of all.
+__device__ inline uint32_t block_scan(uint32_t x, Sums& s, uint32_t& all) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -91,105 +140,209 @@ __device__ inline uint32_t block_scan(uint32_t x, uint32_t* w) {
     if (lane >= o) x += y;
   }
   __syncthreads();
-  if (lane == 63) w[wave] = x;
+  if (lane == 63) s.w[wave] = x;
   __syncthreads();
-  for (int q = 0; q < wave; ++q) x += w[q];
-  return x;
+  all = 0;
+  uint32_t before = 0;
+#pragma unroll
+  for (int q = 0; q < kBestBlock / 64; ++q) {
+    before += q < wave ? s.w[q] : 0;
+    all += s.w[q];
+  }
+  return x + before;
 }
 
-// The bin of digit d in which the wanted row falls, counted from the largest.
-__global__ __launch_bounds__(kBestBlock) void best_pick_kernel(BestArgs A, int d) {
-  __shared__ uint32_t w[kBestBlock / 64];
-  const uint32_t want = A.ctl->want[d];
-  const uint32_t* h = A.ctl->hist[d];
+struct Pick {
+  uint32_t prefix;  // T's digits so far, in place
+  uint32_t want;    // how many rows are still wanted among those that agree with them
+};
+
+// Digit d of T, from the histogram of the rows that agree so far: the bin in which the wanted row falls,
+// counted from the largest.  Where there are fewer rows than wanted, all are: T is 0 then, and of
+// the rows with key 0 all are among the first.
+__device__ inline Pick pick(const uint32_t* h, Pick p, int d, Sums& s, Pick& shared) {
   const int hi = kBins - 1 - 2 * (int)threadIdx.x;
   const uint32_t a = h[hi], b = h[hi - 1];
-  const uint32_t all = block_scan(a + b, w), before = all - a - b;
-  const int sh = shift_of(d);
-  if (before < want && want <= all) {
-    const bool second = before + a < want;
-    A.ctl->prefix[d + 1] = A.ctl->prefix[d] | ((uint32_t)(second ? hi - 1 : hi) << sh);
-    A.ctl->want[d + 1] = want - before - (second ? a : 0);
-  }
-  // fewer rows than wanted: everything is above T = 0 or, with key 0, among the first
-  if (threadIdx.x == kBestBlock - 1 && all < want) {
-    A.ctl->prefix[d + 1] = 0;
-    A.ctl->want[d + 1] = want;
-  }
-}
-
-__global__ __launch_bounds__(kBestBlock) void best_count_kernel(BestArgs A) {
-  __shared__ uint32_t w[kBestBlock / 64];
-  const uint32_t T = A.ctl->prefix[A.digits];
-  const int64_t begin = blockIdx.x * A.chunk, end = min(begin + A.chunk, A.n);
-  uint32_t above = 0, equal = 0;
-  for (int64_t i = begin + threadIdx.x; i < end; i += kBestBlock) {
-    if (A.active && !A.active[i]) continue;
-    const uint32_t key = key_at(A, i);
-    above += key > T;
-    equal += key == T;
-  }
-  const uint32_t a = block_scan(above, w), e = block_scan(equal, w);
-  if (threadIdx.x == kBestBlock - 1) {
-    A.above[blockIdx.x] = a;
-    A.equal[blockIdx.x] = e;
-  }
-}
-
-__global__ __launch_bounds__(kBestBlock) void best_write_kernel(BestArgs A) {
-  __shared__ uint32_t w[kBestBlock / 64];
-  __shared__ uint32_t sum[2];
-  const uint32_t T = A.ctl->prefix[A.digits], want = A.ctl->want[A.digits];
-  const int b = blockIdx.x, groups = gridDim.x;
-  // what the workgroups before this one have
-  uint32_t a = 0, e = 0, all_a = 0, all_e = 0;
-  if ((int)threadIdx.x < groups) {
-    all_a = A.above[threadIdx.x];
-    all_e = A.equal[threadIdx.x];
-    a = (int)threadIdx.x < b ? all_a : 0;
-    e = (int)threadIdx.x < b ? all_e : 0;
-  }
-  a = block_scan(a, w);
-  e = block_scan(e, w);
-  if (threadIdx.x == kBestBlock - 1) {
-    sum[0] = a;
-    sum[1] = e;
-  }
-  all_a = block_scan(all_a, w);
-  all_e = block_scan(all_e, w);
-  __shared__ uint32_t total;
-  if (threadIdx.x == kBestBlock - 1) total = all_a + min(all_e, want);
+  uint32_t all;
+  const uint32_t to = block_scan(a + b, s, all), before = to - a - b;
+  if (threadIdx.x == 0) shared = Pick{0, p.want};
   __syncthreads();
-  uint32_t base_a = sum[0], base_e = sum[1];
-  const int64_t begin = b * A.chunk, end = min(begin + A.chunk, A.n);
-  for (int64_t at = begin; at < end; at += kBestBlock) {
-    const int64_t i = at + threadIdx.x;
-    uint32_t up = 0, eq = 0;
-    if (i < end && !(A.active && !A.active[i])) {
-      const uint32_t key = key_at(A, i);
-      up = key > T;
-      eq = key == T;
-    }
-    const uint32_t both = block_scan(up | (eq << 16), w);  // at most 1024 of each
-    const uint32_t ia = base_a + (both & 0xffffu), ie = base_e + (both >> 16);
-    // rows above T before this one, and those of T that are taken
-    if (up || (eq && ie <= want)) {
-      const uint32_t p = (ia - up) + min(ie - eq, want);
-      if (p < A.k) A.out[p] = (int32_t)i;
-    }
-    __shared__ uint32_t last;
-    if (threadIdx.x == kBestBlock - 1) last = both;
+  if (before < p.want && p.want <= to) {
+    const bool second = before + a < p.want;
+    shared = Pick{p.prefix | (uint32_t)(second ? hi - 1 : hi) << shift_of(d), p.want - before - (second ? a : 0)};
+  }
+  __syncthreads();
+  return shared;
+}
+
+// Rows above and with T among a run's, `equal` in the upper half.
+__device__ inline uint32_t count_run(const uint32_t (&key)[kBestRun], uint32_t on, uint32_t T) {
+  uint32_t c = 0;
+#pragma unroll
+  for (int j = 0; j < kBestRun; ++j)
+    if (on >> j & 1u) c += key[j] > T ? 1u : key[j] == T ? 0x10000u : 0u;
+  return c;
+}
+
+// Writes a run's rows; `a` rows above T and `e` with T come before it.
+__device__ inline void write_run(const BestArgs& A, int64_t i, const uint32_t (&key)[kBestRun], uint32_t on, Pick p,
+                                 uint32_t a, uint32_t e) {
+#pragma unroll
+  for (int j = 0; j < kBestRun; ++j) {
+    if (!(on >> j & 1u)) continue;
+    const bool up = key[j] > p.prefix, eq = key[j] == p.prefix;
+    const uint32_t at = a + min(e, p.want);
+    if ((up || (eq && e < p.want)) && at < A.k) A.out[at] = (int32_t)(i + j);
+    a += up;
+    e += eq;
+  }
+}
+
+template <int kType>
+__global__ __launch_bounds__(kBestBlock) void best_one_kernel(BestArgs A) {
+  __shared__ uint32_t h[kBins];
+  __shared__ Sums s;
+  __shared__ Pick shared;
+  constexpr int kDigits = kType == kAlike ? 0 : kType == GS_TYPE_F32 ? 3 : 2;
+  uint32_t key[kBestOne][kBestRun], on[kBestOne];
+#pragma unroll
+  for (int v = 0; v < kBestOne; ++v) on[v] = keys_at<kType>(A, v * kBestTile + threadIdx.x * kBestRun, key[v]);
+  Pick p{0, A.k};
+#pragma unroll
+  for (int d = 0; d < kDigits; ++d) {
+    h[threadIdx.x] = h[threadIdx.x + kBestBlock] = 0;
     __syncthreads();
-    base_a += last & 0xffffu;
-    base_e += last >> 16;
+#pragma unroll
+    for (int v = 0; v < kBestOne; ++v)
+#pragma unroll
+      for (int j = 0; j < kBestRun; ++j)
+        add_to(h, (on[v] >> j & 1u) && agrees(key[v][j], p.prefix, d), bin_of(key[v][j], d));
+    __syncthreads();
+    p = pick(h, p, d, s, shared);
+  }
+  uint32_t a = 0, e = 0;
+#pragma unroll
+  for (int v = 0; v < kBestOne; ++v) {
+    uint32_t all;
+    const uint32_t own = count_run(key[v], on[v], p.prefix), to = block_scan(own, s, all) - own;
+    write_run(A, v * kBestTile + threadIdx.x * kBestRun, key[v], on[v], p, a + (to & 0xffffu), e + (to >> 16));
+    a += all & 0xffffu;
+    e += all >> 16;
+  }
+  for (uint32_t at = a + min(e, p.want) + threadIdx.x; at < A.k; at += kBestBlock) A.out[at] = -1;
+}
+
+__global__ __launch_bounds__(kBestBlock) void best_clear_kernel(BestControl* ctl) {
+  for (int i = threadIdx.x; i < 3 * kBins; i += kBestBlock) (&ctl->hist[0][0])[i] = 0;
+}
+
+// T's digits before digit d.
+__device__ inline Pick picks(const BestArgs& A, int d, Sums& s, Pick& shared) {
+  Pick p{0, A.k};
+  for (int q = 0; q < d; ++q) p = pick(A.ctl->hist[q], p, q, s, shared);
+  return p;
+}
+
+template <int kType>
+__global__ __launch_bounds__(kBestBlock) void best_hist_kernel(BestArgs A, int d) {
+  __shared__ uint32_t h[kBins];
+  __shared__ Sums s;
+  __shared__ Pick shared;
+  h[threadIdx.x] = h[threadIdx.x + kBestBlock] = 0;
+  const Pick p = picks(A, d, s, shared);
+  __syncthreads();
+  for (int64_t v = 0; v < A.tiles; ++v) {
+    const int64_t i = (blockIdx.x * A.tiles + v) * kBestTile + threadIdx.x * kBestRun;
+    uint32_t key[kBestRun];
+    const uint32_t on = keys_at<kType>(A, i, key);
+#pragma unroll
+    for (int j = 0; j < kBestRun; ++j) add_to(h, (on >> j & 1u) && agrees(key[j], p.prefix, d), bin_of(key[j], d));
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kBins; i += kBestBlock)
+    if (h[i]) atomicAdd(&A.ctl->hist[d][i], h[i]);
+}
+
+template <int kType>
+__global__ __launch_bounds__(kBestBlock) void best_count_kernel(BestArgs A) {
+  __shared__ Sums s;
+  __shared__ Pick shared;
+  constexpr int kDigits = kType == kAlike ? 0 : kType == GS_TYPE_F32 ? 3 : 2;
+  const Pick p = picks(A, kDigits, s, shared);
+  uint32_t above = 0, equal = 0;
+  for (int64_t v = 0; v < A.tiles; ++v) {
+    const int64_t i = (blockIdx.x * A.tiles + v) * kBestTile + threadIdx.x * kBestRun;
+    uint32_t key[kBestRun];
+    const uint32_t on = keys_at<kType>(A, i, key), c = count_run(key, on, p.prefix);
+    above += c & 0xffffu;
+    equal += c >> 16;
+  }
+  uint32_t a, e;
+  block_scan(above, s, a);
+  block_scan(equal, s, e);
+  if (threadIdx.x == 0) {
+    A.ctl->above[blockIdx.x] = a;
+    A.ctl->equal[blockIdx.x] = e;
+  }
+}
+
+template <int kType>
+__global__ __launch_bounds__(kBestBlock) void best_write_kernel(BestArgs A) {
+  __shared__ Sums s;
+  __shared__ Pick shared;
+  constexpr int kDigits = kType == kAlike ? 0 : kType == GS_TYPE_F32 ? 3 : 2;
+  const Pick p = picks(A, kDigits, s, shared);
+  // what the workgroups have, and those before this one
+  const uint32_t b = blockIdx.x, groups = gridDim.x;
+  const uint32_t xa = threadIdx.x < groups ? A.ctl->above[threadIdx.x] : 0;
+  const uint32_t xe = threadIdx.x < groups ? A.ctl->equal[threadIdx.x] : 0;
+  uint32_t a, e, all_a, all_e;
+  __shared__ uint32_t before[2];
+  const uint32_t to_a = block_scan(xa, s, all_a), to_e = block_scan(xe, s, all_e);
+  if (threadIdx.x == b) {
+    before[0] = to_a - xa;
+    before[1] = to_e - xe;
+  }
+  __syncthreads();
+  a = before[0];
+  e = before[1];
+  for (int64_t v = 0; v < A.tiles; ++v) {
+    const int64_t i = (blockIdx.x * A.tiles + v) * kBestTile + threadIdx.x * kBestRun;
+    uint32_t key[kBestRun], all;
+    const uint32_t on = keys_at<kType>(A, i, key), own = count_run(key, on, p.prefix), to = block_scan(own, s, all) - own;
+    write_run(A, i, key, on, p, a + (to & 0xffffu), e + (to >> 16));
+    a += all & 0xffffu;
+    e += all >> 16;
   }
   // nothing behind the last
-  for (int64_t p = total + (int64_t)b * kBestBlock + threadIdx.x; p < A.k; p += (int64_t)groups * kBestBlock) A.out[p] = -1;
+  const int64_t total = (int64_t)all_a + min(all_e, p.want);
+  for (int64_t at = total + (int64_t)b * kBestBlock + threadIdx.x; at < A.k; at += (int64_t)groups * kBestBlock) A.out[at] = -1;
 }
 
-int64_t best_chunk(int64_t n) {
-  const int64_t steps = (n + kBestBlock - 1) / kBestBlock;
-  return (steps + kBestGroups - 1) / kBestGroups * kBestBlock;
+template <int kType>
+int best_rows(hipStream_t s, BestArgs& A) {
+  if (A.n <= kBestOne * kBestTile) {
+    hipLaunchKernelGGL(best_one_kernel<kType>, dim3(1), dim3(kBestBlock), 0, s, A);
+    GS_LAUNCH_CHECK("best_one_kernel");
+    return GS_OK;
+  }
+  const int64_t tiles = (A.n + kBestTile - 1) / kBestTile;
+  A.tiles = (tiles + kBestGroups - 1) / kBestGroups;
+  const dim3 grid((unsigned)((tiles + A.tiles - 1) / A.tiles));
+  constexpr int kDigits = kType == kAlike ? 0 : kType == GS_TYPE_F32 ? 3 : 2;
+  if (kDigits) {
+    hipLaunchKernelGGL(best_clear_kernel, dim3(1), dim3(kBestBlock), 0, s, A.ctl);
+    GS_LAUNCH_CHECK("best_clear_kernel");
+  }
+  for (int d = 0; d < kDigits; ++d) {
+    hipLaunchKernelGGL(best_hist_kernel<kType>, grid, dim3(kBestBlock), 0, s, A, d);
+    GS_LAUNCH_CHECK("best_hist_kernel");
+  }
+  hipLaunchKernelGGL(best_count_kernel<kType>, grid, dim3(kBestBlock), 0, s, A);
+  GS_LAUNCH_CHECK("best_count_kernel");
+  hipLaunchKernelGGL(best_write_kernel<kType>, grid, dim3(kBestBlock), 0, s, A);
+  GS_LAUNCH_CHECK("best_write_kernel");
+  return GS_OK;
 }
 
 }  // namespace
@@ -197,9 +350,7 @@ int64_t best_chunk(int64_t n) {
 
 using namespace gs;
 
-extern "C" size_t gs_best_rows_workspace_size(int64_t rows) {
-  return rows >= 0 ? sizeof(BestControl) + 2 * kBestGroups * sizeof(uint32_t) : 0;
-}
+extern "C" size_t gs_best_rows_workspace_size(int64_t rows) { return rows >= 0 ? sizeof(BestControl) : 0; }
 
 extern "C" int gs_best_rows(void* stream, int64_t rows, const void* scores, int type, const uint8_t* active, int64_t k,
                             void* workspace, size_t workspace_bytes, int32_t* out) {
@@ -217,27 +368,12 @@ extern "C" int gs_best_rows(void* stream, int64_t rows, const void* scores, int 
   A.scores = scores;
   A.active = active;
   A.n = rows;
-  A.chunk = std::max<int64_t>(best_chunk(rows), kBestBlock);
-  A.type = type;
-  A.digits = !scores ? 0 : type == GS_TYPE_F32 ? 3 : 2;
   A.ctl = (BestControl*)workspace;
-  A.above = (uint32_t*)(A.ctl + 1);
-  A.equal = A.above + kBestGroups;
   A.out = out;
   A.k = (uint32_t)k;
   hipStream_t s = (hipStream_t)stream;
-  const dim3 grid((unsigned)std::max<int64_t>(1, (rows + A.chunk - 1) / A.chunk));
-  hipLaunchKernelGGL(best_clear_kernel, dim3(1), dim3(kBestBlock), 0, s, A.ctl, A.k);
-  GS_LAUNCH_CHECK("best_clear_kernel");
-  for (int d = 0; d < A.digits; ++d) {
-    hipLaunchKernelGGL(best_hist_kernel, grid, dim3(kBestBlock), 0, s, A, d);
-    GS_LAUNCH_CHECK("best_hist_kernel");
-    hipLaunchKernelGGL(best_pick_kernel, dim3(1), dim3(kBestBlock), 0, s, A, d);
-    GS_LAUNCH_CHECK("best_pick_kernel");
-  }
-  hipLaunchKernelGGL(best_count_kernel, grid, dim3(kBestBlock), 0, s, A);
-  GS_LAUNCH_CHECK("best_count_kernel");
-  hipLaunchKernelGGL(best_write_kernel, grid, dim3(kBestBlock), 0, s, A);
-  GS_LAUNCH_CHECK("best_write_kernel");
-  return GS_OK;
+  if (!scores) return best_rows<kAlike>(s, A);
+  if (type == GS_TYPE_F32) return best_rows<GS_TYPE_F32>(s, A);
+  if (type == GS_TYPE_BF16) return best_rows<GS_TYPE_BF16>(s, A);
+  return best_rows<GS_TYPE_F16>(s, A);
 }

@@ -5,8 +5,9 @@
 // its rows come from and encoded again, to nearest even.  Values come back as they were but where a
 // larger neighbour raises the exponent of their block.
 //
-// A wave makes a block, four elements a lane.  In a move, blocks without a changed row are left out; the
-// others go to a copy first, for a block is read by others while it changes.
+// A wave makes four blocks, four elements of each a lane, the loads of all four under way before the first is
+// encoded.  In a move, blocks without a changed row are left out; the others go to a copy first, for a block is
+// read by others while it changes.
 #include "gs_moments.h"
 #include "gs_pieces.h"
 #include "gs_rows.h"
@@ -17,7 +18,8 @@ namespace gs {
 namespace {
 
 constexpr int kMomentTensors = 80;  // per launch: the argument block stays below 4 KiB
-constexpr int kMomentGroup = 4;     // blocks per workgroup
+constexpr int kMomentAhead = 4;     // blocks per wave
+constexpr int kMomentGroup = 4 * kMomentAhead;  // per workgroup
 
 struct MomentRecord {
   int64_t count;     // elements behind which there is nothing
@@ -62,82 +64,117 @@ __device__ inline int32_t source(const MomentArgs& A, int32_t i) {
   return x < 0 ? -1 : i;
 }
 
+// The tensor of this workgroup: the last that begins at or before it.
+__device__ inline int tensor_of(const MomentArgs& A, uint32_t b) {
+  const int lane = threadIdx.x & 63;
+  int k = -1;
+  for (int at = 0; at < A.n; at += 64) k += __popcll(__ballot(at + lane < A.n && b >= A.begin[min(at + lane, A.n - 1)]));
+  return __builtin_amdgcn_readfirstlane(k);
+}
+
+// The blocks from `first` on of one tensor (the whole wave).  kQuad: rows of a multiple of four elements, of
+// which a lane's four are of one row and of one block.
+template <bool kMove, bool kQuad>
+__device__ inline void make_blocks(const MomentArgs& A, const MomentRecord& t, uint32_t first) {
+  constexpr int kOf = kQuad ? 1 : 4;  // sources of a lane's elements
+  const int lane = threadIdx.x & 63;
+  const uint32_t len = t.row_len;
+  const int64_t base0 = (int64_t)first * kMomBlock;
+  const uint64_t row0 = t.magic ? __umul64hi((uint64_t)base0, t.magic) : (uint64_t)base0;
+  const uint32_t at0 = (uint32_t)((uint64_t)base0 - row0 * len);
+  int32_t s[kMomentAhead][kOf];
+  uint32_t off[kMomentAhead][kOf];
+  uint32_t some = 0;  // blocks to make
+#pragma unroll
+  for (int g = 0; g < kMomentAhead; ++g) {
+    bool moved = false;
+#pragma unroll
+    for (int j = 0; j < kOf; ++j) {
+      const uint32_t d = g * kMomBlock + lane * 4 + j, e = at0 + d;
+      // less than row_len + 1024 elements from the first row
+      const uint32_t q = len > 4096u ? (e >= len ? 1u : 0u) : t.magic ? __umulhi(e, (uint32_t)(t.magic >> 32) + 1u) : e;
+      const int32_t row = (int32_t)(row0 + q);
+      const bool in = base0 + d < t.count;
+      off[g][j] = e - q * len;
+      s[g][j] = in ? source<kMove>(A, row) : -1;
+      if (kMove) moved |= in && s[g][j] != row;
+    }
+    if (first + g < t.blocks && (!kMove || __ballot(moved))) some |= 1u << g;
+  }
+  if (kMove) {
+    if (lane < kMomentAhead && first + lane < t.blocks) A.changed[t.dst_at + first + lane] = some >> lane & 1u;
+    if (some == 0) return;
+  }
+  const uint64_t from = (uint64_t)t.src_at * kMomBlock;
+  uint32_t wm[kMomentAhead], wr[kMomentAhead], f[kMomentAhead][kOf];
+#pragma unroll
+  for (int g = 0; g < kMomentAhead; ++g) {
+    wm[g] = wr[g] = 0;
+    if (!(some >> g & 1u)) continue;
+#pragma unroll
+    for (int j = 0; j < kOf; ++j) {
+      f[g][j] = 0;
+      if (s[g][j] < 0) continue;
+      const uint64_t at = from + (uint64_t)s[g][j] * len + off[g][j];
+      if (kQuad) {
+        wm[g] = *reinterpret_cast<const uint32_t*>(A.m8 + at);
+        wr[g] = *reinterpret_cast<const uint32_t*>(A.r8 + at);
+      } else {
+        wm[g] |= (uint32_t)A.m8[at] << (8 * j);
+        wr[g] |= (uint32_t)A.r8[at] << (8 * j);
+      }
+      f[g][j] = *(const uint16_t*)(A.fields + 2 * (at >> 8));
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < kMomentAhead; ++g) {
+    if (!(some >> g & 1u)) continue;
+    int fm[4], fr[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      fm[j] = (int)(f[g][j % kOf] & 255u);
+      fr[j] = (int)(f[g][j % kOf] >> 8);
+    }
+    float m[4], r[4];
+    decode_m4(wm[g], fm, m);
+    decode_r4(wr[g], fr, r);
+    const uint32_t none[4] = {0, 0, 0, 0};
+    uint32_t cm, cr, fields;
+    encode_block<false>(m, r, none, cm, cr, fields);
+    const uint64_t to = ((uint64_t)t.dst_at + first + g) * kMomBlock + lane * 4;
+    *reinterpret_cast<uint32_t*>(A.to_m8 + to) = cm;
+    *reinterpret_cast<uint32_t*>(A.to_r8 + to) = cr;
+    if (lane == 0) *(uint16_t*)(A.to_fields + 2 * (to >> 8)) = (uint16_t)fields;
+  }
+}
+
 template <bool kMove>
 __global__ __launch_bounds__(256) void moment_rows_kernel(MomentArgs A) {
   const uint32_t b = blockIdx.x;
-  const int lane = threadIdx.x & 63;
   if (b >= A.groups) return;
-  int k = -1;
-  for (int at = 0; at < A.n; at += 64) k += __popcll(__ballot(at + lane < A.n && b >= A.begin[min(at + lane, A.n - 1)]));
-  k = __builtin_amdgcn_readfirstlane(k);
+  const int k = tensor_of(A, b);
   const MomentRecord& t = A.t[k];
-  const uint32_t block = __builtin_amdgcn_readfirstlane((b - A.begin[k]) * kMomentGroup + (threadIdx.x >> 6));
-  if (block >= t.blocks) return;
-  const int64_t base = (int64_t)block * kMomBlock;
-  const uint64_t row0 = t.magic ? __umul64hi((uint64_t)base, t.magic) : (uint64_t)base;
-  const uint32_t len = t.row_len;
-  const uint32_t e0 = (uint32_t)((uint64_t)base - row0 * len) + lane * 4;
-  const uint64_t from = (uint64_t)t.src_at * kMomBlock;
-  uint32_t wm = 0, wr = 0;
-  int fm[4], fr[4];
-  bool moved = false;
-  int32_t row[4], s[4];
-  uint32_t off[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint32_t e = e0 + j;
-    // a lane is less than row_len + 256 from its block's first row
-    const uint32_t q = len > 4096u ? (e >= len ? 1u : 0u) : t.magic ? __umulhi(e, (uint32_t)(t.magic >> 32) + 1u) : e;
-    row[j] = (int32_t)(row0 + q);
-    off[j] = e - q * len;
-    s[j] = base + lane * 4 + j < t.count ? source<kMove>(A, row[j]) : -1;
-    if (kMove) moved |= base + lane * 4 + j < t.count && s[j] != row[j];
-  }
-  if (kMove) {
-    const bool any = __ballot(moved) != 0;
-    if (lane == 0) A.changed[t.dst_at + block] = any;
-    if (!any) return;
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    uint32_t cm = 0, cr = 0, f = 0;
-    if (s[j] >= 0) {
-      const uint64_t at = from + (uint64_t)s[j] * len + off[j];
-      cm = A.m8[at];
-      cr = A.r8[at];
-      f = *(const uint16_t*)(A.fields + 2 * (at >> 8));
-    }
-    wm |= cm << (8 * j);
-    wr |= cr << (8 * j);
-    fm[j] = (int)(f & 255u);
-    fr[j] = (int)(f >> 8);
-  }
-  float m[4], r[4];
-  decode_m4(wm, fm, m);
-  decode_r4(wr, fr, r);
-  const uint32_t none[4] = {0, 0, 0, 0};
-  uint32_t cm, cr, f;
-  encode_block<false>(m, r, none, cm, cr, f);
-  const uint64_t to = (uint64_t)t.dst_at * kMomBlock + base + lane * 4;
-  *reinterpret_cast<uint32_t*>(A.to_m8 + to) = cm;
-  *reinterpret_cast<uint32_t*>(A.to_r8 + to) = cr;
-  if (lane == 0) *(uint16_t*)(A.to_fields + 2 * ((uint64_t)t.dst_at + block)) = (uint16_t)f;
+  const uint32_t first =
+      __builtin_amdgcn_readfirstlane((b - A.begin[k]) * kMomentGroup + (threadIdx.x >> 6) * kMomentAhead);
+  if (first >= t.blocks) return;
+  if (t.row_len % 4 == 0) make_blocks<kMove, true>(A, t, first);
+  else make_blocks<kMove, false>(A, t, first);
 }
 
-// The changed blocks from the copy into their places.
-__global__ __launch_bounds__(256) void moment_back_kernel(int64_t blocks, const uint8_t* __restrict__ changed,
-                                                          const uint8_t* __restrict__ from_m8,
-                                                          const uint8_t* __restrict__ from_r8,
-                                                          const uint8_t* __restrict__ from_fields,
-                                                          uint8_t* __restrict__ m8, uint8_t* __restrict__ r8,
-                                                          uint8_t* __restrict__ fields) {
-  const int64_t block = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (block >= blocks || !changed[block]) return;
-  const int64_t at = block * kMomBlock + lane * 4;
-  *reinterpret_cast<uint32_t*>(m8 + at) = *reinterpret_cast<const uint32_t*>(from_m8 + at);
-  *reinterpret_cast<uint32_t*>(r8 + at) = *reinterpret_cast<const uint32_t*>(from_r8 + at);
-  if (lane == 0) *(uint16_t*)(fields + 2 * block) = *(const uint16_t*)(from_fields + 2 * block);
+// The changed blocks from the copy into their places, 16 bytes a lane and array.
+__global__ __launch_bounds__(256) void moment_back_kernel(MomentArgs A) {
+  typedef uint32_t vec __attribute__((ext_vector_type(4)));
+  const uint32_t b = blockIdx.x;
+  if (b >= A.groups) return;
+  const int k = tensor_of(A, b);
+  const uint32_t block = (b - A.begin[k]) * kMomentGroup + (threadIdx.x >> 4);
+  if (block >= A.t[k].blocks) return;
+  const uint64_t i = (uint64_t)A.t[k].dst_at + block;
+  if (!A.changed[i]) return;
+  const uint64_t at = i * kMomBlock + (threadIdx.x & 15) * 16;
+  *reinterpret_cast<vec*>(const_cast<uint8_t*>(A.m8) + at) = *reinterpret_cast<const vec*>(A.to_m8 + at);
+  *reinterpret_cast<vec*>(const_cast<uint8_t*>(A.r8) + at) = *reinterpret_cast<const vec*>(A.to_r8 + at);
+  if ((threadIdx.x & 15) == 0) *(uint16_t*)(const_cast<uint8_t*>(A.fields) + 2 * i) = *(const uint16_t*)(A.to_fields + 2 * i);
 }
 
 bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
@@ -157,8 +194,9 @@ int check_side(const char* what, int num, const int64_t* row_lens, int64_t rows,
   return GS_OK;
 }
 
-template <bool kMove>
-int launch(hipStream_t stream, int num, const int64_t* row_lens, const int64_t* offsets, const int64_t* out_offsets,
+enum { kTake, kMove, kBack };
+
+int launch(int what, hipStream_t stream, int num, const int64_t* row_lens, const int64_t* offsets, const int64_t* out_offsets,
            int64_t count, MomentArgs& A) {
   for (int i = 0; i < num;) {
     int k = 0;
@@ -182,7 +220,8 @@ int launch(hipStream_t stream, int num, const int64_t* row_lens, const int64_t* 
     if (k == 0) continue;
     A.n = k;
     A.groups = (uint32_t)groups;
-    hipLaunchKernelGGL(moment_rows_kernel<kMove>, dim3((unsigned)groups), dim3(256), 0, stream, A);
+    auto* kernel = what == kTake ? moment_rows_kernel<false> : what == kMove ? moment_rows_kernel<true> : moment_back_kernel;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), 0, stream, A);
     GS_LAUNCH_CHECK("moment_rows_kernel");
   }
   return GS_OK;
@@ -227,7 +266,7 @@ extern "C" int gs_moments_take(void* stream, int num, const int64_t* row_lens, i
   A.index = index;
   A.rows = (uint32_t)rows;
   A.wide = index_bits == 64;
-  return launch<false>((hipStream_t)stream, num, row_lens, offsets, out_offsets, count, A);
+  return launch(kTake, (hipStream_t)stream, num, row_lens, offsets, out_offsets, count, A);
 }
 
 extern "C" size_t gs_moments_move_workspace_size(int64_t state_size) {
@@ -267,17 +306,7 @@ extern "C" int gs_moments_move(void* stream, int num, const int64_t* row_lens, i
   A.index = index;
   A.rows = (uint32_t)rows;
   A.wide = index_bits == 64;
-  const int done = launch<true>((hipStream_t)stream, num, row_lens, offsets, offsets, rows, A);
+  const int done = launch(kMove, (hipStream_t)stream, num, row_lens, offsets, offsets, rows, A);
   if (done != GS_OK) return done;
-  // tensor by tensor: blocks between them belong to nobody
-  for (int i = 0; i < num; ++i) {
-    const int64_t first = offsets[i] / kMomBlock, here = (row_lens[i] * rows + kMomBlock - 1) / kMomBlock;
-    if (here == 0) continue;
-    const int64_t at = first * kMomBlock;
-    hipLaunchKernelGGL(moment_back_kernel, dim3((unsigned)div_up(here, 4)), dim3(256), 0, (hipStream_t)stream, here,
-                       A.changed + first, A.to_m8 + at, A.to_r8 + at, A.to_fields + 2 * first, mu8 + at, nu8 + at,
-                       fields + 2 * first);
-    GS_LAUNCH_CHECK("moment_back_kernel");
-  }
-  return GS_OK;
+  return launch(kBack, (hipStream_t)stream, num, row_lens, offsets, offsets, rows, A);
 }

@@ -58,6 +58,44 @@ NormLayout norm_layout(int num, const int64_t* counts) {
   return L;
 }
 
+// Deals the tensors out to launches, in order.
+struct NormList {
+  int num;
+  const void* const* grads;
+  const int* types;
+  const int64_t* counts;
+  const int64_t* row_lens;
+  const uint8_t* active;
+  int64_t run;
+  int tensor = 0;
+  int64_t done = 0;  // workgroups of the launches before
+
+  NormList(int num_, const void* const* grads_, const int* types_, const int64_t* counts_, const int64_t* row_lens_,
+           const uint8_t* active_, const NormLayout& L)
+      : num(num_), grads(grads_), types(types_), counts(counts_), row_lens(row_lens_), active(active_), run(L.run) {}
+
+  bool next(NormArgs& A) {
+    if (tensor >= num) return false;
+    int k = 0;
+    int64_t groups = 0;
+    for (; tensor < num && k < kNormTensors; ++tensor) {
+      A.grad[k] = grads[tensor];
+      A.count[k] = counts[tensor];
+      A.row_len[k] = active && counts[tensor] ? (int32_t)row_lens[tensor] : 1;
+      A.type[k] = (uint8_t)types[tensor];
+      A.begin[k++] = (uint32_t)groups;
+      groups += (counts[tensor] + run - 1) / run;
+    }
+    A.active = active;
+    A.run = run;
+    A.n = k;
+    A.groups = (uint32_t)groups;
+    A.first_partial = (int32_t)done;
+    done += groups;
+    return true;
+  }
+};
+
 __device__ inline double wave_sum(double x) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
@@ -218,19 +256,41 @@ __device__ inline void run_scale(G* __restrict__ g, const uint8_t* __restrict__ 
                                  int64_t end, float f) {
   constexpr int kVec = 16 / sizeof(G);
   constexpr int kStep = 256 * kVec;
+  constexpr int kAhead = 4;
+  constexpr uint32_t kAll = (1u << kVec) - 1u;
   typedef G vec __attribute__((ext_vector_type(kVec), aligned(sizeof(G))));
   const uint32_t l = threadIdx.x * kVec;
   const uint64_t magic = active && row_len > 1 ? ~(uint64_t)0 / (uint32_t)row_len + 1 : 0;
-  for (int64_t base = begin; base < end; base += kStep) {
+  int64_t base = begin;
+  for (; base + kAhead * kStep <= end; base += kAhead * kStep) {
+    vec v[kAhead];
+    uint32_t on[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      on[u] = active ? rows_on<kVec>(active, magic, row_len, base + u * kStep, l, kVec) : kAll;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (on[u]) v[u] = *reinterpret_cast<const vec*>(g + base + u * kStep + l);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (!on[u]) continue;
+#pragma unroll
+      for (int j = 0; j < kVec; ++j)
+        if (on[u] >> j & 1u) v[u][j] = (G)((float)v[u][j] * f);
+      *reinterpret_cast<vec*>(g + base + u * kStep + l) = v[u];
+    }
+  }
+  for (; base < end; base += kStep) {
     const int64_t left = end - base - l;
     const int n = left >= kVec ? kVec : left > 0 ? (int)left : 0;
     const uint32_t some = active ? rows_on<kVec>(active, magic, row_len, base, l, n) : (1u << n) - 1u;
     if (some == 0) continue;
     G* p = g + base + l;
-    if (some == (1u << kVec) - 1u) {
+    if (n == kVec) {
       vec v = *reinterpret_cast<const vec*>(p);
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) v[j] = (G)((float)v[j] * f);
+      for (int j = 0; j < kVec; ++j)
+        if (some >> j & 1u) v[j] = (G)((float)v[j] * f);
       *reinterpret_cast<vec*>(p) = v;
     } else {
 #pragma unroll
@@ -240,16 +300,69 @@ __device__ inline void run_scale(G* __restrict__ g, const uint8_t* __restrict__ 
   }
 }
 
-__global__ __launch_bounds__(256) void grad_scale_kernel(NormArgs A, const float* __restrict__ factor) {
+struct ScaleArgs {
+  NormArgs a;              // its partial and first are not used
+  const double* partial;   // of all launches; NULL: the factor is there already
+  int32_t partials;
+  int32_t writes;          // this launch's first workgroup writes the results
+  double max_norm;
+  const float* grad_scale;
+  float* norms;            // of this launch's first tensor, or NULL
+  float* out;
+};
+static_assert(sizeof(ScaleArgs) <= 4096, "kernel arguments");
+
+// The sum of n partial sums, in a fixed order, in every thread.
+__device__ inline double sum_of(const double* __restrict__ partial, int n, double (&w)[4]) {
+  double acc[2] = {0.0, 0.0};
+  for (int i = threadIdx.x; i < n; i += 2 * 256 * 4) {
+    double v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = partial[min(i + u * 256, n - 1)];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) acc[u & 1] += i + u * 256 < n ? v[u] : 0.0;
+  }
+  const double x = wave_sum(acc[0] + acc[1]);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = x;
+  __syncthreads();
+  return (w[0] + w[1]) + (w[2] + w[3]);
+}
+
+// Every workgroup adds all partial sums for itself: up to 16 KiB out of L2, which takes less than a launch that does
+// it once for all.
+__global__ __launch_bounds__(256) void grad_scale_kernel(ScaleArgs S) {
+  const NormArgs& A = S.a;
   const uint32_t b = blockIdx.x;
   const int lane = threadIdx.x & 63;
-  const float f = *factor;
-  if (b >= A.groups || f == 1.0f || !(fabsf(f) < __builtin_huge_valf())) return;
+  __shared__ double w[4];
+  float f;
+  if (S.partial) {
+    const double s = S.grad_scale ? (double)*S.grad_scale : 1.0;
+    const double n = sqrt(sum_of(S.partial, S.partials, w)) * fabs(s);
+    f = (float)(s * fmin(1.0, S.max_norm / (n + 1e-6)));
+    if (!(n < __builtin_huge_val())) f = bits_to_float(0x7fc00000u);
+    if (b == 0 && S.writes && threadIdx.x == 0) {
+      S.out[0] = (float)n;
+      S.out[1] = f;
+    }
+    if (b == 0 && S.norms)
+      for (int k = threadIdx.x; k < A.n; k += 256)
+        if (A.count[k] == 0) S.norms[k] = (float)fabs(0.0 * s);
+  } else {
+    f = S.out[1];
+  }
+  if (b >= A.groups) return;
   int k = -1;
   for (int at = 0; at < A.n; at += 64) k += __popcll(__ballot(at + lane < A.n && b >= A.begin[min(at + lane, A.n - 1)]));
   k = __builtin_amdgcn_readfirstlane(k);
   const int64_t begin = (int64_t)(b - A.begin[k]) * A.run, count = A.count[k];
   const int64_t end = begin + A.run < count ? begin + A.run : count;
+  if (S.partial && S.norms && begin == 0) {  // a tensor's first workgroup: its own norm
+    const double x = sum_of(S.partial + A.first_partial + b, (int)((count + A.run - 1) / A.run), w);
+    if (threadIdx.x == 0) S.norms[k] = (float)(sqrt(x) * (S.grad_scale ? fabs((double)*S.grad_scale) : 1.0));
+  }
+  if (f == 1.0f || !(fabsf(f) < __builtin_huge_valf())) return;
   const int type = A.type[k], row_len = A.row_len[k];
   void* g = const_cast<void*>(A.grad[k]);
   if (type == GS_TYPE_F32) run_scale((float*)g, A.active, row_len, begin, end, f);
@@ -269,58 +382,48 @@ extern "C" size_t gs_grad_norms_workspace_size(int num, const int64_t* counts) {
   return norm_layout(num, counts).total;
 }
 
-extern "C" int gs_grad_norms(void* stream, int num, const void* const* grads, const int* grad_types,
-                             const int64_t* counts, const int64_t* row_lens, const uint8_t* active, int64_t rows,
-                             double max_norm, const float* grad_scale, void* workspace, size_t workspace_bytes,
-                             float* norms, float* out) {
-  GS_REQUIRE(num >= 0, "gs_grad_norms: %d tensors", num);
-  GS_REQUIRE(num == 0 || (grads && grad_types && counts), "gs_grad_norms: NULL argument");
-  GS_REQUIRE(out && workspace, "gs_grad_norms: NULL argument");
-  GS_REQUIRE(!active || row_lens, "gs_grad_norms: a mask needs row lengths");
-  GS_REQUIRE(max_norm == max_norm, "gs_grad_norms: the norm to clip to is not a number");
+namespace {
+
+// Both norms and clipping: checks, and the launches of the partial sums.
+int norm_launches(const char* what, hipStream_t s, int num, const void* const* grads, const int* grad_types,
+                  const int64_t* counts, const int64_t* row_lens, const uint8_t* active, int64_t rows, double max_norm,
+                  void* workspace, size_t workspace_bytes, const float* out, NormLayout& L) {
+  GS_REQUIRE(num >= 0, "%s: %d tensors", what, num);
+  GS_REQUIRE(num == 0 || (grads && grad_types && counts), "%s: NULL argument", what);
+  GS_REQUIRE(out && workspace, "%s: NULL argument", what);
+  GS_REQUIRE(!active || row_lens, "%s: a mask needs row lengths", what);
+  GS_REQUIRE(max_norm == max_norm, "%s: the norm to clip to is not a number", what);
   for (int i = 0; i < num; ++i) {
-    GS_REQUIRE(counts[i] >= 0 && counts[i] < ((int64_t)1 << 40), "gs_grad_norms: tensor %d has %lld elements", i,
+    GS_REQUIRE(counts[i] >= 0 && counts[i] < ((int64_t)1 << 40), "%s: tensor %d has %lld elements", what, i,
                (long long)counts[i]);
-    GS_REQUIRE(counts[i] == 0 || grads[i], "gs_grad_norms: NULL tensor %d", i);
-    GS_REQUIRE(grad_types[i] >= GS_TYPE_F32 && grad_types[i] <= GS_TYPE_F16, "gs_grad_norms: type of tensor %d", i);
+    GS_REQUIRE(counts[i] == 0 || grads[i], "%s: NULL tensor %d", what, i);
+    GS_REQUIRE(grad_types[i] >= GS_TYPE_F32 && grad_types[i] <= GS_TYPE_F16, "%s: type of tensor %d", what, i);
     GS_REQUIRE((reinterpret_cast<uintptr_t>(grads[i]) & (grad_types[i] == GS_TYPE_F32 ? 3 : 1)) == 0,
-               "gs_grad_norms: tensor %d is not aligned to its type", i);
+               "%s: tensor %d is not aligned to its type", what, i);
     if (active && counts[i])
       GS_REQUIRE(row_lens[i] >= 1 && row_lens[i] < kMaxRowLen && rows >= 0 &&
                      counts[i] % row_lens[i] == 0 && counts[i] / row_lens[i] == rows,
-                 "gs_grad_norms: tensor %d has %lld elements, not rows x row length", i, (long long)counts[i]);
+                 "%s: tensor %d has %lld elements, not rows x row length", what, i, (long long)counts[i]);
   }
-  const NormLayout L = norm_layout(num, counts);
-  GS_REQUIRE(workspace_bytes >= L.total, "gs_grad_norms: workspace of %zu bytes, %zu needed", workspace_bytes,
-             L.total);
-  GS_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 7) == 0, "gs_grad_norms: the workspace must be 8-byte aligned");
-  GS_REQUIRE(L.partials < 0x7fffffff, "gs_grad_norms: too many elements");
+  L = norm_layout(num, counts);
+  GS_REQUIRE(workspace_bytes >= L.total, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, L.total);
+  GS_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 7) == 0, "%s: the workspace must be 8-byte aligned", what);
+  GS_REQUIRE(L.partials < 0x7fffffff, "%s: too many elements", what);
   char* ws = (char*)workspace;
   NormArgs A{};
-  A.active = active;
-  A.run = L.run;
-  hipStream_t s = (hipStream_t)stream;
-  int64_t done = 0;
-  for (int i = 0; i < num;) {
-    int k = 0;
-    int64_t groups = 0;
-    for (; i < num && k < kNormTensors; ++i) {
-      A.grad[k] = grads[i];
-      A.count[k] = counts[i];
-      A.row_len[k] = active && counts[i] ? (int32_t)row_lens[i] : 1;
-      A.type[k] = (uint8_t)grad_types[i];
-      A.begin[k++] = (uint32_t)groups;
-      groups += (counts[i] + L.run - 1) / L.run;
-    }
-    A.n = k;
-    A.groups = (uint32_t)groups;
-    A.first = (int32_t*)(ws + L.first) + (i - k);
-    A.partial = (double*)ws + done;
-    A.first_partial = (int32_t)done;
-    done += groups;
-    hipLaunchKernelGGL(grad_norms_kernel, dim3((unsigned)(groups > 0 ? groups : 1)), dim3(256), 0, s, A);
+  NormList list(num, grads, grad_types, counts, active ? row_lens : nullptr, active, L);
+  while (list.next(A)) {
+    A.first = (int32_t*)(ws + L.first) + list.tensor - A.n;
+    A.partial = (double*)ws + A.first_partial;
+    hipLaunchKernelGGL(grad_norms_kernel, dim3(A.groups ? A.groups : 1), dim3(256), 0, s, A);
     GS_LAUNCH_CHECK("grad_norms_kernel");
   }
+  return GS_OK;
+}
+
+int total_launch(hipStream_t s, int num, const NormLayout& L, double max_norm, const float* grad_scale, void* workspace,
+                 float* norms, float* out) {
+  const char* ws = (const char*)workspace;
   // all threads at once for few tensors; at least eight a tensor, whose loads then wait together
   int group_log2 = 10;
   while (group_log2 > 3 && (1024 >> group_log2) < num) --group_log2;
@@ -330,33 +433,47 @@ extern "C" int gs_grad_norms(void* stream, int num, const void* const* grads, co
   return GS_OK;
 }
 
+}  // namespace
+
+extern "C" int gs_grad_norms(void* stream, int num, const void* const* grads, const int* grad_types,
+                             const int64_t* counts, const int64_t* row_lens, const uint8_t* active, int64_t rows,
+                             double max_norm, const float* grad_scale, void* workspace, size_t workspace_bytes,
+                             float* norms, float* out) {
+  NormLayout L;
+  const int rc = norm_launches("gs_grad_norms", (hipStream_t)stream, num, grads, grad_types, counts, row_lens, active, rows,
+                               max_norm, workspace, workspace_bytes, out, L);
+  if (rc != GS_OK) return rc;
+  return total_launch((hipStream_t)stream, num, L, max_norm, grad_scale, workspace, norms, out);
+}
+
 extern "C" int gs_clip_grads(void* stream, int num, void* const* grads, const int* grad_types, const int64_t* counts,
                              const int64_t* row_lens, const uint8_t* active, int64_t rows, double max_norm,
                              const float* grad_scale, void* workspace, size_t workspace_bytes, float* norms, float* out) {
   GS_REQUIRE(max_norm > 0.0, "gs_clip_grads: the norm to clip to must be positive");
-  const int rc = gs_grad_norms(stream, num, grads, grad_types, counts, row_lens, active, rows, max_norm, grad_scale,
-                               workspace, workspace_bytes, norms, out);
+  hipStream_t s = (hipStream_t)stream;
+  NormLayout L;
+  int rc = norm_launches("gs_clip_grads", s, num, grads, grad_types, counts, row_lens, active, rows, max_norm, workspace,
+                         workspace_bytes, out, L);
   if (rc != GS_OK) return rc;
-  const NormLayout L = norm_layout(num, counts);
-  NormArgs A{};
-  A.active = active;
-  A.run = L.run;
-  for (int i = 0; i < num;) {
-    int k = 0;
-    int64_t groups = 0;
-    for (; i < num && k < kNormTensors; ++i) {
-      A.grad[k] = grads[i];
-      A.count[k] = counts[i];
-      A.row_len[k] = active && counts[i] ? (int32_t)row_lens[i] : 1;
-      A.type[k] = (uint8_t)grad_types[i];
-      A.begin[k++] = (uint32_t)groups;
-      groups += (counts[i] + L.run - 1) / L.run;
-    }
-    if (groups == 0) continue;
-    A.n = k;
-    A.groups = (uint32_t)groups;
-    hipLaunchKernelGGL(grad_scale_kernel, dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, A, out + 1);
+  ScaleArgs S{};
+  // more partial sums (of very many tensors) are added up once
+  const bool apart = L.partials > 2 * kNormRuns;
+  if (apart || num == 0) {
+    rc = total_launch(s, num, L, max_norm, grad_scale, workspace, norms, out);
+    if (rc != GS_OK) return rc;
+  }
+  S.partial = apart ? nullptr : (const double*)workspace;
+  S.partials = (int32_t)L.partials;
+  S.writes = 1;
+  S.max_norm = max_norm;
+  S.grad_scale = grad_scale;
+  S.out = out;
+  NormList list(num, grads, grad_types, counts, active ? row_lens : nullptr, active, L);
+  while (list.next(S.a)) {
+    S.norms = norms ? norms + list.tensor - S.a.n : nullptr;
+    hipLaunchKernelGGL(grad_scale_kernel, dim3(S.a.groups ? S.a.groups : 1), dim3(256), 0, s, S);
     GS_LAUNCH_CHECK("grad_scale_kernel");
+    S.writes = 0;
   }
   return GS_OK;
 }
