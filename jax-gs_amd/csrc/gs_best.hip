@@ -6,10 +6,11 @@
 // bin in which the k-th falls.  Rows with a key above T are taken, and of those with T the first.  Counts are
 // integers, so the result does not depend on the order of the atomics.
 //
-// Few bytes move (3M half scores and their mask 9 MB, 1.3 us), so launches and their latency bound it.  Up to 16384
-// rows one workgroup does everything with its keys in registers.  Beyond, a launch for each digit, one that counts
-// what each workgroup takes and one that writes; the bin of a digit is found by every workgroup of the next launch for
-// itself, which reads 8 KiB but saves a launch.
+// Few bytes move (3M half scores and their mask 9 MB, 1.3 us), so launches and their latency bound it, and for many rows
+// the atomics in LDS.  Up to 16384 rows one workgroup does everything with its keys in registers (2000 rows 10 us, 16000 16).
+// Beyond, a launch for each digit, one that counts what each workgroup takes and one that writes; the bin of a digit is
+// found by every workgroup of the next launch for itself, which reads 16 KiB but saves a launch.  500k rows 23 us in float32
+// and 20 in half types, 3M 37 and 32, 20M 113 and 95.
 #include "gs_common.h"
 
 #include <algorithm>
@@ -17,17 +18,27 @@
 namespace gs {
 namespace {
 
-constexpr int kBestBlock = 1024;
+constexpr int kBestBlock = 512;
 constexpr int kBestRun = 8;        // consecutive rows a thread
 constexpr int kBestTile = kBestBlock * kBestRun;
+constexpr int kOneBlock = 1024;    // of the workgroup that does everything
+constexpr int kOneTile = kOneBlock * kBestRun;
 constexpr int kBestGroups = 512;   // at most
 constexpr int kBestOne = 2;        // tiles that one workgroup holds in registers
 constexpr int kBins = 2048;
+// Histograms in memory, by turns of the workgroups, whose atomics wait for each other (3M float32 36.5 us, one 40.8, four 37.2).
+constexpr int kSplit = 2;
 constexpr int kAlike = 3;          // in place of a type: no scores
 
+struct Pick {
+  uint32_t prefix;  // T's digits so far, in place
+  uint32_t want;    // how many rows are still wanted among those that agree with them
+};
+
 struct BestControl {
-  uint32_t hist[3][kBins];
+  uint32_t hist[3][kSplit][kBins];
   uint32_t above[kBestGroups], equal[kBestGroups];  // rows above T and with T of each workgroup
+  Pick picks[4];                                    // before digit d
 };
 
 struct BestArgs {
@@ -114,24 +125,12 @@ __device__ inline bool agrees(uint32_t key, uint32_t prefix, int d) {
   return d == 0 || (key ^ prefix) >> (d == 1 ? 21 : 10) == 0;
 }
 
-// One row for each lane with `in`, into the histogram; the bin of the first such lane, which many may
-// share (scores that are zero), costs one atomic.
-__device__ inline void add_to(uint32_t* h, bool in, uint32_t bin) {
-  const uint64_t all = __ballot(in);
-  if (all == 0) return;
-  const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)bin, __builtin_ctzll(all));
-  const uint64_t same = __ballot(in && bin == first);
-  if (in) {
-    if (bin != first) atomicAdd(&h[bin], 1u);
-    else if ((threadIdx.x & 63) == __builtin_ctzll(same)) atomicAdd(&h[bin], (uint32_t)__popcll(same));
-  }
-}
-
 struct Sums {
-  uint32_t w[kBestBlock / 64];
+  uint32_t w[kOneBlock / 64];
 };
 
 // Inclusive sum over the workgroup's threads of x, in thread order, and the sum of all.
+template <int kBlock>
 __device__ inline uint32_t block_scan(uint32_t x, Sums& s, uint32_t& all) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -145,31 +144,35 @@ __device__ inline uint32_t block_scan(uint32_t x, Sums& s, uint32_t& all) {
   all = 0;
   uint32_t before = 0;
 #pragma unroll
-  for (int q = 0; q < kBestBlock / 64; ++q) {
+  for (int q = 0; q < kBlock / 64; ++q) {
     before += q < wave ? s.w[q] : 0;
     all += s.w[q];
   }
   return x + before;
 }
 
-struct Pick {
-  uint32_t prefix;  // T's digits so far, in place
-  uint32_t want;    // how many rows are still wanted among those that agree with them
-};
-
 // Digit d of T, from the histogram of the rows that agree so far: the bin in which the wanted row falls,
 // counted from the largest.  Where there are fewer rows than wanted, all are: T is 0 then, and of
 // the rows with key 0 all are among the first.
+template <int kBlock, int kHists>
 __device__ inline Pick pick(const uint32_t* h, Pick p, int d, Sums& s, Pick& shared) {
-  const int hi = kBins - 1 - 2 * (int)threadIdx.x;
-  const uint32_t a = h[hi], b = h[hi - 1];
-  uint32_t all;
-  const uint32_t to = block_scan(a + b, s, all), before = to - a - b;
-  if (threadIdx.x == 0) shared = Pick{0, p.want};
-  __syncthreads();
-  if (before < p.want && p.want <= to) {
-    const bool second = before + a < p.want;
-    shared = Pick{p.prefix | (uint32_t)(second ? hi - 1 : hi) << shift_of(d), p.want - before - (second ? a : 0)};
+  constexpr int kEach = kBins / kBlock;  // bins a thread
+  uint32_t x[kEach], own = 0, all;
+  const int hi = kBins - 1 - kEach * (int)threadIdx.x;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    x[j] = h[hi - j];
+#pragma unroll
+    for (int q = 1; q < kHists; ++q) x[j] += h[q * kBins + hi - j];
+    own += x[j];
+  }
+  uint32_t before = block_scan<kBlock>(own, s, all) - own;
+  if (threadIdx.x == 0 && all < p.want) shared = Pick{0, p.want};
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    if (before < p.want && p.want <= before + x[j])
+      shared = Pick{p.prefix | (uint32_t)(hi - j) << shift_of(d), p.want - before};
+    before += x[j];
   }
   __syncthreads();
   return shared;
@@ -184,83 +187,108 @@ __device__ inline uint32_t count_run(const uint32_t (&key)[kBestRun], uint32_t o
   return c;
 }
 
-// Writes a run's rows; `a` rows above T and `e` with T come before it.
-__device__ inline void write_run(const BestArgs& A, int64_t i, const uint32_t (&key)[kBestRun], uint32_t on, Pick p,
-                                 uint32_t a, uint32_t e) {
+// The rows of a tile that are taken, which follow one another in the result: `a` rows above T and `e` with T come before
+// the tile, `own` are this run's and `to` those of the tile before it.  By way of LDS, so that neighbours write
+// side by side.
+template <int kBlock>
+__device__ inline void write_tile(const BestArgs& A, int64_t i, const uint32_t (&key)[kBestRun], uint32_t on, Pick p,
+                                  uint32_t a, uint32_t e, uint32_t to, uint32_t all, int32_t* lds) {
+  const uint32_t base = a + min(e, p.want), end = a + (all & 0xffffu) + min(e + (all >> 16), p.want);
+  uint32_t ra = a + (to & 0xffffu), re = e + (to >> 16);
 #pragma unroll
   for (int j = 0; j < kBestRun; ++j) {
     if (!(on >> j & 1u)) continue;
     const bool up = key[j] > p.prefix, eq = key[j] == p.prefix;
-    const uint32_t at = a + min(e, p.want);
-    if ((up || (eq && e < p.want)) && at < A.k) A.out[at] = (int32_t)(i + j);
-    a += up;
-    e += eq;
+    if (up || (eq && re < p.want)) lds[ra + min(re, p.want) - base] = (int32_t)(i + j);
+    ra += up;
+    re += eq;
   }
+  __syncthreads();
+  for (uint32_t at = base + threadIdx.x; at < min(end, A.k); at += kBlock) A.out[at] = lds[at - base];
 }
 
 template <int kType>
-__global__ __launch_bounds__(kBestBlock) void best_one_kernel(BestArgs A) {
+__global__ __launch_bounds__(kOneBlock) void best_one_kernel(BestArgs A) {
   __shared__ uint32_t h[kBins];
+  __shared__ int32_t lds[kOneTile];
   __shared__ Sums s;
   __shared__ Pick shared;
   constexpr int kDigits = kType == kAlike ? 0 : kType == GS_TYPE_F32 ? 3 : 2;
   uint32_t key[kBestOne][kBestRun], on[kBestOne];
 #pragma unroll
-  for (int v = 0; v < kBestOne; ++v) on[v] = keys_at<kType>(A, v * kBestTile + threadIdx.x * kBestRun, key[v]);
+  for (int v = 0; v < kBestOne; ++v) on[v] = keys_at<kType>(A, v * kOneTile + threadIdx.x * kBestRun, key[v]);
   Pick p{0, A.k};
 #pragma unroll
   for (int d = 0; d < kDigits; ++d) {
-    h[threadIdx.x] = h[threadIdx.x + kBestBlock] = 0;
+#pragma unroll
+    for (int j = 0; j < kBins / kOneBlock; ++j) h[threadIdx.x + j * kOneBlock] = 0;
     __syncthreads();
 #pragma unroll
     for (int v = 0; v < kBestOne; ++v)
 #pragma unroll
       for (int j = 0; j < kBestRun; ++j)
-        add_to(h, (on[v] >> j & 1u) && agrees(key[v][j], p.prefix, d), bin_of(key[v][j], d));
+        if ((on[v] >> j & 1u) && agrees(key[v][j], p.prefix, d)) atomicAdd(&h[bin_of(key[v][j], d)], 1u);
     __syncthreads();
-    p = pick(h, p, d, s, shared);
+    p = pick<kOneBlock, 1>(h, p, d, s, shared);
   }
   uint32_t a = 0, e = 0;
 #pragma unroll
   for (int v = 0; v < kBestOne; ++v) {
     uint32_t all;
-    const uint32_t own = count_run(key[v], on[v], p.prefix), to = block_scan(own, s, all) - own;
-    write_run(A, v * kBestTile + threadIdx.x * kBestRun, key[v], on[v], p, a + (to & 0xffffu), e + (to >> 16));
+    const uint32_t own = count_run(key[v], on[v], p.prefix), to = block_scan<kOneBlock>(own, s, all) - own;
+    write_tile<kOneBlock>(A, v * kOneTile + threadIdx.x * kBestRun, key[v], on[v], p, a, e, to, all, lds);
     a += all & 0xffffu;
     e += all >> 16;
   }
-  for (uint32_t at = a + min(e, p.want) + threadIdx.x; at < A.k; at += kBestBlock) A.out[at] = -1;
+  for (uint32_t at = a + min(e, p.want) + threadIdx.x; at < A.k; at += kOneBlock) A.out[at] = -1;
 }
 
 __global__ __launch_bounds__(kBestBlock) void best_clear_kernel(BestControl* ctl) {
-  for (int i = threadIdx.x; i < 3 * kBins; i += kBestBlock) (&ctl->hist[0][0])[i] = 0;
+  for (int i = threadIdx.x; i < 3 * kSplit * kBins; i += kBestBlock) (&ctl->hist[0][0][0])[i] = 0;
 }
 
-// T's digits before digit d.
+// T's digits before digit d: those before d - 1 are there from the launch before, the last is found by every workgroup.
 __device__ inline Pick picks(const BestArgs& A, int d, Sums& s, Pick& shared) {
-  Pick p{0, A.k};
-  for (int q = 0; q < d; ++q) p = pick(A.ctl->hist[q], p, q, s, shared);
+  if (d == 0) return Pick{0, A.k};
+  const Pick p = pick<kBestBlock, kSplit>(A.ctl->hist[d - 1][0], d == 1 ? Pick{0, A.k} : A.ctl->picks[d - 1], d - 1, s, shared);
+  if (blockIdx.x == 0 && threadIdx.x == 0) A.ctl->picks[d] = p;
   return p;
 }
 
+// Four histograms in LDS, one word beside another: lanes with one bin (scores that are zero, or all alike) then wait for
+// a quarter of the others (20M equal scores 266 -> 115 us, eight 98; 3M different ones are as fast with one).
+constexpr int kCopies = 4;
 template <int kType>
 __global__ __launch_bounds__(kBestBlock) void best_hist_kernel(BestArgs A, int d) {
-  __shared__ uint32_t h[kBins];
+  __shared__ uint32_t h[kBins * kCopies];
   __shared__ Sums s;
   __shared__ Pick shared;
-  h[threadIdx.x] = h[threadIdx.x + kBestBlock] = 0;
+  // the first keys come while the last digit is found
+  int64_t i = blockIdx.x * A.tiles * kBestTile + threadIdx.x * kBestRun;
+  uint32_t key[kBestRun], on = keys_at<kType>(A, i, key);
+#pragma unroll
+  for (int j = 0; j < kBins / kBestBlock * kCopies; ++j) h[threadIdx.x + j * kBestBlock] = 0;
   const Pick p = picks(A, d, s, shared);
   __syncthreads();
-  for (int64_t v = 0; v < A.tiles; ++v) {
-    const int64_t i = (blockIdx.x * A.tiles + v) * kBestTile + threadIdx.x * kBestRun;
-    uint32_t key[kBestRun];
-    const uint32_t on = keys_at<kType>(A, i, key);
+  for (int64_t v = 0;;) {
 #pragma unroll
-    for (int j = 0; j < kBestRun; ++j) add_to(h, (on >> j & 1u) && agrees(key[j], p.prefix, d), bin_of(key[j], d));
+    for (int j = 0; j < kBestRun; ++j) {
+      if (!((on >> j & 1u) && agrees(key[j], p.prefix, d))) continue;
+      atomicAdd(&h[bin_of(key[j], d) * kCopies + threadIdx.x % kCopies], 1u);
+    }
+    if (++v == A.tiles) break;
+    i += kBestTile;
+    on = keys_at<kType>(A, i, key);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < kBins; i += kBestBlock)
-    if (h[i]) atomicAdd(&A.ctl->hist[d][i], h[i]);
+#pragma unroll
+  for (int j = 0; j < kBins / kBestBlock; ++j) {
+    const uint32_t bin = threadIdx.x + j * kBestBlock;
+    uint32_t c = 0;
+#pragma unroll
+    for (int q = 0; q < kCopies; ++q) c += h[bin * kCopies + q];
+    if (c) atomicAdd(&A.ctl->hist[d][blockIdx.x % kSplit][bin], c);
+  }
 }
 
 template <int kType>
@@ -268,18 +296,21 @@ __global__ __launch_bounds__(kBestBlock) void best_count_kernel(BestArgs A) {
   __shared__ Sums s;
   __shared__ Pick shared;
   constexpr int kDigits = kType == kAlike ? 0 : kType == GS_TYPE_F32 ? 3 : 2;
+  int64_t i = blockIdx.x * A.tiles * kBestTile + threadIdx.x * kBestRun;
+  uint32_t key[kBestRun], on = keys_at<kType>(A, i, key);
   const Pick p = picks(A, kDigits, s, shared);
   uint32_t above = 0, equal = 0;
-  for (int64_t v = 0; v < A.tiles; ++v) {
-    const int64_t i = (blockIdx.x * A.tiles + v) * kBestTile + threadIdx.x * kBestRun;
-    uint32_t key[kBestRun];
-    const uint32_t on = keys_at<kType>(A, i, key), c = count_run(key, on, p.prefix);
+  for (int64_t v = 0;;) {
+    const uint32_t c = count_run(key, on, p.prefix);
     above += c & 0xffffu;
     equal += c >> 16;
+    if (++v == A.tiles) break;
+    i += kBestTile;
+    on = keys_at<kType>(A, i, key);
   }
   uint32_t a, e;
-  block_scan(above, s, a);
-  block_scan(equal, s, e);
+  block_scan<kBestBlock>(above, s, a);
+  block_scan<kBestBlock>(equal, s, e);
   if (threadIdx.x == 0) {
     A.ctl->above[blockIdx.x] = a;
     A.ctl->equal[blockIdx.x] = e;
@@ -288,31 +319,37 @@ __global__ __launch_bounds__(kBestBlock) void best_count_kernel(BestArgs A) {
 
 template <int kType>
 __global__ __launch_bounds__(kBestBlock) void best_write_kernel(BestArgs A) {
+  __shared__ int32_t lds[kBestTile];
   __shared__ Sums s;
-  __shared__ Pick shared;
   constexpr int kDigits = kType == kAlike ? 0 : kType == GS_TYPE_F32 ? 3 : 2;
-  const Pick p = picks(A, kDigits, s, shared);
+  int64_t i = blockIdx.x * A.tiles * kBestTile + threadIdx.x * kBestRun;
+  uint32_t key[kBestRun], on = keys_at<kType>(A, i, key);
+  const Pick p = kDigits ? A.ctl->picks[kDigits] : Pick{0, A.k};
   // what the workgroups have, and those before this one
   const uint32_t b = blockIdx.x, groups = gridDim.x;
-  const uint32_t xa = threadIdx.x < groups ? A.ctl->above[threadIdx.x] : 0;
-  const uint32_t xe = threadIdx.x < groups ? A.ctl->equal[threadIdx.x] : 0;
-  uint32_t a, e, all_a, all_e;
-  __shared__ uint32_t before[2];
-  const uint32_t to_a = block_scan(xa, s, all_a), to_e = block_scan(xe, s, all_e);
-  if (threadIdx.x == b) {
-    before[0] = to_a - xa;
-    before[1] = to_e - xe;
+  uint32_t a = 0, e = 0, all_a = 0, all_e = 0;
+#pragma unroll
+  for (int j = 0; j < kBestGroups / kBestBlock; ++j) {
+    const uint32_t g = threadIdx.x + j * kBestBlock;
+    const uint32_t xa = g < groups ? A.ctl->above[g] : 0, xe = g < groups ? A.ctl->equal[g] : 0;
+    all_a += xa;
+    all_e += xe;
+    a += g < b ? xa : 0;
+    e += g < b ? xe : 0;
   }
-  __syncthreads();
-  a = before[0];
-  e = before[1];
-  for (int64_t v = 0; v < A.tiles; ++v) {
-    const int64_t i = (blockIdx.x * A.tiles + v) * kBestTile + threadIdx.x * kBestRun;
-    uint32_t key[kBestRun], all;
-    const uint32_t on = keys_at<kType>(A, i, key), own = count_run(key, on, p.prefix), to = block_scan(own, s, all) - own;
-    write_run(A, i, key, on, p, a + (to & 0xffffu), e + (to >> 16));
+  block_scan<kBestBlock>(a, s, a);
+  block_scan<kBestBlock>(e, s, e);
+  block_scan<kBestBlock>(all_a, s, all_a);
+  block_scan<kBestBlock>(all_e, s, all_e);
+  for (int64_t v = 0;;) {
+    uint32_t all;
+    const uint32_t own = count_run(key, on, p.prefix), to = block_scan<kBestBlock>(own, s, all) - own;
+    write_tile<kBestBlock>(A, i, key, on, p, a, e, to, all, lds);
     a += all & 0xffffu;
     e += all >> 16;
+    if (++v == A.tiles) break;
+    i += kBestTile;
+    on = keys_at<kType>(A, i, key);
   }
   // nothing behind the last
   const int64_t total = (int64_t)all_a + min(all_e, p.want);
@@ -321,8 +358,8 @@ __global__ __launch_bounds__(kBestBlock) void best_write_kernel(BestArgs A) {
 
 template <int kType>
 int best_rows(hipStream_t s, BestArgs& A) {
-  if (A.n <= kBestOne * kBestTile) {
-    hipLaunchKernelGGL(best_one_kernel<kType>, dim3(1), dim3(kBestBlock), 0, s, A);
+  if (A.n <= kBestOne * kOneTile) {
+    hipLaunchKernelGGL(best_one_kernel<kType>, dim3(1), dim3(kOneBlock), 0, s, A);
     GS_LAUNCH_CHECK("best_one_kernel");
     return GS_OK;
   }

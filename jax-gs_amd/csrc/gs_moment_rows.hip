@@ -5,9 +5,10 @@
 // its rows come from and encoded again, to nearest even.  Values come back as they were but where a
 // larger neighbour raises the exponent of their block.
 //
-// A wave makes four blocks, four elements of each a lane, the loads of all four under way before the first is
-// encoded.  In a move, blocks without a changed row are left out; the others go to a copy first, for a block is
-// read by others while it changes.
+// A wave makes four blocks: sixteen lanes a block where rows are a multiple of sixteen elements, else four elements of
+// each block a lane, with the loads of all four under way before the first is encoded.  In a move a workgroup first finds
+// which of its 64 blocks hold a changed row, and makes those; they go to a copy first, for a block is read by
+// others while it changes.
 #include "gs_moments.h"
 #include "gs_pieces.h"
 #include "gs_rows.h"
@@ -17,9 +18,10 @@
 namespace gs {
 namespace {
 
-constexpr int kMomentTensors = 80;  // per launch: the argument block stays below 4 KiB
+constexpr int kMomentTensors = 72;  // per launch: the argument block stays below 4 KiB
 constexpr int kMomentAhead = 4;     // blocks per wave
-constexpr int kMomentGroup = 4 * kMomentAhead;  // per workgroup
+constexpr int kTakeGroup = 4 * kMomentAhead;  // per workgroup
+constexpr int kMoveGroup = 64;      // in a move; 16 with rows of fewer elements than 16, of which they hold as many rows
 
 struct MomentRecord {
   int64_t count;     // elements behind which there is nothing
@@ -27,6 +29,7 @@ struct MomentRecord {
   uint32_t src_at, dst_at;  // blocks
   uint32_t row_len;
   uint32_t blocks;
+  uint32_t group;    // blocks per workgroup
 };
 
 struct MomentArgs {
@@ -34,7 +37,8 @@ struct MomentArgs {
   uint32_t begin[kMomentTensors];
   const uint8_t *m8, *r8, *fields;
   uint8_t *to_m8, *to_r8, *to_fields;
-  uint8_t* changed;  // per block of a move
+  uint64_t* changed;  // per workgroup of a move: its blocks, bit by bit
+  int64_t state_size;
   const void* index;
   uint32_t rows;     // of the tensors that are read
   int32_t n;
@@ -43,25 +47,43 @@ struct MomentArgs {
 };
 static_assert(sizeof(MomentArgs) <= 4096, "kernel arguments");
 
-// Entry i of the index, -1 for one that is no row.
+// Entry i of the index: a row, -1 for a negative one, -2 for one beyond the rows.
+template <bool kWide>
 __device__ inline int32_t entry(const MomentArgs& A, int64_t i) {
-  if (A.wide) {
+  if constexpr (kWide) {
     const int64_t x = ((const int64_t*)A.index)[i];
-    return x >= 0 && x < (int64_t)A.rows ? (int32_t)x : -1;
+    return x < 0 ? -1 : x < (int64_t)A.rows ? (int32_t)x : -2;
+  } else {
+    const int32_t x = ((const int32_t*)A.index)[i];
+    return x < 0 ? -1 : (uint32_t)x < A.rows ? x : -2;
   }
-  const int32_t x = ((const int32_t*)A.index)[i];
-  return x >= 0 && (uint32_t)x < A.rows ? x : -1;
 }
 
-// Where row i comes from, -1 for nowhere.
-template <bool kMove>
-__device__ inline int32_t source(const MomentArgs& A, int32_t i) {
-  const int32_t s = entry(A, i);
-  if (!kMove || s == i) return s;
-  if (s >= 0) return entry(A, s) == s ? s : i;
-  // a negative index frees the row, one beyond the rows leaves it
-  const int64_t x = A.wide ? ((const int64_t*)A.index)[i] : ((const int32_t*)A.index)[i];
-  return x < 0 ? -1 : i;
+// Where the rows come from, negative for nowhere, from their entries, all loads under way at once: in a move a row stays
+// whose source does not.
+template <bool kMove, bool kWide, int kN>
+__device__ inline void sources(const MomentArgs& A, const int32_t (&row)[kN], const bool (&in)[kN], int32_t (&s)[kN]) {
+#pragma unroll
+  for (int j = 0; j < kN; ++j) s[j] = entry<kWide>(A, in[j] ? row[j] : 0);
+  if (kMove) {
+    bool check = false;
+#pragma unroll
+    for (int j = 0; j < kN; ++j) {
+      if (s[j] == -2) s[j] = row[j];
+      check |= in[j] && s[j] >= 0 && s[j] != row[j];
+    }
+    if (__ballot(check)) {
+      int32_t of[kN];
+#pragma unroll
+      for (int j = 0; j < kN; ++j) of[j] = entry<kWide>(A, s[j] >= 0 ? s[j] : 0);
+#pragma unroll
+      for (int j = 0; j < kN; ++j)
+        if (s[j] >= 0 && of[j] != s[j]) s[j] = row[j];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kN; ++j)
+    if (!in[j]) s[j] = -1;
 }
 
 // The tensor of this workgroup: the last that begins at or before it.
@@ -72,68 +94,214 @@ __device__ inline int tensor_of(const MomentArgs& A, uint32_t b) {
   return __builtin_amdgcn_readfirstlane(k);
 }
 
-// The blocks from `first` on of one tensor (the whole wave).  kQuad: rows of a multiple of four elements, of
-// which a lane's four are of one row and of one block.
-template <bool kMove, bool kQuad>
-__device__ inline void make_blocks(const MomentArgs& A, const MomentRecord& t, uint32_t first) {
-  constexpr int kOf = kQuad ? 1 : 4;  // sources of a lane's elements
-  const int lane = threadIdx.x & 63;
+// A block's first row, and how far into it the block begins.
+__device__ inline uint64_t first_row(const MomentRecord& t, int64_t base, uint32_t& at) {
+  const uint64_t row = t.magic ? __umul64hi((uint64_t)base, t.magic) : (uint64_t)base;
+  at = (uint32_t)((uint64_t)base - row * t.row_len);
+  return row;
+}
+// The row of element e from a block's first row on, e less than row_len + 256.
+__device__ inline uint32_t row_of(const MomentRecord& t, uint32_t e) {
+  return t.row_len > 4096u ? (e >= t.row_len ? 1u : 0u) : t.magic ? __umulhi(e, (uint32_t)(t.magic >> 32) + 1u) : e;
+}
+
+// Maxima over each sixteen lanes, in every one of them.
+__device__ inline void row_max2_u32(uint32_t& x, uint32_t& y) {
+#define GS_DPP_MAX(ctrl)                                                                                  \
+  {                                                                                                       \
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, 0xf, 0xf, true));                   \
+    y = max(y, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)y, ctrl, 0xf, 0xf, true));                   \
+  }
+  GS_DPP_MAX(0xB1);   // quad_perm [1, 0, 3, 2]
+  GS_DPP_MAX(0x4E);   // quad_perm [2, 3, 0, 1]
+  GS_DPP_MAX(0x141);  // row_half_mirror
+  GS_DPP_MAX(0x140);  // row_mirror
+#undef GS_DPP_MAX
+}
+
+// encode_block to nearest for a block in sixteen lanes, sixteen values each.  kOdd: values that are not finite or
+// the largest exponents among them.
+template <bool kOdd>
+__device__ inline void encode_sixteen(const float (&m)[16], const float (&r)[16], uint32_t mm, uint32_t rr, uint32_t (&m8)[4],
+                                      uint32_t (&r8)[4], uint32_t& fields) {
+  constexpr uint32_t kInf = 0x7f800000u;
+  row_max2_u32(mm, rr);
+  const uint32_t fm = moment_field<3>(mm), fr = moment_field<4>(rr);
+  fields = fm | (fr << 8);
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    uint32_t cm[4], cr[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float x = m[4 * w + j], y = r[4 * w + j];
+      uint32_t a = moment_top<3, false>(fabsf(x), (int)fm, 0), b = moment_top<4, false>(y, (int)fr, 0);
+      if (kOdd) {
+        a = (float_to_bits(x) & 0x7fffffffu) >= kInf ? 127u << 24 : min(a, (126u << 24) | 0xffffffu);
+        b = float_to_bits(y) >= kInf ? 255u << 24 : min(b, (254u << 24) | 0xffffffu);
+      }
+      cm[j] = (a & 0x7fffffffu) | (float_to_bits(x) & 0x80000000u);
+      cr[j] = b;
+    }
+    m8[w] = pack_top(cm);
+    r8[w] = pack_top(cr);
+  }
+}
+
+// A block of a tensor with rows of a multiple of sixteen elements by sixteen lanes (of which the block may be none of
+// the tensor's): sixteen elements a lane, which are of one row and of one block.
+template <bool kMove, bool kWide>
+__device__ inline void make_even(const MomentArgs& A, const MomentRecord& t, uint32_t block, bool make) {
+  typedef uint32_t vec __attribute__((ext_vector_type(4)));
+  const int lane = threadIdx.x & 15;
   const uint32_t len = t.row_len;
-  const int64_t base0 = (int64_t)first * kMomBlock;
-  const uint64_t row0 = t.magic ? __umul64hi((uint64_t)base0, t.magic) : (uint64_t)base0;
-  const uint32_t at0 = (uint32_t)((uint64_t)base0 - row0 * len);
-  int32_t s[kMomentAhead][kOf];
-  uint32_t off[kMomentAhead][kOf];
-  uint32_t some = 0;  // blocks to make
+  const int64_t base = (int64_t)block * kMomBlock;
+  uint32_t at0;
+  const uint64_t row0 = first_row(t, base, at0);
+  const uint32_t e = at0 + lane * 16, q = row_of(t, e);
+  const int32_t row[1] = {(int32_t)(row0 + q)};
+  const bool in[1] = {make && base + lane * 16 < t.count};
+  int32_t s[1];
+  sources<kMove, kWide>(A, row, in, s);
+  vec wm{}, wr{};
+  uint32_t f = 0;
+  if (s[0] >= 0) {
+    const uint64_t at = (uint64_t)t.src_at * kMomBlock + (uint64_t)s[0] * len + (e - q * len);
+    wm = *reinterpret_cast<const vec*>(A.m8 + at);
+    wr = *reinterpret_cast<const vec*>(A.r8 + at);
+    f = *(const uint16_t*)(A.fields + 2 * (at >> 8));
+  }
+  float m[16], r[16];
+  uint32_t mm = 0, rr = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    float x[4], y[4];
+    decode_m4(wm[w], (int)(f & 255u), x);
+    decode_r4(wr[w], (int)(f >> 8), y);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      m[4 * w + j] = x[j];
+      r[4 * w + j] = y[j];
+      mm = max(mm, float_to_bits(x[j]) & 0x7fffffffu);
+      rr = max(rr, float_to_bits(y[j]));
+    }
+  }
+  uint32_t cm[4], cr[4], fields;
+  if (__ballot(mm >= 0x7e800000u || rr >= 0x7e800000u)) {  // as encode_block decides
+    mm = rr = 0;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const uint32_t x = float_to_bits(m[j]) & 0x7fffffffu, y = float_to_bits(r[j]);
+      mm = max(mm, x < 0x7f800000u ? x : 0u);
+      rr = max(rr, y < 0x7f800000u ? y : 0u);
+    }
+    encode_sixteen<true>(m, r, mm, rr, cm, cr, fields);
+  } else {
+    encode_sixteen<false>(m, r, mm, rr, cm, cr, fields);
+  }
+  if (!make) return;
+  const uint64_t to = (uint64_t)t.dst_at * kMomBlock + base + lane * 16;
+  *reinterpret_cast<vec*>(A.to_m8 + to) = vec{cm[0], cm[1], cm[2], cm[3]};
+  *reinterpret_cast<vec*>(A.to_r8 + to) = vec{cr[0], cr[1], cr[2], cr[3]};
+  if (lane == 0) *(uint16_t*)(A.to_fields + 2 * (to >> 8)) = (uint16_t)fields;
+}
+
+// Four bytes from `at` on, of which those that lie in the array are right.
+__device__ inline uint32_t four_at(const uint8_t* p, uint64_t at, uint64_t size) {
+  typedef uint32_t any4 __attribute__((aligned(1)));
+  const uint64_t from = at < size - 4 ? at : size - 4;
+  return *reinterpret_cast<const any4*>(p + from) >> (8 * (uint32_t)(at - from));
+}
+
+// Four blocks (the same for the wave, none beyond `some`) of a tensor with other rows, four elements of each a lane.
+// kOf rows they can be of: 1 with rows of a multiple of four elements, 2 with rows of three and more, 4.
+template <bool kMove, bool kWide, int kOf>
+__device__ inline void make_odd(const MomentArgs& A, const MomentRecord& t, const uint32_t (&block)[kMomentAhead], int some) {
+  constexpr int kN = kMomentAhead * kOf;
+  const uint32_t len = t.row_len, l = (threadIdx.x & 63) * 4;
+  int32_t row[kN], s[kN];
+  uint32_t off[kN];  // of the first element that is of the row
+  bool in[kN];
 #pragma unroll
   for (int g = 0; g < kMomentAhead; ++g) {
-    bool moved = false;
+    const int64_t base = (int64_t)block[g] * kMomBlock;
+    uint32_t at0;
+    const uint64_t row0 = first_row(t, base, at0);
+    if (kOf == 4) {
 #pragma unroll
-    for (int j = 0; j < kOf; ++j) {
-      const uint32_t d = g * kMomBlock + lane * 4 + j, e = at0 + d;
-      // less than row_len + 1024 elements from the first row
-      const uint32_t q = len > 4096u ? (e >= len ? 1u : 0u) : t.magic ? __umulhi(e, (uint32_t)(t.magic >> 32) + 1u) : e;
-      const int32_t row = (int32_t)(row0 + q);
-      const bool in = base0 + d < t.count;
-      off[g][j] = e - q * len;
-      s[g][j] = in ? source<kMove>(A, row) : -1;
-      if (kMove) moved |= in && s[g][j] != row;
+      for (int j = 0; j < kOf; ++j) {
+        const uint32_t e = at0 + l + j, q = row_of(t, e);
+        row[g * kOf + j] = (int32_t)(row0 + q);
+        off[g * kOf + j] = e - q * len;
+        in[g * kOf + j] = g < some && base + l + j < t.count;
+      }
+    } else {
+      const uint32_t e = at0 + l, q = row_of(t, e);
+      row[g * kOf] = (int32_t)(row0 + q);
+      off[g * kOf] = e - q * len;
+      in[g * kOf] = g < some && base + l < t.count;
+      if (kOf == 2) {
+        const uint32_t here = len - off[g * kOf];  // elements of the first row from this lane's on
+        row[g * kOf + 1] = row[g * kOf] + 1;
+        off[g * kOf + 1] = 0;
+        in[g * kOf + 1] = g < some && here < 4 && base + l + here < t.count;
+      }
     }
-    if (first + g < t.blocks && (!kMove || __ballot(moved))) some |= 1u << g;
   }
-  if (kMove) {
-    if (lane < kMomentAhead && first + lane < t.blocks) A.changed[t.dst_at + first + lane] = some >> lane & 1u;
-    if (some == 0) return;
-  }
-  const uint64_t from = (uint64_t)t.src_at * kMomBlock;
-  uint32_t wm[kMomentAhead], wr[kMomentAhead], f[kMomentAhead][kOf];
+  sources<kMove, kWide>(A, row, in, s);
+  const uint64_t from = (uint64_t)t.src_at * kMomBlock, size = (uint64_t)A.state_size;
+  uint32_t wm[kMomentAhead], wr[kMomentAhead], f[kMomentAhead][4];
 #pragma unroll
   for (int g = 0; g < kMomentAhead; ++g) {
     wm[g] = wr[g] = 0;
-    if (!(some >> g & 1u)) continue;
 #pragma unroll
-    for (int j = 0; j < kOf; ++j) {
-      f[g][j] = 0;
-      if (s[g][j] < 0) continue;
-      const uint64_t at = from + (uint64_t)s[g][j] * len + off[g][j];
-      if (kQuad) {
-        wm[g] = *reinterpret_cast<const uint32_t*>(A.m8 + at);
-        wr[g] = *reinterpret_cast<const uint32_t*>(A.r8 + at);
-      } else {
-        wm[g] |= (uint32_t)A.m8[at] << (8 * j);
-        wr[g] |= (uint32_t)A.r8[at] << (8 * j);
+    for (int j = 0; j < 4; ++j) f[g][j] = 0;
+    if (g >= some || A.rows == 0) continue;
+    if (kOf == 4) {
+      uint32_t cm[4], cr[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int k = g * kOf + j;
+        // a row that comes from nowhere reads the first, and is none
+        const uint64_t at = from + (s[k] >= 0 ? (uint64_t)s[k] * len + off[k] : 0u);
+        cm[j] = A.m8[at];
+        cr[j] = A.r8[at];
+        f[g][j] = *(const uint16_t*)(A.fields + 2 * (at >> 8));
       }
-      f[g][j] = *(const uint16_t*)(A.fields + 2 * (at >> 8));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        wm[g] |= s[g * kOf + j] >= 0 ? cm[j] << (8 * j) : 0u;
+        wr[g] |= s[g * kOf + j] >= 0 ? cr[j] << (8 * j) : 0u;
+      }
+    } else if (kOf == 2) {
+      const int k = g * kOf;
+      const uint64_t a = from + (s[k] >= 0 ? (uint64_t)s[k] * len + off[k] : 0u);
+      const uint64_t b = from + (s[k + 1] >= 0 ? (uint64_t)s[k + 1] * len : 0u);
+      const uint32_t here = len - off[k] < 4 ? len - off[k] : 4;
+      const uint32_t am = four_at(A.m8, a, size), ar = four_at(A.r8, a, size);
+      const uint32_t bm = four_at(A.m8, b, size), br = four_at(A.r8, b, size);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint64_t at = (uint32_t)j < here ? a + j : b + (j - here);
+        f[g][j] = *(const uint16_t*)(A.fields + 2 * ((at < size ? at : 0u) >> 8));
+      }
+      const uint32_t mask = here < 4 ? (1u << (8 * here)) - 1u : ~0u;
+      wm[g] = (s[k] >= 0 ? am & mask : 0u) | (s[k + 1] >= 0 && here < 4 ? bm << (8 * (here & 3)) : 0u);
+      wr[g] = (s[k] >= 0 ? ar & mask : 0u) | (s[k + 1] >= 0 && here < 4 ? br << (8 * (here & 3)) : 0u);
+    } else if (s[g] >= 0) {
+      const uint64_t at = from + (uint64_t)s[g] * len + off[g];
+      wm[g] = *reinterpret_cast<const uint32_t*>(A.m8 + at);
+      wr[g] = *reinterpret_cast<const uint32_t*>(A.r8 + at);
+      f[g][0] = f[g][1] = f[g][2] = f[g][3] = *(const uint16_t*)(A.fields + 2 * (at >> 8));
     }
   }
 #pragma unroll
   for (int g = 0; g < kMomentAhead; ++g) {
-    if (!(some >> g & 1u)) continue;
+    if (g >= some) continue;
     int fm[4], fr[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      fm[j] = (int)(f[g][j % kOf] & 255u);
-      fr[j] = (int)(f[g][j % kOf] >> 8);
+      fm[j] = (int)(f[g][j] & 255u);
+      fr[j] = (int)(f[g][j] >> 8);
     }
     float m[4], r[4];
     decode_m4(wm[g], fm, m);
@@ -141,24 +309,101 @@ __device__ inline void make_blocks(const MomentArgs& A, const MomentRecord& t, u
     const uint32_t none[4] = {0, 0, 0, 0};
     uint32_t cm, cr, fields;
     encode_block<false>(m, r, none, cm, cr, fields);
-    const uint64_t to = ((uint64_t)t.dst_at + first + g) * kMomBlock + lane * 4;
+    const uint64_t to = ((uint64_t)t.dst_at + block[g]) * kMomBlock + l;
     *reinterpret_cast<uint32_t*>(A.to_m8 + to) = cm;
     *reinterpret_cast<uint32_t*>(A.to_r8 + to) = cr;
-    if (lane == 0) *(uint16_t*)(A.to_fields + 2 * (to >> 8)) = (uint16_t)fields;
+    if (l == 0) *(uint16_t*)(A.to_fields + 2 * (to >> 8)) = (uint16_t)fields;
   }
 }
 
-template <bool kMove>
-__global__ __launch_bounds__(256) void moment_rows_kernel(MomentArgs A) {
+template <bool kMove, bool kWide>
+__device__ inline void make_four(const MomentArgs& A, const MomentRecord& t, const uint32_t (&block)[kMomentAhead], int some) {
+  if (t.row_len % 4 == 0) make_odd<kMove, kWide, 1>(A, t, block, some);
+  else if (t.row_len >= 3) make_odd<kMove, kWide, 2>(A, t, block, some);
+  else make_odd<kMove, kWide, 4>(A, t, block, some);
+}
+
+template <bool kWide>
+__global__ __launch_bounds__(256) void moment_take_kernel(MomentArgs A) {
   const uint32_t b = blockIdx.x;
   if (b >= A.groups) return;
   const int k = tensor_of(A, b);
   const MomentRecord& t = A.t[k];
   const uint32_t first =
-      __builtin_amdgcn_readfirstlane((b - A.begin[k]) * kMomentGroup + (threadIdx.x >> 6) * kMomentAhead);
+      __builtin_amdgcn_readfirstlane((b - A.begin[k]) * kTakeGroup + (threadIdx.x >> 6) * kMomentAhead);
   if (first >= t.blocks) return;
-  if (t.row_len % 4 == 0) make_blocks<kMove, true>(A, t, first);
-  else make_blocks<kMove, false>(A, t, first);
+  if (t.row_len % 16 == 0) {
+    const uint32_t block = first + ((threadIdx.x >> 4) & 3);
+    make_even<false, kWide>(A, t, block, block < t.blocks);
+    return;
+  }
+  uint32_t block[kMomentAhead];
+#pragma unroll
+  for (int g = 0; g < kMomentAhead; ++g) block[g] = first + g;
+  make_four<false, kWide>(A, t, block, (int)min(t.blocks - first, (uint32_t)kMomentAhead));
+}
+
+template <bool kWide>
+__global__ __launch_bounds__(256) void moment_move_kernel(MomentArgs A) {
+  __shared__ uint32_t changed[2];
+  __shared__ uint8_t list[kMoveGroup];
+  const uint32_t b = blockIdx.x;
+  if (b >= A.groups) return;
+  const int k = tensor_of(A, b);
+  const MomentRecord& t = A.t[k];
+  const uint32_t group = t.group, first = (b - A.begin[k]) * group, len = t.row_len;
+  if (threadIdx.x < 2) changed[threadIdx.x] = 0;
+  __syncthreads();
+  // the rows with an element in these blocks, four of them under way at once
+  const int64_t base = (int64_t)first * kMomBlock, end = min(base + group * kMomBlock, t.count);
+  uint32_t at0, at1;
+  const int64_t row0 = (int64_t)first_row(t, base, at0), row1 = (int64_t)first_row(t, end - 1, at1);
+  uint32_t lo = 0, hi = 0;
+  for (int64_t r = row0 + threadIdx.x; r <= row1; r += 256 * 4) {
+    int32_t row[4], s[4];
+    bool in[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      row[j] = (int32_t)(r + 256 * j);
+      in[j] = r + 256 * j <= row1;
+    }
+    sources<true, kWide>(A, row, in, s);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (!in[j] || s[j] == row[j]) continue;
+      const int64_t e = (int64_t)row[j] * len - base;
+      const int from = e > 0 ? (int)(e / kMomBlock) : 0, to = (int)(min(e + len, end - base) - 1) / kMomBlock;
+      const uint64_t bits = ((uint64_t)2 << to) - ((uint64_t)1 << from);
+      lo |= (uint32_t)bits;
+      hi |= (uint32_t)(bits >> 32);
+    }
+  }
+  if (lo | hi) {  // once for each lane's part: lanes beside each other mostly have the same
+    const uint32_t first_lo = __builtin_amdgcn_readfirstlane(lo), first_hi = __builtin_amdgcn_readfirstlane(hi);
+    const bool other = lo != first_lo || hi != first_hi;
+    if (other || (threadIdx.x & 63) == __builtin_ctzll(__ballot(!other))) {
+      if (lo) atomicOr(&changed[0], lo);
+      if (hi) atomicOr(&changed[1], hi);
+    }
+  }
+  __syncthreads();
+  const uint64_t bits = (uint64_t)changed[1] << 32 | changed[0];
+  if (threadIdx.x == 0) A.changed[b] = bits;
+  if (bits == 0) return;
+  if (threadIdx.x < kMoveGroup && (bits >> threadIdx.x & 1u))
+    list[__popcll(bits & (((uint64_t)1 << threadIdx.x) - 1u))] = (uint8_t)threadIdx.x;
+  __syncthreads();
+  const int n = __popcll(bits);
+  if (len % 16 == 0) {
+    for (int i = threadIdx.x >> 4; (i & ~3) < n; i += 16) make_even<true, kWide>(A, t, first + list[min(i, n - 1)], i < n);
+    return;
+  }
+  for (int i = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * kMomentAhead; i < n; i += 4 * kMomentAhead) {
+    uint32_t block[kMomentAhead];
+#pragma unroll
+    for (int g = 0; g < kMomentAhead; ++g) block[g] = first + __builtin_amdgcn_readfirstlane(list[min(i + g, n - 1)]);
+    make_four<true, kWide>(A, t, block, min(n - i, kMomentAhead));
+  }
 }
 
 // The changed blocks from the copy into their places, 16 bytes a lane and array.
@@ -166,15 +411,19 @@ __global__ __launch_bounds__(256) void moment_back_kernel(MomentArgs A) {
   typedef uint32_t vec __attribute__((ext_vector_type(4)));
   const uint32_t b = blockIdx.x;
   if (b >= A.groups) return;
-  const int k = tensor_of(A, b);
-  const uint32_t block = (b - A.begin[k]) * kMomentGroup + (threadIdx.x >> 4);
-  if (block >= A.t[k].blocks) return;
-  const uint64_t i = (uint64_t)A.t[k].dst_at + block;
-  if (!A.changed[i]) return;
-  const uint64_t at = i * kMomBlock + (threadIdx.x & 15) * 16;
-  *reinterpret_cast<vec*>(const_cast<uint8_t*>(A.m8) + at) = *reinterpret_cast<const vec*>(A.to_m8 + at);
-  *reinterpret_cast<vec*>(const_cast<uint8_t*>(A.r8) + at) = *reinterpret_cast<const vec*>(A.to_r8 + at);
-  if ((threadIdx.x & 15) == 0) *(uint16_t*)(const_cast<uint8_t*>(A.fields) + 2 * i) = *(const uint16_t*)(A.to_fields + 2 * i);
+  const uint64_t bits = A.changed[b];
+  if (bits == 0) return;
+  const int k = tensor_of(A, b), lane = threadIdx.x & 15;
+  const uint64_t first = (uint64_t)A.t[k].dst_at + (b - A.begin[k]) * A.t[k].group;
+#pragma unroll
+  for (int g = 0; g < kMoveGroup / 16; ++g) {
+    const uint32_t block = g * 16 + (threadIdx.x >> 4);
+    if (!(bits >> block & 1u)) continue;
+    const uint64_t i = first + block, at = i * kMomBlock + lane * 16;
+    *reinterpret_cast<vec*>(const_cast<uint8_t*>(A.m8) + at) = *reinterpret_cast<const vec*>(A.to_m8 + at);
+    *reinterpret_cast<vec*>(const_cast<uint8_t*>(A.r8) + at) = *reinterpret_cast<const vec*>(A.to_r8 + at);
+    if (lane == 0) *(uint16_t*)(const_cast<uint8_t*>(A.fields) + 2 * i) = *(const uint16_t*)(A.to_fields + 2 * i);
+  }
 }
 
 bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
@@ -198,13 +447,15 @@ enum { kTake, kMove, kBack };
 
 int launch(int what, hipStream_t stream, int num, const int64_t* row_lens, const int64_t* offsets, const int64_t* out_offsets,
            int64_t count, MomentArgs& A) {
+  uint64_t* const changed = A.changed;
+  int64_t done = 0;  // workgroups of the launches before
   for (int i = 0; i < num;) {
     int k = 0;
     int64_t groups = 0;
     for (; i < num && k < kMomentTensors; ++i) {
       const int64_t elements = row_lens[i] * count, blocks = (elements + kMomBlock - 1) / kMomBlock;
       if (blocks == 0) continue;
-      const int64_t more = (blocks + kMomentGroup - 1) / kMomentGroup;
+      const int64_t per = what == kTake ? kTakeGroup : row_lens[i] < 16 ? 16 : kMoveGroup, more = (blocks + per - 1) / per;
       GS_REQUIRE(more <= kMaxGroups, "gs_moments: tensor %d is too large", i);
       if (groups + more > kMaxGroups) break;
       MomentRecord& t = A.t[k];
@@ -214,16 +465,22 @@ int launch(int what, hipStream_t stream, int num, const int64_t* row_lens, const
       t.src_at = (uint32_t)(offsets[i] / kMomBlock);
       t.dst_at = (uint32_t)(out_offsets[i] / kMomBlock);
       t.blocks = (uint32_t)blocks;
+      t.group = (uint32_t)per;
       A.begin[k++] = (uint32_t)groups;
       groups += more;
     }
     if (k == 0) continue;
     A.n = k;
     A.groups = (uint32_t)groups;
-    auto* kernel = what == kTake ? moment_rows_kernel<false> : what == kMove ? moment_rows_kernel<true> : moment_back_kernel;
+    A.changed = changed + done;
+    done += groups;
+    auto* kernel = what == kBack   ? moment_back_kernel
+                   : what == kMove ? (A.wide ? moment_move_kernel<true> : moment_move_kernel<false>)
+                                   : (A.wide ? moment_take_kernel<true> : moment_take_kernel<false>);
     hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), 0, stream, A);
     GS_LAUNCH_CHECK("moment_rows_kernel");
   }
+  A.changed = changed;
   return GS_OK;
 }
 
@@ -260,6 +517,7 @@ extern "C" int gs_moments_take(void* stream, int num, const int64_t* row_lens, i
   A.m8 = mu8;
   A.r8 = nu8;
   A.fields = fields;
+  A.state_size = state_size;
   A.to_m8 = out_mu8;
   A.to_r8 = out_nu8;
   A.to_fields = out_fields;
@@ -272,7 +530,8 @@ extern "C" int gs_moments_take(void* stream, int num, const int64_t* row_lens, i
 extern "C" size_t gs_moments_move_workspace_size(int64_t state_size) {
   if (state_size < 0 || state_size % kMomBlock) return 0;
   const int64_t blocks = state_size / kMomBlock;
-  return (size_t)state_size * 2 + padded(blocks * 2) + padded(blocks);
+  // codes, exponents, and which blocks changed: eight bytes for each workgroup, at most one a block
+  return (size_t)state_size * 2 + padded(blocks * 2) + padded(blocks * 8);
 }
 
 extern "C" int gs_moments_move(void* stream, int num, const int64_t* row_lens, int64_t rows, const int64_t* offsets,
@@ -302,7 +561,8 @@ extern "C" int gs_moments_move(void* stream, int num, const int64_t* row_lens, i
   A.to_m8 = ws;
   A.to_r8 = ws + state_size;
   A.to_fields = ws + 2 * state_size;
-  A.changed = ws + 2 * state_size + padded(blocks * 2);
+  A.changed = (uint64_t*)(ws + 2 * state_size + padded(blocks * 2));
+  A.state_size = state_size;
   A.index = index;
   A.rows = (uint32_t)rows;
   A.wide = index_bits == 64;

@@ -104,6 +104,17 @@ def _scalar(grad_scale, dev, what: str):
     return grad_scale.resolve_neg() if grad_scale.is_neg() else grad_scale
 
 
+def row_index(index, dev, what: str) -> torch.Tensor:
+    """The index of rows, contiguous."""
+    if not isinstance(index, torch.Tensor) or index.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{what}: the index must be an int32 or int64 tensor")
+    if index.dim() != 1:
+        raise ValueError(f"{what}: the index must have one dimension, not {index.dim()}")
+    if index.device != dev:
+        raise ValueError(f"{what}: the index is on {index.device}, the tensors are on {dev}")
+    return index if index.is_contiguous() and not index.is_neg() else index.resolve_neg().contiguous()
+
+
 def _address(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
@@ -183,18 +194,20 @@ class AdamWState:
 
     def __init__(self, keys, shapes, bits: int):
         self.keys, self.shapes, self.bits = keys, [torch.Size(s) for s in shapes], bits
-        self.counts, self.offsets, at = [], [], 0
-        for s in self.shapes:
-            n = s.numel()
-            self.counts.append(n)
-            self.offsets.append(at)
-            at += -(-n // BLOCK) * BLOCK
-        self.size = at
-        self._offsets = array("q", self.offsets).tobytes()
+        self._row_layout = None  # _rows
+        self._lay_out([s.numel() for s in self.shapes])
         self.mu_flat = self.nu_flat = self.fields = self.master_flat = self.powers = None
         self._powers_stream: Optional[int] = None  # that the powers were allocated on
         self.count = 0
         self.norms: Optional[GradNorms] = None
+
+    def _lay_out(self, counts: list) -> None:
+        self.counts, self.offsets, at = counts, [], 0
+        for n in counts:
+            self.offsets.append(at)
+            at += -(-n // BLOCK) * BLOCK
+        self.size = at
+        self._offsets = array("q", self.offsets).tobytes()
 
     def _allocate(self, dev, zero: bool):
         new = torch.zeros if zero else torch.empty
@@ -272,74 +285,79 @@ class AdamWState:
                 mu, nu, fields, self.mu_flat, self.nu_flat)))
 
     def _rows(self, what: str):
-        """(rows, elements per row of each tensor) of a state whose tensors have the same rows."""
-        rows = self.shapes[0][0] if len(self.shapes[0]) else None
-        if any([not len(s) or s[0] != rows for s in self.shapes]):
-            raise ValueError(f"AdamWState.{what}: the state's tensors do not have the same rows")
-        return rows, array("q", [s[1:].numel() for s in self.shapes])
+        """(rows, elements per row of each tensor, the same as int64, bytes per row in 32 bits) of a state whose
+        tensors have the same rows."""
+        if self._row_layout is None:
+            rows = self.shapes[0][0] if len(self.shapes[0]) else None
+            if any([not len(s) or s[0] != rows for s in self.shapes]):
+                raise ValueError(f"AdamWState.{what}: the state's tensors do not have the same rows")
+            lens = [s[1:].numel() for s in self.shapes]
+            self._row_layout = rows, lens, array("q", lens).tobytes(), array("q", [4 * n for n in lens]).tobytes()
+        return self._row_layout
 
-    def _row_views(self, flat, rows: int, lens):
-        """A flat array's tensors by their addresses and row bytes."""
-        at, size = flat.data_ptr(), flat.element_size()
-        return array("q", [at + o * size for o in self.offsets]).tobytes(), array("q", [n * size for n in lens]).tobytes()
+    def _flats(self) -> list:
+        """The float32 arrays."""
+        flats = [self.mu_flat, self.nu_flat] if self.bits == 32 else []
+        return flats if self.master_flat is None else flats + [self.master_flat]
+
+    def _addresses(self, flats) -> bytes:
+        """Of every tensor in each of the float32 arrays."""
+        offsets = self.offsets
+        return array("q", [at + 4 * o for at in [x.data_ptr() for x in flats] for o in offsets]).tobytes()
 
     def take_rows(self, index) -> "AdamWState":
         """A state of its own for tensors whose row i is these tensors' row ``index[i]`` (``rows.take_rows``
         of the parameters): moments and masters of those rows, zeros where ``index`` is no row's.  8-bit
         moments are rounded to nearest where a new neighbour raises the exponent of their block."""
-        from .rows import _index
-
         dev = self.mu_flat.device
-        index = _index(index, dev, "AdamWState.take_rows")
-        rows, lens = self._rows("take_rows")
-        count = index.numel()
-        to = AdamWState(self.keys, [(count, *s[1:]) for s in self.shapes], self.bits)
-        to.count, to.powers, to._powers_stream = self.count, self.powers, self._powers_stream
+        index = row_index(index, dev, "AdamWState.take_rows")
+        rows, lens, lens_bytes, row_bytes = self._rows("take_rows")
+        count, k = index.numel(), len(lens)
+        to = AdamWState.__new__(AdamWState)
+        to.__dict__.update(self.__dict__)  # the powers are never written in place
+        to.norms = None
+        to.shapes = [torch.Size((count, *s[1:])) for s in self.shapes]
+        to._lay_out([n * count for n in lens])
+        to._row_layout = count, lens, lens_bytes, row_bytes
         with _lib.on(dev):
             to._allocate(dev, zero=False)
-            stream, of = _lib.stream_handle(dev), (index.data_ptr(), 8 * index.element_size(), count)
-            pairs = [(self.mu_flat, to.mu_flat), (self.nu_flat, to.nu_flat)] if self.bits == 32 else []
             if self.master_flat is not None:
                 to.master_flat = torch.empty((to.size,), dtype=torch.float32, device=dev)
-                pairs.append((self.master_flat, to.master_flat))
-            if pairs:
-                k = len(pairs) * len(lens)
-                sources, bytes_ = zip(*[self._row_views(a, rows, lens) for a, _ in pairs])
-                outs = b"".join([to._row_views(b, count, lens)[0] for _, b in pairs])
-                padded = array("q", [-(-n // BLOCK) * BLOCK * 4 for n in to.counts]).tobytes() * len(pairs)
-                row_bytes = b"".join(bytes_)
-                _lib.call("gs_take_rows", stream, k, b"".join(sources), row_bytes, row_bytes, rows, outs, padded, None, *of)
+            stream, of = _lib.stream_handle(dev), (index.data_ptr(), 8 * index.element_size(), count)
+            flats = self._flats()
+            if flats:
+                each = len(flats)
+                padded = array("q", [4 * (b - a) for a, b in zip(to.offsets, to.offsets[1:] + [to.size])]).tobytes()
+                _lib.call("gs_take_rows", stream, each * k, self._addresses(flats), row_bytes * each, row_bytes * each,
+                          rows, to._addresses(to._flats()), padded * each, None, *of)
             if self.bits == 8:
-                _lib.call("gs_moments_take", stream, len(lens), lens.tobytes(), rows, self._offsets, self.size,
-                          *map(_address, (self.mu_flat, self.nu_flat, self.fields)), *of, to._offsets, to.size,
-                          *map(_address, (to.mu_flat, to.nu_flat, to.fields)))
+                _lib.call("gs_moments_take", stream, k, lens_bytes, rows, self._offsets, self.size,
+                          self.mu_flat.data_ptr(), self.nu_flat.data_ptr(), self.fields.data_ptr(), *of, to._offsets,
+                          to.size, to.mu_flat.data_ptr(), to.nu_flat.data_ptr(), to.fields.data_ptr())
         return to
 
     def move_rows_(self, index) -> "AdamWState":
         """In place, the moments and masters of row i become those of row ``index[i]``, or zero where ``index``
         is negative, as ``rows.move_rows_`` moves the parameters.  Returns the state."""
-        from .rows import _index
-
         dev = self.mu_flat.device
-        index = _index(index, dev, "AdamWState.move_rows_")
-        rows, lens = self._rows("move_rows_")
+        index = row_index(index, dev, "AdamWState.move_rows_")
+        rows, lens, lens_bytes, row_bytes = self._rows("move_rows_")
         if index.numel() != rows:
             raise ValueError(f"AdamWState.move_rows_: {index.numel()} indices for {rows} rows")
+        k = len(lens)
         with _lib.on(dev):
             stream, bits = _lib.stream_handle(dev), 8 * index.element_size()
-            flats = [self.mu_flat, self.nu_flat] if self.bits == 32 else []
-            if self.master_flat is not None:
-                flats.append(self.master_flat)
+            flats = self._flats()
             if flats:
-                at, bytes_ = zip(*[self._row_views(x, rows, lens) for x in flats])
-                row_bytes = b"".join(bytes_)
-                _lib.call("gs_move_rows", stream, len(flats) * len(lens), b"".join(at), row_bytes, row_bytes, rows, None,
-                          index.data_ptr(), bits, None)
+                each = len(flats)
+                _lib.call("gs_move_rows", stream, each * k, self._addresses(flats), row_bytes * each, row_bytes * each,
+                          rows, None, index.data_ptr(), bits, None)
             if self.bits == 8:
                 nbytes = _lib.lib().gs_moments_move_workspace_size(self.size)
                 ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-                _lib.call("gs_moments_move", stream, len(lens), lens.tobytes(), rows, self._offsets, self.size,
-                          *map(_address, (self.mu_flat, self.nu_flat, self.fields)), index.data_ptr(), bits, ws.data_ptr(), nbytes)
+                _lib.call("gs_moments_move", stream, k, lens_bytes, rows, self._offsets, self.size,
+                          self.mu_flat.data_ptr(), self.nu_flat.data_ptr(), self.fields.data_ptr(), index.data_ptr(), bits,
+                          ws.data_ptr(), nbytes)
         _lib.tensors().written([], [], [self.mu_flat, self.nu_flat, self.fields, self.master_flat])
         return self
 

@@ -22,22 +22,10 @@ import torch
 from .. import _lib
 from ..core.gaussians import Gaussians
 from ..renderer._buffers import as_bytes
-from .adamw import _device, _keys, _tensors
-
-
-def _index(index, dev, what: str) -> torch.Tensor:
-    if not isinstance(index, torch.Tensor) or index.dtype not in (torch.int32, torch.int64):
-        raise TypeError(f"{what}: the index must be an int32 or int64 tensor")
-    if index.dim() != 1:
-        raise ValueError(f"{what}: the index must have one dimension, not {index.dim()}")
-    if index.device != dev:
-        raise ValueError(f"{what}: the index is on {index.device}, the tensors are on {dev}")
-    return index.resolve_neg().contiguous()
+from .adamw import _device, _keys, _tensors, row_index
 
 
 def _fills(fill, keys, count: int, what: str):
-    if fill is None:
-        return None
     fills = _tensors(fill, keys)
     if len(fills) != count:
         raise ValueError(f"{what}: {len(fills)} fills for {count} tensors")
@@ -61,10 +49,10 @@ def take_rows(tensors, index: torch.Tensor, fill=None):
     if not ts:
         raise ValueError("take_rows: no tensors")
     dev = _device(ts[0], "take_rows")
-    index = _index(index, dev, "take_rows")
+    index = row_index(index, dev, "take_rows")
     with _lib.on(dev):
         pointers, row_bytes, strides, rows, fills, out, new, kept = _lib.tensors().take(
-            ts, _fills(fill, _keys(tensors), len(ts), "take_rows"), index.numel(), dev.index, "take_rows")
+            ts, None if fill is None else _fills(fill, _keys(tensors), len(ts), "take_rows"), index.numel(), dev.index, "take_rows")
         _lib.call("gs_take_rows", _lib.stream_handle(dev), len(ts), pointers, row_bytes, strides, rows, out, None, fills,
                   index.data_ptr(), 8 * index.element_size(), index.numel())
     return _like(tensors, new)
@@ -81,13 +69,13 @@ def move_rows_(tensors, index: torch.Tensor, fill=None, left: Optional[torch.Ten
     if not ts:
         raise ValueError("move_rows_: no tensors")
     dev = _device(ts[0], "move_rows_")
-    index = _index(index, dev, "move_rows_")
+    index = row_index(index, dev, "move_rows_")
     if left is not None and (left.dtype != torch.int32 or left.numel() != 1 or left.device != dev):
         raise ValueError(f"move_rows_: left must be one int32 on {dev}")
     native = _lib.tensors()
     with _lib.on(dev):
         pointers, row_bytes, strides, rows, fills, kept = native.move(
-            ts, _fills(fill, _keys(tensors), len(ts), "move_rows_"), index, dev.index, "move_rows_")
+            ts, None if fill is None else _fills(fill, _keys(tensors), len(ts), "move_rows_"), index, dev.index, "move_rows_")
         if index.numel() != rows:
             raise ValueError(f"move_rows_: {index.numel()} indices for {rows} rows")
         _lib.call("gs_move_rows", _lib.stream_handle(dev), len(ts), pointers, row_bytes, strides, rows, fills,

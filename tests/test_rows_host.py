@@ -252,5 +252,5 @@ def test_states_of_different_rows_have_no_rows():
     for shapes in (((300,), (7,)), ((300, 2), ())):
         with pytest.raises(ValueError, match="same rows"):
             AdamWState(None, shapes, 32)._rows("take_rows")
-    rows, lens = AdamWState(None, ((5, 2, 3), (5,), (5, 0)), 8)._rows("take_rows")
-    assert rows == 5 and list(lens) == [6, 1, 0]
+    rows, lens, *_ = AdamWState(None, ((5, 2, 3), (5,), (5, 0)), 8)._rows("take_rows")
+    assert rows == 5 and lens == [6, 1, 0]
