@@ -5,10 +5,13 @@
 // its rows come from and encoded again, to nearest even.  Values come back as they were but where a
 // larger neighbour raises the exponent of their block.
 //
-// A wave makes four blocks: sixteen lanes a block where rows are a multiple of sixteen elements, else four elements of
-// each block a lane, with the loads of all four under way before the first is encoded.  In a move a workgroup first finds
-// which of its 64 blocks hold a changed row, and makes those; they go to a copy first, for a block is read by
-// others while it changes.
+// Sixteen lanes make two blocks where rows are a multiple of sixteen elements, else a wave four, four elements of each a
+// lane, with all loads under way before the first is encoded.  In a move a workgroup first finds which of its 64 blocks
+// hold a changed row, and makes those; they go to a copy first, for a block is read by others while it changes.
+//
+// 70 % of 2M rows of 48 elements taken: 63 us, bound by memory (at 5.4 TB/s with the lines of rows that are skipped); of the
+// Gaussians' five tensors 92, where the 11 of 59 elements in short rows take 30: their fields and codes come element by
+// element.  2M Gaussians moved, 8 % at random: 182 us, 8 % at the end 60, none 26.
 #include "gs_moments.h"
 #include "gs_pieces.h"
 #include "gs_rows.h"
@@ -21,6 +24,7 @@ namespace {
 constexpr int kMomentTensors = 72;  // per launch: the argument block stays below 4 KiB
 constexpr int kMomentAhead = 4;     // blocks per wave
 constexpr int kTakeGroup = 4 * kMomentAhead;  // per workgroup
+constexpr int kEvenAhead = 2;       // blocks of sixteen lanes (1.5M rows of 48 taken: 63 us, one 70, four 68)
 constexpr int kMoveGroup = 64;      // in a move; 16 with rows of fewer elements than 16, of which they hold as many rows
 
 struct MomentRecord {
@@ -119,58 +123,34 @@ __device__ inline void row_max2_u32(uint32_t& x, uint32_t& y) {
 #undef GS_DPP_MAX
 }
 
-// encode_block to nearest for a block in sixteen lanes, sixteen values each.  kOdd: values that are not finite or
-// the largest exponents among them.
-template <bool kOdd>
-__device__ inline void encode_sixteen(const float (&m)[16], const float (&r)[16], uint32_t mm, uint32_t rr, uint32_t (&m8)[4],
-                                      uint32_t (&r8)[4], uint32_t& fields) {
-  constexpr uint32_t kInf = 0x7f800000u;
-  row_max2_u32(mm, rr);
-  const uint32_t fm = moment_field<3>(mm), fr = moment_field<4>(rr);
-  fields = fm | (fr << 8);
+typedef uint32_t vec4u __attribute__((ext_vector_type(4)));
+typedef uint16_t pair __attribute__((ext_vector_type(2)));
+
+// Codes of roots under another exponent of their block, as integers: a code above gradual underflow that stays there
+// changes by 16 for each power of two.  all: the largest (exponent field * 16 + code) * 2 + (code >= 16) of the block;
+// false where the general way is needed.
+__device__ inline bool shift_roots(vec4u& w, uint32_t field, uint32_t all, uint32_t least, uint32_t& fields) {
+  const uint32_t top = all >> 1;
+  // a float32's exponent field of the largest root, as moment_field takes it
+  const uint32_t to = all ? (top >> 4) - 15u + ((top & 15u) == 15u ? 1u : 0u) : 0u;
+  fields |= to << 8;
+  const bool fine = all == 0 || ((all & 1u) && (top >> 4) >= 16u && to < 253u);
+  const int by = 16 * ((int)field - (int)to);
+  const bool kept = least == 0xffffu || by == 0 || (least >= 15u && (int)least + 1 + by >= 16);  // least: smallest code above 0, less 1
+  const uint32_t step = (uint32_t)(by < 0 ? -by : by) * 0x01010101u;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    uint32_t cm[4], cr[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float x = m[4 * w + j], y = r[4 * w + j];
-      uint32_t a = moment_top<3, false>(fabsf(x), (int)fm, 0), b = moment_top<4, false>(y, (int)fr, 0);
-      if (kOdd) {
-        a = (float_to_bits(x) & 0x7fffffffu) >= kInf ? 127u << 24 : min(a, (126u << 24) | 0xffffffu);
-        b = float_to_bits(y) >= kInf ? 255u << 24 : min(b, (254u << 24) | 0xffffffu);
-      }
-      cm[j] = (a & 0x7fffffffu) | (float_to_bits(x) & 0x80000000u);
-      cr[j] = b;
-    }
-    m8[w] = pack_top(cm);
-    r8[w] = pack_top(cr);
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t y = (((w[j] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | w[j]) & 0x80808080u;  // bytes that are not zero
+    const uint32_t d = step & (y | (y - (y >> 7)));
+    w[j] = by < 0 ? w[j] - d : w[j] + d;
   }
+  return fine && kept;
 }
 
-// A block of a tensor with rows of a multiple of sixteen elements by sixteen lanes (of which the block may be none of
-// the tensor's): sixteen elements a lane, which are of one row and of one block.
-template <bool kMove, bool kWide>
-__device__ inline void make_even(const MomentArgs& A, const MomentRecord& t, uint32_t block, bool make) {
-  typedef uint32_t vec __attribute__((ext_vector_type(4)));
-  const int lane = threadIdx.x & 15;
-  const uint32_t len = t.row_len;
-  const int64_t base = (int64_t)block * kMomBlock;
-  uint32_t at0;
-  const uint64_t row0 = first_row(t, base, at0);
-  const uint32_t e = at0 + lane * 16, q = row_of(t, e);
-  const int32_t row[1] = {(int32_t)(row0 + q)};
-  const bool in[1] = {make && base + lane * 16 < t.count};
-  int32_t s[1];
-  sources<kMove, kWide>(A, row, in, s);
-  vec wm{}, wr{};
-  uint32_t f = 0;
-  if (s[0] >= 0) {
-    const uint64_t at = (uint64_t)t.src_at * kMomBlock + (uint64_t)s[0] * len + (e - q * len);
-    wm = *reinterpret_cast<const vec*>(A.m8 + at);
-    wr = *reinterpret_cast<const vec*>(A.r8 + at);
-    f = *(const uint16_t*)(A.fields + 2 * (at >> 8));
-  }
-  float m[16], r[16];
+// The general way, as encode_block_odd: decode, and encode to nearest.  Everything is decoded twice, so that four values
+// at a time are in registers.
+__device__ inline void remake(vec4u& wm, vec4u& wr, uint32_t f, uint32_t& fields) {
+  constexpr uint32_t kInf = 0x7f800000u;
   uint32_t mm = 0, rr = 0;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
@@ -179,30 +159,127 @@ __device__ inline void make_even(const MomentArgs& A, const MomentRecord& t, uin
     decode_r4(wr[w], (int)(f >> 8), y);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      m[4 * w + j] = x[j];
-      r[4 * w + j] = y[j];
-      mm = max(mm, float_to_bits(x[j]) & 0x7fffffffu);
-      rr = max(rr, float_to_bits(y[j]));
+      const uint32_t a = float_to_bits(x[j]) & 0x7fffffffu, b = float_to_bits(y[j]);
+      mm = max(mm, a < kInf ? a : 0u);
+      rr = max(rr, b < kInf ? b : 0u);
     }
   }
-  uint32_t cm[4], cr[4], fields;
-  if (__ballot(mm >= 0x7e800000u || rr >= 0x7e800000u)) {  // as encode_block decides
-    mm = rr = 0;
+  row_max2_u32(mm, rr);
+  const uint32_t fm = moment_field<3>(mm), fr = moment_field<4>(rr);
+  fields = fm | (fr << 8);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const uint32_t x = float_to_bits(m[j]) & 0x7fffffffu, y = float_to_bits(r[j]);
-      mm = max(mm, x < 0x7f800000u ? x : 0u);
-      rr = max(rr, y < 0x7f800000u ? y : 0u);
+  for (int w = 0; w < 4; ++w) {
+    float x[4], y[4];
+    decode_m4(wm[w], (int)(f & 255u), x);
+    decode_r4(wr[w], (int)(f >> 8), y);
+    uint32_t cm[4], cr[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t a = float_to_bits(x[j]) & 0x7fffffffu, b = float_to_bits(y[j]);
+      const uint32_t c = a >= kInf ? 127u << 24 : min(moment_top<3, false>(bits_to_float(a), (int)fm, 0), (126u << 24) | 0xffffffu);
+      cm[j] = (c & 0x7fffffffu) | (float_to_bits(x[j]) & 0x80000000u);
+      cr[j] = b >= kInf ? 255u << 24 : min(moment_top<4, false>(y[j], (int)fr, 0), (254u << 24) | 0xffffffu);
     }
-    encode_sixteen<true>(m, r, mm, rr, cm, cr, fields);
-  } else {
-    encode_sixteen<false>(m, r, mm, rr, cm, cr, fields);
+    wm[w] = pack_top(cm);
+    wr[w] = pack_top(cr);
   }
-  if (!make) return;
-  const uint64_t to = (uint64_t)t.dst_at * kMomBlock + base + lane * 16;
-  *reinterpret_cast<vec*>(A.to_m8 + to) = vec{cm[0], cm[1], cm[2], cm[3]};
-  *reinterpret_cast<vec*>(A.to_r8 + to) = vec{cr[0], cr[1], cr[2], cr[3]};
-  if (lane == 0) *(uint16_t*)(A.to_fields + 2 * (to >> 8)) = (uint16_t)fields;
+}
+
+// Sixteen codes a lane, of a block in sixteen lanes, under the exponents of their new block.  The signed codes go through
+// the machine's scaled conversions, two values each, the roots' as integers; waves with values that are not finite, with
+// float32's least exponents or with roots under gradual underflow take the general way, with twice the instructions
+// (2M rows moved, 8 % at random: 83 us, 98 where all went that way).
+__device__ inline void recode(vec4u& wm, vec4u& wr, uint32_t f, uint32_t& fields) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  constexpr uint32_t kLeastField = 18;  // all values are normal float32s from here on
+  const uint32_t fm = f & 255u, fr = f >> 8;
+  const float scale = bits_to_float((max(fm, kLeastField) - 8u) << 23);
+  float m[16];
+  uint32_t mm = 0, some = 0;
+  pair most = 0, least = (uint16_t)0xffffu;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(wm[w], scale, false);
+    const f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(wm[w], scale, true);
+    m[4 * w] = a[0];
+    m[4 * w + 1] = a[1];
+    m[4 * w + 2] = b[0];
+    m[4 * w + 3] = b[1];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) mm = max(mm, float_to_bits(m[4 * w + j]) & 0x7fffffffu);
+    some |= wm[w];
+    const pair even = __builtin_bit_cast(pair, wr[w] & 0x00ff00ffu), odd = __builtin_bit_cast(pair, (wr[w] >> 8) & 0x00ff00ffu);
+    most = __builtin_elementwise_max(__builtin_elementwise_max(most, even), odd);
+    // zero becomes the largest
+    least = __builtin_elementwise_min(__builtin_elementwise_min(least, (pair)(even - (uint16_t)1)), (pair)(odd - (uint16_t)1));
+  }
+  const uint32_t top = max((uint32_t)most[0], (uint32_t)most[1]), low = min((uint32_t)least[0], (uint32_t)least[1]);
+  uint32_t key = top ? (fr * 16 + top) * 2 + (top >= 16 ? 1u : 0u) : 0u;
+  bool fine = mm < 0x7e800000u && top != 255u && (fm >= kLeastField || (some & 0x7f7f7f7fu) == 0);
+  row_max2_u32(mm, key);
+  const uint32_t to = moment_field<3>(mm);
+  fields = to;
+  vec4u roots = wr;
+  fine &= shift_roots(roots, fr, key, low, fields) && (mm == 0 || to >= kLeastField);
+  if (__ballot(!fine)) {
+    remake(wm, wr, f, fields);
+    return;
+  }
+  wr = roots;
+  const float down = bits_to_float((max(to, kLeastField) - 8u) << 23);
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    s16x2 c{};
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, m[4 * w], m[4 * w + 1], down, false);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, m[4 * w + 2], m[4 * w + 3], down, true);
+    wm[w] = __builtin_bit_cast(uint32_t, c);
+  }
+}
+
+// kEvenAhead blocks of a tensor with rows of a multiple of sixteen elements by sixteen lanes (those with `make`; the
+// others may be none of the tensor's): sixteen elements a lane, which are of one row and of one block.
+template <bool kMove, bool kWide>
+__device__ inline void make_even(const MomentArgs& A, const MomentRecord& t, const uint32_t (&block)[kEvenAhead],
+                                 const bool (&make)[kEvenAhead]) {
+  const int lane = threadIdx.x & 15;
+  const uint32_t len = t.row_len;
+  int32_t row[kEvenAhead], s[kEvenAhead];
+  uint32_t off[kEvenAhead];
+  bool in[kEvenAhead];
+#pragma unroll
+  for (int g = 0; g < kEvenAhead; ++g) {
+    const int64_t base = (int64_t)block[g] * kMomBlock;
+    uint32_t at0;
+    const uint64_t row0 = first_row(t, base, at0);
+    const uint32_t e = at0 + lane * 16, q = row_of(t, e);
+    row[g] = (int32_t)(row0 + q);
+    off[g] = e - q * len;
+    in[g] = make[g] && base + lane * 16 < t.count;
+  }
+  sources<kMove, kWide>(A, row, in, s);
+  vec4u wm[kEvenAhead], wr[kEvenAhead];
+  uint32_t f[kEvenAhead];
+#pragma unroll
+  for (int g = 0; g < kEvenAhead; ++g) {
+    wm[g] = wr[g] = vec4u{};
+    f[g] = 0;
+    if (s[g] < 0) continue;
+    const uint64_t at = (uint64_t)t.src_at * kMomBlock + (uint64_t)s[g] * len + off[g];
+    wm[g] = *reinterpret_cast<const vec4u*>(A.m8 + at);
+    wr[g] = *reinterpret_cast<const vec4u*>(A.r8 + at);
+    f[g] = *(const uint16_t*)(A.fields + 2 * (at >> 8));
+  }
+#pragma unroll
+  for (int g = 0; g < kEvenAhead; ++g) {
+    uint32_t fields;
+    recode(wm[g], wr[g], f[g], fields);
+    if (!make[g]) continue;
+    const uint64_t to = ((uint64_t)t.dst_at + block[g]) * kMomBlock + lane * 16;
+    *reinterpret_cast<vec4u*>(A.to_m8 + to) = wm[g];
+    *reinterpret_cast<vec4u*>(A.to_r8 + to) = wr[g];
+    if (lane == 0) *(uint16_t*)(A.to_fields + 2 * (to >> 8)) = (uint16_t)fields;
+  }
 }
 
 // Four bytes from `at` on, of which those that lie in the array are right.
@@ -329,14 +406,20 @@ __global__ __launch_bounds__(256) void moment_take_kernel(MomentArgs A) {
   if (b >= A.groups) return;
   const int k = tensor_of(A, b);
   const MomentRecord& t = A.t[k];
-  const uint32_t first =
-      __builtin_amdgcn_readfirstlane((b - A.begin[k]) * kTakeGroup + (threadIdx.x >> 6) * kMomentAhead);
-  if (first >= t.blocks) return;
+  const uint32_t group = (b - A.begin[k]) * t.group;
   if (t.row_len % 16 == 0) {
-    const uint32_t block = first + ((threadIdx.x >> 4) & 3);
-    make_even<false, kWide>(A, t, block, block < t.blocks);
+    uint32_t block[kEvenAhead];
+    bool make[kEvenAhead];
+#pragma unroll
+    for (int g = 0; g < kEvenAhead; ++g) {
+      block[g] = group + g * 16 + (threadIdx.x >> 4);
+      make[g] = block[g] < t.blocks;
+    }
+    make_even<false, kWide>(A, t, block, make);
     return;
   }
+  const uint32_t first = __builtin_amdgcn_readfirstlane(group + (threadIdx.x >> 6) * kMomentAhead);
+  if (first >= t.blocks) return;
   uint32_t block[kMomentAhead];
 #pragma unroll
   for (int g = 0; g < kMomentAhead; ++g) block[g] = first + g;
@@ -395,7 +478,16 @@ __global__ __launch_bounds__(256) void moment_move_kernel(MomentArgs A) {
   __syncthreads();
   const int n = __popcll(bits);
   if (len % 16 == 0) {
-    for (int i = threadIdx.x >> 4; (i & ~3) < n; i += 16) make_even<true, kWide>(A, t, first + list[min(i, n - 1)], i < n);
+    for (int i = threadIdx.x >> 4; (i & ~3) < n; i += 16 * kEvenAhead) {
+      uint32_t block[kEvenAhead];
+      bool make[kEvenAhead];
+#pragma unroll
+      for (int g = 0; g < kEvenAhead; ++g) {
+        make[g] = i + 16 * g < n;
+        block[g] = first + list[min(i + 16 * g, n - 1)];
+      }
+      make_even<true, kWide>(A, t, block, make);
+    }
     return;
   }
   for (int i = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * kMomentAhead; i < n; i += 4 * kMomentAhead) {
@@ -455,7 +547,7 @@ int launch(int what, hipStream_t stream, int num, const int64_t* row_lens, const
     for (; i < num && k < kMomentTensors; ++i) {
       const int64_t elements = row_lens[i] * count, blocks = (elements + kMomBlock - 1) / kMomBlock;
       if (blocks == 0) continue;
-      const int64_t per = what == kTake ? kTakeGroup : row_lens[i] < 16 ? 16 : kMoveGroup, more = (blocks + per - 1) / per;
+      const int64_t per = what != kTake ? (row_lens[i] < 16 ? 16 : kMoveGroup) : row_lens[i] % 16 ? kTakeGroup : 16 * kEvenAhead, more = (blocks + per - 1) / per;
       GS_REQUIRE(more <= kMaxGroups, "gs_moments: tensor %d is too large", i);
       if (groups + more > kMaxGroups) break;
       MomentRecord& t = A.t[k];
