@@ -358,14 +358,16 @@ __global__ __launch_bounds__(kBestBlock) void best_write_kernel(BestArgs A) {
 
 template <int kType>
 int best_rows(hipStream_t s, BestArgs& A) {
-  if (A.n <= kBestOne * kOneTile) {
+  // (what it writes behind the last row takes one workgroup long, where that is much more)
+  if (A.n <= kBestOne * kOneTile && A.k <= 16 * kBestOne * kOneTile) {
     hipLaunchKernelGGL(best_one_kernel<kType>, dim3(1), dim3(kOneBlock), 0, s, A);
     GS_LAUNCH_CHECK("best_one_kernel");
     return GS_OK;
   }
   const int64_t tiles = (A.n + kBestTile - 1) / kBestTile;
-  A.tiles = (tiles + kBestGroups - 1) / kBestGroups;
-  const dim3 grid((unsigned)((tiles + A.tiles - 1) / A.tiles));
+  A.tiles = std::max<int64_t>((tiles + kBestGroups - 1) / kBestGroups, 1);
+  const int64_t groups = (tiles + A.tiles - 1) / A.tiles;
+  const dim3 grid((unsigned)std::max(groups, std::min<int64_t>(A.k >> 16, kBestGroups)));
   constexpr int kDigits = kType == kAlike ? 0 : kType == GS_TYPE_F32 ? 3 : 2;
   if (kDigits) {
     hipLaunchKernelGGL(best_clear_kernel, dim3(1), dim3(kBestBlock), 0, s, A.ctl);

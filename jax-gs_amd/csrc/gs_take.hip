@@ -452,6 +452,7 @@ extern "C" int gs_move_rows(void* stream, int num, void* const* tensors, const i
       // arrays, the last 5 % change, 12.7 us by 64, 17.8 by 128, 29.9 by 256; but 3M rows of four tensors, one in six
       // changes, 109, 82 and 69
       M.tile = rows <= ((int64_t)1 << 18) ? 64 : rows <= ((int64_t)1 << 19) ? 128 : kMoveRows;
+      while (M.tile > 32 && M.tile * pieces > 16384 && div_up(rows, M.tile / 2) <= kMaxGroups) M.tile /= 2;
     } else {
       const int64_t fit = kWidePieces / std::min<int64_t>(most, kWidePieces);
       M.tile = (int)std::min<int64_t>(fit, 64);

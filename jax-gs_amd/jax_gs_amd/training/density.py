@@ -82,6 +82,8 @@ def densify_and_prune(state: DensityState, generator: Optional[torch.Generator] 
     opt = state.opt_state
     # 8-bit moments follow the other arrays by the index of sources
     after = opt is not None and getattr(opt, "bits", 32) == 8
+    if after and (opt._rows("move_rows_")[0] != M or opt.mu_flat.device != dev):
+        raise ValueError(f"densify_and_prune: the optimizer's state must have the capacity rows, on {dev}")
     if opt is not None and not after:
         mu, nu = opt.mu, opt.nu
         moments = [mu[f] for f in FIELDS] + [nu[f] for f in FIELDS]

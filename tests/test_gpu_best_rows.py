@@ -93,3 +93,15 @@ def test_no_rows_and_strided_scores(cuda):
         best_rows(x.double().to(cuda)[:, 0], 5)
     with pytest.raises(ValueError, match="active_mask"):
         best_rows(x.to(cuda)[:, 0], 5, active_mask=torch.ones(999, device=cuda))
+
+
+@pytest.mark.parametrize("n", [0, 3, 5000, 40_000])
+def test_many_more_than_there_are(cuda, n):
+    """What lies behind the last row is written by many workgroups."""
+    scores = some_scores(n, "normal", 1) if n else torch.zeros(0)
+    for k in (300_000, 20_000_001):
+        for x, mask in ((scores, None), (None, torch.arange(n) % 3 > 0)):
+            got = best_rows(None if x is None else x.to(cuda), k, None if mask is None else mask.to(cuda))
+            rows = torch.arange(n, device=cuda, dtype=torch.int32)
+            rows = rows if mask is None else rows[mask.to(cuda)]
+            assert torch.equal(got[:len(rows)], rows) and bool((got[len(rows):] == -1).all())

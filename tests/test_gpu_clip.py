@@ -124,6 +124,20 @@ def test_many_tensors_and_large_ones(cuda):
     check(g, clip_grads_(g, 3.0), want)
 
 
+def test_very_many_tensors_and_none(cuda):
+    """More partial sums than every workgroup would add for itself, and no elements at all."""
+    g = [some((1 + i % 7,), i, torch.float32, cuda) for i in range(5000)]
+    want = want_clipped(g, 3.0)
+    norms = clip_grads_(g, 3.0)
+    check(g, norms, want)
+    each = grad_norms(g).per_tensor
+    assert norms.per_tensor.shape == each.shape and bool(torch.isfinite(norms.per_tensor).all())
+    for none in ([torch.zeros(0, device=cuda)], [None, torch.zeros(0, 3, device=cuda), None]):
+        norms = clip_grads_(none, 1.0)
+        assert float(norms.total) == 0.0 and float(norms.scale) == 1.0 and not bool(norms.per_tensor.any())
+    assert float(clip_grads_([g[0]], float("inf")).scale) == 1.0
+
+
 def test_captured_and_replayed(cuda):
     g = [torch.randn(70_000, device=cuda), torch.randn(333, 3, device=cuda).bfloat16()]
     clip_grads_([x.clone() for x in g], 1.0)

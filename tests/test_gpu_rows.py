@@ -160,6 +160,21 @@ def test_move_rows(cuda, n, dtype):
         np.testing.assert_array_equal(raw(got), raw(want_taken(x, index)))
 
 
+@pytest.mark.parametrize("n, row", [(300, 2048), (300, 8000), (70, 9000), (5, 70_000), (1025, 700)])
+def test_wide_rows_move(cuda, n, row):
+    """Rows of up to many workgroups' pieces, by themselves and beside short ones, all changed rows together and scattered."""
+    tensors = [bits((n, row), torch.uint8, 1, cuda), bits((n, 3), torch.float32, 2, cuda), bits((n, row + 1), torch.uint8, 3, cuda),
+               bits((n,), torch.float16, 4, cuda)]
+    end = torch.arange(n)
+    end[n - n // 3:] = torch.arange(n // 3)
+    for index in (a_move(n, row, torch.int32), end):
+        for some in (tensors[:1], tensors):
+            before = [t.clone() for t in some]
+            move_rows_(some, index.to(cuda))
+            for x, got in zip(before, some):
+                np.testing.assert_array_equal(raw(got), raw(want_taken(x, index)))
+
+
 def test_move_rows_between_others(cuda):
     """Halves of a pool's pages with other pages between: what is not theirs stays; fills."""
     pool = bits((400, 3, 10), torch.float16, 1, cuda)
@@ -499,6 +514,14 @@ def test_device_refusals(cuda):
     state = AdamW(1e-3, moment_bits=8).init([x])
     with pytest.raises(ValueError, match="4 indices for 5 rows"):
         state.move_rows_(index[:4])
+    other = a_state(cuda, AdamW(RATES, moment_bits=8))
+    other.opt_state = AdamW(RATES, moment_bits=8).init(take_rows(other.gaussians, index))
+    before = other.active_mask.clone()
+    with pytest.raises(ValueError, match="capacity rows"):
+        from jax_gs_amd.training.density import densify_and_prune
+
+        densify_and_prune(other, extent=1e-3)
+    assert torch.equal(other.active_mask, before)
     with pytest.raises(ValueError, match="capacity 0"):
         from jax_gs_amd.training.density import resize_density_state
 

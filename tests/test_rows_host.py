@@ -194,6 +194,12 @@ def test_rows_of_a_list_are_looked_over():
             call()
 
 
+def test_no_memory_is_an_error_of_its_kind():
+    """2^31 rows of 2^31 bytes: the allocator's own error, not a process that ends."""
+    with pytest.raises(RuntimeError, match="[Mm]emory|alloc"):
+        _lib.tensors().take([torch.zeros(1, 1 << 20).expand(1, 1 << 20)], None, 1 << 38, -1, "take_rows")
+
+
 def test_overlapping_rows_are_refused():
     move, dense = _lib.tensors().move, _lib.tensors().dense
     index = torch.zeros(6, dtype=torch.int32)
