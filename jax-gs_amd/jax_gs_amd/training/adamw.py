@@ -285,14 +285,15 @@ class AdamWState:
                 mu, nu, fields, self.mu_flat, self.nu_flat)))
 
     def _rows(self, what: str):
-        """(rows, elements per row of each tensor, the same as int64, bytes per row in 32 bits) of a state whose
-        tensors have the same rows."""
+        """(rows, elements per row of each tensor, the same as int64, bytes per row in 32 bits, a row's shapes) of a
+        state whose tensors have the same rows."""
         if self._row_layout is None:
             rows = self.shapes[0][0] if len(self.shapes[0]) else None
             if any([not len(s) or s[0] != rows for s in self.shapes]):
                 raise ValueError(f"AdamWState.{what}: the state's tensors do not have the same rows")
             lens = [s[1:].numel() for s in self.shapes]
-            self._row_layout = rows, lens, array("q", lens).tobytes(), array("q", [4 * n for n in lens]).tobytes()
+            self._row_layout = (rows, lens, array("q", lens).tobytes(), array("q", [4 * n for n in lens]).tobytes(),
+                                [tuple(s[1:]) for s in self.shapes])
         return self._row_layout
 
     def _flats(self) -> list:
@@ -311,14 +312,14 @@ class AdamWState:
         moments are rounded to nearest where a new neighbour raises the exponent of their block."""
         dev = self.mu_flat.device
         index = row_index(index, dev, "AdamWState.take_rows")
-        rows, lens, lens_bytes, row_bytes = self._rows("take_rows")
+        rows, lens, lens_bytes, row_bytes, row_shapes = self._rows("take_rows")
         count, k = index.numel(), len(lens)
         to = AdamWState.__new__(AdamWState)
         to.__dict__.update(self.__dict__)  # the powers are never written in place
         to.norms = None
-        to.shapes = [torch.Size((count, *s[1:])) for s in self.shapes]
+        to.shapes = [torch.Size((count, *s)) for s in row_shapes]
         to._lay_out([n * count for n in lens])
-        to._row_layout = count, lens, lens_bytes, row_bytes
+        to._row_layout = count, lens, lens_bytes, row_bytes, row_shapes
         with _lib.on(dev):
             to._allocate(dev, zero=False)
             if self.master_flat is not None:
@@ -341,7 +342,7 @@ class AdamWState:
         is negative, as ``rows.move_rows_`` moves the parameters.  Returns the state."""
         dev = self.mu_flat.device
         index = row_index(index, dev, "AdamWState.move_rows_")
-        rows, lens, lens_bytes, row_bytes = self._rows("move_rows_")
+        rows, lens, lens_bytes, row_bytes, _ = self._rows("move_rows_")
         if index.numel() != rows:
             raise ValueError(f"AdamWState.move_rows_: {index.numel()} indices for {rows} rows")
         k = len(lens)

@@ -104,10 +104,10 @@ class Adam:
         return state
 
 
-def make_optimizer(extent: float, num_iterations: int) -> Adam:
+def make_optimizer(extent: float, num_iterations: int, max_grad_norm: Optional[float] = None) -> Adam:
     """train.py:127-155: means 0.00016*extent*3 decaying to 0.0000016*extent*3 over the
-    run; scales 0.005, quaternions 0.001, opacities 0.05, SH 0.0025."""
+    run; scales 0.005, quaternions 0.001, opacities 0.05, SH 0.0025.  ``max_grad_norm``: as Adam's."""
     lr_init = 0.00016 * extent * 3.0
     lr_end = 0.0000016 * extent * 3.0
     return Adam({"means": exponential_decay(lr_init, num_iterations, lr_end / lr_init), "scales": 0.005,
-                 "quaternions": 0.001, "opacities": 0.05, "sh_coeffs": 0.0025})
+                 "quaternions": 0.001, "opacities": 0.05, "sh_coeffs": 0.0025}, max_grad_norm=max_grad_norm)

@@ -428,6 +428,47 @@ def test_what_else_a_program_keeps_follows_density_control(cuda, opt):
     assert densify_and_prune(state, densify_enabled=False).last_sources is not None
 
 
+@pytest.mark.parametrize("kind", ["adam", "8"])
+def test_a_run_with_all_of_them(cuda, kind):
+    """Clipped steps, density control with a table of features, a cut to a budget and a larger capacity, in turn: training
+    goes on, the features stay with their Gaussians, and what is rendered does not change by a resize."""
+    from jax_gs_amd import render, scenes
+    from jax_gs_amd.training.adamw import make_adamw
+    from jax_gs_amd.training.density import densify_and_prune, init_density_state, resize_density_state
+    from jax_gs_amd.training.optimizer import make_optimizer
+    from jax_gs_amd.training.trainer import train_step
+
+    sc = scenes.make_scene(1, n=1500, width=96, height=64)
+    g, cam, tgt, _ = scenes.to_torch(sc, "cuda:0")
+    opt = make_optimizer(1.0, 100, max_grad_norm=0.01) if kind == "adam" else make_adamw(1.0, 100, moment_bits=8, max_grad_norm=0.01)
+    static = (cam.W, cam.H, cam.fx, cam.fy, cam.cx, cam.cy)
+    state = init_density_state(g, opt, 2000)
+    features = torch.randn(2000, 5, device=cuda).half()
+    for round in range(3):
+        for _ in range(3):
+            state, loss, metrics = train_step(state, tgt, cam.W2C, static, opt, sh_degree=3)
+            assert bool(torch.isfinite(loss)) and bool(torch.isfinite(metrics["grad_norm"]))
+        state.grad_accum.zero_()
+        state.grad_accum[:200], state.denom[:200] = 1.0, 1
+        tag = state.gaussians.quaternions.clone()
+        densify_and_prune(state, extent=5.0, sources=True, generator=torch.Generator(device=cuda).manual_seed(round))
+        assert int(state.last_counts[0] + state.last_counts[1]) > 0
+        move_rows_([features, tag], state.last_sources)
+        assert torch.equal(tag, state.gaussians.quaternions)
+        active = int(state.active_mask.sum())
+        # to a capacity that holds them all, then to a smaller budget, then to a larger capacity
+        for capacity in (active, 1200, 2500):
+            keep = best_rows(state.gaussians.opacities.reshape(-1), capacity, state.active_mask)
+            before = render(state.gaussians, cam, mask=state.active_mask.bool(), sh_degree=3)[0]
+            state, features, old = resize_density_state(state, capacity), take_rows(features, keep), features
+            k = state.num_active
+            assert torch.equal(features[:k], old[keep[:k].long()]) and not bool(features[k:].any())
+            if capacity != 1200:
+                after = render(state.gaussians, cam, mask=state.active_mask.bool(), sh_degree=3)[0]
+                assert torch.equal(before, after)
+    assert state.opt_state.count == 9 and state.gaussians.means.shape[0] == 2500
+
+
 def test_sources_only_where_they_are_asked_for(cuda):
     from jax_gs_amd.training.density import densify_and_prune
 

@@ -2,6 +2,7 @@
 import ctypes
 from array import array
 
+import numpy as np
 import pytest
 import torch
 
@@ -260,3 +261,26 @@ def test_states_of_different_rows_have_no_rows():
             AdamWState(None, shapes, 32)._rows("take_rows")
     rows, lens, *_ = AdamWState(None, ((5, 2, 3), (5,), (5, 0)), 8)._rows("take_rows")
     assert rows == 5 and lens == [6, 1, 0]
+
+
+def exact(d, magic, largest):
+    """Whether the upper half of e * magic is e // d for all e up to the largest."""
+    e = np.arange(largest + 1, dtype=np.uint64)
+    return np.array_equal((e * np.uint64(magic)) >> np.uint64(32), e // np.uint64(d))
+
+
+def test_reciprocals_are_exact_where_they_are_used():
+    """floor(2^32 / d) + 1 in place of a division: rows of up to 8192 bytes with offsets below a row and a workgroup's 8192;
+    up to 256 rows by up to 512 pieces of all tensors, 64 rows by up to 4096 pieces of one, rows by rows that move;
+    moments' rows of up to 4096 elements, where it is the upper half of floor(2^64 / d) + 1, plus 1."""
+    plain = lambda d: (1 << 32) // d + 1
+    for d in [*range(2, 260), *range(260, 8193, 37), 4095, 4096, 4097, 8191, 8192]:
+        assert exact(d, plain(d), d + 8192), d
+    for m in range(2, 257):
+        assert exact(m, 0xFFFFFFFF // m + 1, m * 512 - 1), m
+    for pieces in [*range(2, 513, 7), 511, 512]:
+        assert exact(pieces, plain(pieces), 256 * pieces - 1), pieces
+    for pieces in [*range(2, 4097, 61), 4095, 4096]:
+        assert exact(pieces, 0xFFFFFFFF // pieces + 1, 64 * pieces - 1), pieces
+    for d in [*range(2, 4097, 13), 4095, 4096]:
+        assert exact(d, (((1 << 64) // d + 1 if d & (d - 1) else (1 << 64) // d + 0) >> 32) + 1, d + 256), d
