@@ -74,17 +74,11 @@ __device__ inline const char* row_ptr(const RowRecord& t, int32_t s) { return s 
 
 // The 16 bytes that begin `k` bytes before the end of a (1 <= k <= 15) and go on with b.
 __device__ inline vec16 join(vec16 a, vec16 b, uint32_t k) {
-  // words w[0..7] = a, b; the result begins at byte 16 - k
-  const uint32_t at = 16 - k, word = at >> 2, byte = at & 3;
+  const uint32_t w[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  const uint32_t word = (16 - k) >> 2, byte = (16 - k) & 3;  // where they begin
   uint32_t x[5];
 #pragma unroll
-  for (int j = 0; j < 5; ++j) {
-    const uint32_t w0 = j < 4 ? a[j] : b[0];
-    const uint32_t w1 = j < 3 ? a[j + 1] : b[j - 3];
-    const uint32_t w2 = j < 2 ? a[j + 2] : b[j - 2];
-    const uint32_t w3 = j < 1 ? a[3] : j < 5 ? b[j < 1 ? 0 : j - 1] : 0;
-    x[j] = word == 0 ? w0 : word == 1 ? w1 : word == 2 ? w2 : w3;
-  }
+  for (int j = 0; j < 5; ++j) x[j] = word == 0 ? w[j] : word == 1 ? w[j + 1] : word == 2 ? w[j + 2] : w[j + 3];
   vec16 r;
 #pragma unroll
   for (int j = 0; j < 4; ++j) r[j] = __builtin_amdgcn_alignbyte(x[j + 1], x[j], byte);
@@ -363,7 +357,7 @@ extern "C" int gs_take_rows(void* stream, int num, const void* const* tensors, c
   for (int i = 0; i < num; ++i) {
     GS_REQUIRE(row_bytes[i] >= 0 && row_bytes[i] < kMaxRowBytes, "gs_take_rows: rows of %lld bytes", (long long)row_bytes[i]);
     const int64_t need = row_bytes[i] * count, all = out_bytes ? out_bytes[i] : need;
-    GS_REQUIRE(all >= need && all < ((int64_t)1 << 38) && (all == 0 || row_bytes[i] > 0), "gs_take_rows: output %d of %lld bytes for %lld", i,
+    GS_REQUIRE(all >= need && all <= kMaxGroups * kTakeBytes && (all == 0 || row_bytes[i] > 0), "gs_take_rows: output %d of %lld bytes for %lld", i,
                (long long)all, (long long)need);
     GS_REQUIRE(all == 0 || out[i], "gs_take_rows: NULL output %d", i);
     GS_REQUIRE(need == 0 || rows == 0 || tensors[i], "gs_take_rows: NULL tensor %d", i);
@@ -384,7 +378,6 @@ extern "C" int gs_take_rows(void* stream, int num, const void* const* tensors, c
       const int64_t all = out_bytes ? out_bytes[i] : row_bytes[i] * count;
       if (all == 0) continue;
       const int64_t per = row_bytes[i] < 16 ? kTakeRows * row_bytes[i] : kTakeBytes, more = (all + per - 1) / per;
-      GS_REQUIRE(more <= kMaxGroups, "gs_take_rows: output %d of %lld bytes", i, (long long)all);
       if (groups + more > kMaxGroups) break;
       RowRecord& t = A.t[k];
       t.src = (const char*)tensors[i];
@@ -394,7 +387,7 @@ extern "C" int gs_take_rows(void* stream, int num, const void* const* tensors, c
       t.bytes = all;
       t.row = (uint32_t)row_bytes[i];
       t.magic = reciprocal(t.row);
-      // exact for offsets times rows below 2^64; outputs stay below 2^38 bytes
+      // exact for offsets times rows below 2^64; outputs stay below 2^37 bytes
       t.magic64 = row_bytes[i] < ((int64_t)1 << 26) ? ~(uint64_t)0 / t.row + 1 : 0;
       A.begin[k++] = (uint32_t)groups;
       groups += more;

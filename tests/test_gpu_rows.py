@@ -313,6 +313,42 @@ def test_moments_that_are_not_finite_and_tiny_ones_move(cuda):
     assert bool((nu[300:] > 0).all()) and torch.equal(mu[300:], before[0][300:])
 
 
+@pytest.mark.parametrize("row", [16, 48, 64, 272, 3, 4, 1, 45])
+@pytest.mark.parametrize("kind", ["near", "wide", "tiny", "odd"])
+def test_moments_of_all_sizes_side_by_side(cuda, row, kind):
+    """Rows whose exponents differ a little, by all of float32's range, lie at its lower end, and with values that are not finite
+    and rows of zeros between: what the way by 32 bits gives, value by value."""
+    n = 1200
+    gen = torch.Generator().manual_seed(row)
+    low, high = {"near": (-2, 2), "wide": (-37, 37), "tiny": (-44, -30), "odd": (-20, 20)}[kind]
+    size = 10.0 ** (torch.rand(n, 1, generator=gen).double() * (high - low) + low)
+    m = (torch.randn(n, row, generator=gen).double() * size).float()
+    # roots whose squares are float32s: the way by 32 bits goes through them
+    size = 10.0 ** (torch.rand(n, 1, generator=gen).double() * (min(high, 18) - max(low, -18)) + max(low, -18))
+    v = ((torch.rand(n, row, generator=gen).double() * size) ** 2).clamp(max=1e37).float()
+    zero = torch.rand(n, generator=gen) < 0.2
+    m[zero], v[zero] = 0.0, 0.0
+    if kind == "odd":
+        for value in (float("nan"), float("inf"), -float("inf")):
+            m[torch.rand(n, row, generator=gen) < 3e-4] = value
+        v[torch.rand(n, row, generator=gen) < 3e-4] = float("inf")
+    opt = AdamW(1e-3, moment_bits=8)
+    state = opt.restore([torch.zeros(n, row, device=cuda)], [m.to(cuda)], [v.to(cuda)], 1)
+    was = [x[0].cpu() for x in state.moments()]
+
+    def check(got, index):
+        rows = [want_taken(x, index).to(cuda) for x in was]
+        want = opt.restore([torch.zeros_like(rows[0])], [rows[0]], [rows[1]], 1)
+        for a, b in zip(got.moments(), want.moments()):
+            a, b = a[0].cpu(), b[0].cpu()
+            assert torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(a.nan_to_num(), b.nan_to_num())
+
+    for index in (an_index(n, 1500, row, torch.int32), torch.randperm(n, generator=gen)):
+        check(state.take_rows(index.to(cuda)), index)
+    index = a_move(n, row, torch.int32, moved=0.1, freed=0.05)
+    check(state.move_rows_(index.to(cuda)), index)
+
+
 def test_masters_follow(cuda):
     for moment_bits in (32, 8):
         p = [torch.randn(200, 3, device=cuda).bfloat16(), torch.randn(200, device=cuda).half()]
