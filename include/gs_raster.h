@@ -614,8 +614,8 @@ int gs_moments_take(void* stream, int num, const int64_t* row_lens, int64_t rows
                     int64_t out_size, uint8_t* out_mu8, uint8_t* out_nu8, uint8_t* out_fields);
 
 /* gs_move_rows of moments in 8 bits; freed rows become zero.  workspace: 16-byte aligned, of
- * gs_moments_move_workspace_size(state_size) bytes. */
-size_t gs_moments_move_workspace_size(int64_t state_size);
+ * gs_moments_move_workspace_size(num, row_lens, rows) bytes (0 for a bad size). */
+size_t gs_moments_move_workspace_size(int num, const int64_t* row_lens, int64_t rows);
 int gs_moments_move(void* stream, int num, const int64_t* row_lens, int64_t rows, const int64_t* offsets,
                     int64_t state_size, uint8_t* mu8, uint8_t* nu8, uint8_t* fields, const void* index,
                     int index_bits, void* workspace, size_t workspace_bytes);

@@ -5,13 +5,16 @@
 // its rows come from and encoded again, to nearest even.  Values come back as they were but where a
 // larger neighbour raises the exponent of their block.
 //
-// Sixteen lanes make two blocks where rows are a multiple of sixteen elements, else a wave four, four elements of each a
-// lane, with all loads under way before the first is encoded.  In a move a workgroup first finds which of its 64 blocks
-// hold a changed row, and makes those; they go to a copy first, for a block is read by others while it changes.
+// Taken: sixteen lanes make two blocks where rows are a multiple of sixteen elements, else a wave four, four elements of each
+// a lane, with all loads under way before the first is encoded.  70 % of 2M rows of 48 elements: 63 us, bound by memory (at
+// 5.4 TB/s with the lines of rows that are skipped); of the Gaussians' five tensors 92, where the 11 of 59 elements in
+// short rows take 30: their fields and codes come element by element.
 //
-// 70 % of 2M rows of 48 elements taken: 63 us, bound by memory (at 5.4 TB/s with the lines of rows that are skipped); of the
-// Gaussians' five tensors 92, where the 11 of 59 elements in short rows take 30: their fields and codes come element by
-// element.  2M Gaussians moved, 8 % at random: 182 us, 8 % at the end 60, none 26.
+// Moved: a first launch looks the index over, marks the rows that change bit by bit, and copies the codes and exponents
+// that they get; a second (one for each kind of rows, as they want registers or waves) makes the blocks that hold such a row
+// anew, in place, from their own codes and those.  So no block is read by others while it changes, and blocks without a
+// changed row are not touched.  2M Gaussians, 8 % of them at random: 139 us (187 where changed blocks went to a copy and
+// back, and each tensor looked the index over), 8 % at the end 62 (60), none 17 (27).
 #include "gs_moments.h"
 #include "gs_pieces.h"
 #include "gs_rows.h"
@@ -23,9 +26,11 @@ namespace {
 
 constexpr int kMomentTensors = 72;  // per launch: the argument block stays below 4 KiB
 constexpr int kMomentAhead = 4;     // blocks per wave
-constexpr int kTakeGroup = 4 * kMomentAhead;  // per workgroup
+constexpr int kOddGroup = 4 * kMomentAhead;  // per workgroup
 constexpr int kEvenAhead = 2;       // blocks of sixteen lanes (1.5M rows of 48 taken: 63 us, one 70, four 68)
-constexpr int kMoveGroup = 64;      // in a move; 16 with rows of fewer elements than 16, of which they hold as many rows
+constexpr int kEvenGroup = 16 * kEvenAhead;
+constexpr int kRemakeGroup = 64;    // in a move's second launch
+constexpr int kOddAhead = 2;        // blocks of a wave there (139 us; four 148)
 
 struct MomentRecord {
   int64_t count;     // elements behind which there is nothing
@@ -33,7 +38,6 @@ struct MomentRecord {
   uint32_t src_at, dst_at;  // blocks
   uint32_t row_len;
   uint32_t blocks;
-  uint32_t group;    // blocks per workgroup
 };
 
 struct MomentArgs {
@@ -41,19 +45,17 @@ struct MomentArgs {
   uint32_t begin[kMomentTensors];
   const uint8_t *m8, *r8, *fields;
   uint8_t *to_m8, *to_r8, *to_fields;
-  uint64_t* changed;  // per workgroup of a move: its blocks, bit by bit
   int64_t state_size;
   const void* index;
   uint32_t rows;     // of the tensors that are read
   int32_t n;
   uint32_t groups;
-  int32_t wide;
 };
 static_assert(sizeof(MomentArgs) <= 4096, "kernel arguments");
 
 // Entry i of the index: a row, -1 for a negative one, -2 for one beyond the rows.
-template <bool kWide>
-__device__ inline int32_t entry(const MomentArgs& A, int64_t i) {
+template <bool kWide, class Args>
+__device__ inline int32_t entry(const Args& A, int64_t i) {
   if constexpr (kWide) {
     const int64_t x = ((const int64_t*)A.index)[i];
     return x < 0 ? -1 : x < (int64_t)A.rows ? (int32_t)x : -2;
@@ -63,35 +65,19 @@ __device__ inline int32_t entry(const MomentArgs& A, int64_t i) {
   }
 }
 
-// Where the rows come from, negative for nowhere, from their entries, all loads under way at once: in a move a row stays
-// whose source does not.
-template <bool kMove, bool kWide, int kN>
+// Where the rows come from, negative for nowhere.
+template <bool kWide, int kN>
 __device__ inline void sources(const MomentArgs& A, const int32_t (&row)[kN], const bool (&in)[kN], int32_t (&s)[kN]) {
 #pragma unroll
   for (int j = 0; j < kN; ++j) s[j] = entry<kWide>(A, in[j] ? row[j] : 0);
-  if (kMove) {
-    bool check = false;
-#pragma unroll
-    for (int j = 0; j < kN; ++j) {
-      if (s[j] == -2) s[j] = row[j];
-      check |= in[j] && s[j] >= 0 && s[j] != row[j];
-    }
-    if (__ballot(check)) {
-      int32_t of[kN];
-#pragma unroll
-      for (int j = 0; j < kN; ++j) of[j] = entry<kWide>(A, s[j] >= 0 ? s[j] : 0);
-#pragma unroll
-      for (int j = 0; j < kN; ++j)
-        if (s[j] >= 0 && of[j] != s[j]) s[j] = row[j];
-    }
-  }
 #pragma unroll
   for (int j = 0; j < kN; ++j)
     if (!in[j]) s[j] = -1;
 }
 
 // The tensor of this workgroup: the last that begins at or before it.
-__device__ inline int tensor_of(const MomentArgs& A, uint32_t b) {
+template <class Args>
+__device__ inline int tensor_of(const Args& A, uint32_t b) {
   const int lane = threadIdx.x & 63;
   int k = -1;
   for (int at = 0; at < A.n; at += 64) k += __popcll(__ballot(at + lane < A.n && b >= A.begin[min(at + lane, A.n - 1)]));
@@ -99,13 +85,15 @@ __device__ inline int tensor_of(const MomentArgs& A, uint32_t b) {
 }
 
 // A block's first row, and how far into it the block begins.
-__device__ inline uint64_t first_row(const MomentRecord& t, int64_t base, uint32_t& at) {
+template <class Record>
+__device__ inline uint64_t first_row(const Record& t, int64_t base, uint32_t& at) {
   const uint64_t row = t.magic ? __umul64hi((uint64_t)base, t.magic) : (uint64_t)base;
   at = (uint32_t)((uint64_t)base - row * t.row_len);
   return row;
 }
 // The row of element e from a block's first row on, e less than row_len + 256.
-__device__ inline uint32_t row_of(const MomentRecord& t, uint32_t e) {
+template <class Record>
+__device__ inline uint32_t row_of(const Record& t, uint32_t e) {
   return t.row_len > 4096u ? (e >= t.row_len ? 1u : 0u) : t.magic ? __umulhi(e, (uint32_t)(t.magic >> 32) + 1u) : e;
 }
 
@@ -187,8 +175,7 @@ __device__ inline void remake(vec4u& wm, vec4u& wr, uint32_t f, uint32_t& fields
 
 // Sixteen codes a lane, of a block in sixteen lanes, under the exponents of their new block.  The signed codes go through
 // the machine's scaled conversions, two values each, the roots' as integers; waves with values that are not finite, with
-// float32's least exponents or with roots under gradual underflow take the general way, with twice the instructions
-// (2M rows moved, 8 % at random: 83 us, 98 where all went that way).
+// float32's least exponents or with roots under gradual underflow take the general way, with twice the instructions.
 __device__ inline void recode(vec4u& wm, vec4u& wr, uint32_t f, uint32_t& fields) {
   typedef float f32x2 __attribute__((ext_vector_type(2)));
   typedef short s16x2 __attribute__((ext_vector_type(2)));
@@ -239,7 +226,7 @@ __device__ inline void recode(vec4u& wm, vec4u& wr, uint32_t f, uint32_t& fields
 
 // kEvenAhead blocks of a tensor with rows of a multiple of sixteen elements by sixteen lanes (those with `make`; the
 // others may be none of the tensor's): sixteen elements a lane, which are of one row and of one block.
-template <bool kMove, bool kWide>
+template <bool kWide>
 __device__ inline void make_even(const MomentArgs& A, const MomentRecord& t, const uint32_t (&block)[kEvenAhead],
                                  const bool (&make)[kEvenAhead]) {
   const int lane = threadIdx.x & 15;
@@ -257,7 +244,7 @@ __device__ inline void make_even(const MomentArgs& A, const MomentRecord& t, con
     off[g] = e - q * len;
     in[g] = make[g] && base + lane * 16 < t.count;
   }
-  sources<kMove, kWide>(A, row, in, s);
+  sources<kWide>(A, row, in, s);
   vec4u wm[kEvenAhead], wr[kEvenAhead];
   uint32_t f[kEvenAhead];
 #pragma unroll
@@ -291,7 +278,7 @@ __device__ inline uint32_t four_at(const uint8_t* p, uint64_t at, uint64_t size)
 
 // Four blocks (the same for the wave, none beyond `some`) of a tensor with other rows, four elements of each a lane.
 // kOf rows they can be of: 1 with rows of a multiple of four elements, 2 with rows of three and more, 4.
-template <bool kMove, bool kWide, int kOf>
+template <bool kWide, int kOf>
 __device__ inline void make_odd(const MomentArgs& A, const MomentRecord& t, const uint32_t (&block)[kMomentAhead], int some) {
   constexpr int kN = kMomentAhead * kOf;
   const uint32_t len = t.row_len, l = (threadIdx.x & 63) * 4;
@@ -324,7 +311,7 @@ __device__ inline void make_odd(const MomentArgs& A, const MomentRecord& t, cons
       }
     }
   }
-  sources<kMove, kWide>(A, row, in, s);
+  sources<kWide>(A, row, in, s);
   const uint64_t from = (uint64_t)t.src_at * kMomBlock, size = (uint64_t)A.state_size;
   uint32_t wm[kMomentAhead], wr[kMomentAhead], f[kMomentAhead][4];
 #pragma unroll
@@ -393,129 +380,342 @@ __device__ inline void make_odd(const MomentArgs& A, const MomentRecord& t, cons
   }
 }
 
-template <bool kMove, bool kWide>
-__device__ inline void make_four(const MomentArgs& A, const MomentRecord& t, const uint32_t (&block)[kMomentAhead], int some) {
-  if (t.row_len % 4 == 0) make_odd<kMove, kWide, 1>(A, t, block, some);
-  else if (t.row_len >= 3) make_odd<kMove, kWide, 2>(A, t, block, some);
-  else make_odd<kMove, kWide, 4>(A, t, block, some);
+template <bool kWide>
+__device__ inline void take_odd(const MomentArgs& A, const MomentRecord& t, uint32_t group) {
+  const uint32_t first = __builtin_amdgcn_readfirstlane(group * kOddGroup + (threadIdx.x >> 6) * kMomentAhead);
+  if (first >= t.blocks) return;
+  uint32_t block[kMomentAhead];
+#pragma unroll
+  for (int g = 0; g < kMomentAhead; ++g) block[g] = first + g;
+  const int some = (int)min(t.blocks - first, (uint32_t)kMomentAhead);
+  if (t.row_len % 4 == 0) make_odd<kWide, 1>(A, t, block, some);
+  else if (t.row_len >= 3) make_odd<kWide, 2>(A, t, block, some);
+  else make_odd<kWide, 4>(A, t, block, some);
 }
 
+// Where there are rows of a multiple of sixteen elements, which want registers (of 48: 65 us at five waves a SIMD, 133 at
+// eight), all tensors go together, where there are none at eight waves (rows of 45: 114 us, 133 at five).
 template <bool kWide>
 __global__ __launch_bounds__(256) void moment_take_kernel(MomentArgs A) {
   const uint32_t b = blockIdx.x;
   if (b >= A.groups) return;
   const int k = tensor_of(A, b);
   const MomentRecord& t = A.t[k];
-  const uint32_t group = (b - A.begin[k]) * t.group;
-  if (t.row_len % 16 == 0) {
-    uint32_t block[kEvenAhead];
-    bool make[kEvenAhead];
-#pragma unroll
-    for (int g = 0; g < kEvenAhead; ++g) {
-      block[g] = group + g * 16 + (threadIdx.x >> 4);
-      make[g] = block[g] < t.blocks;
-    }
-    make_even<false, kWide>(A, t, block, make);
+  if (t.row_len % 16) {
+    take_odd<kWide>(A, t, b - A.begin[k]);
     return;
   }
-  const uint32_t first = __builtin_amdgcn_readfirstlane(group + (threadIdx.x >> 6) * kMomentAhead);
-  if (first >= t.blocks) return;
-  uint32_t block[kMomentAhead];
+  uint32_t block[kEvenAhead];
+  bool make[kEvenAhead];
 #pragma unroll
-  for (int g = 0; g < kMomentAhead; ++g) block[g] = first + g;
-  make_four<false, kWide>(A, t, block, (int)min(t.blocks - first, (uint32_t)kMomentAhead));
+  for (int g = 0; g < kEvenAhead; ++g) {
+    block[g] = (b - A.begin[k]) * kEvenGroup + g * 16 + (threadIdx.x >> 4);
+    make[g] = block[g] < t.blocks;
+  }
+  make_even<kWide>(A, t, block, make);
 }
 
 template <bool kWide>
-__global__ __launch_bounds__(256) void moment_move_kernel(MomentArgs A) {
-  __shared__ uint32_t changed[2];
-  __shared__ uint8_t list[kMoveGroup];
+__global__ __launch_bounds__(256, 8) void moment_take_odd_kernel(MomentArgs A) {
   const uint32_t b = blockIdx.x;
   if (b >= A.groups) return;
   const int k = tensor_of(A, b);
-  const MomentRecord& t = A.t[k];
-  const uint32_t group = t.group, first = (b - A.begin[k]) * group, len = t.row_len;
-  if (threadIdx.x < 2) changed[threadIdx.x] = 0;
-  __syncthreads();
-  // the rows with an element in these blocks, four of them under way at once
-  const int64_t base = (int64_t)first * kMomBlock, end = min(base + group * kMomBlock, t.count);
-  uint32_t at0, at1;
-  const int64_t row0 = (int64_t)first_row(t, base, at0), row1 = (int64_t)first_row(t, end - 1, at1);
-  uint32_t lo = 0, hi = 0;
-  for (int64_t r = row0 + threadIdx.x; r <= row1; r += 256 * 4) {
-    int32_t row[4], s[4];
-    bool in[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      row[j] = (int32_t)(r + 256 * j);
-      in[j] = r + 256 * j <= row1;
+  take_odd<kWide>(A, A.t[k], b - A.begin[k]);
+}
+
+// ---- moves --------------------------------------------------------------------------------------------
+
+// What changed rows get is laid out as the tensor: with rows of a multiple of sixteen elements the codes of both arrays and
+// two exponents for each sixteen elements, with others a word an element, m | r << 8 | exponents << 16.
+struct MoveRecord {
+  int64_t count;
+  uint64_t magic;    // row_magic
+  uint8_t* stage;
+  int64_t plane;     // bytes from the one array's codes to the other's, and on to the exponents; 0: a word an element
+  uint32_t at;       // blocks
+  uint32_t row_len;
+  uint32_t blocks;
+  uint32_t pieces;   // of a row: sixteen elements, or four
+  uint32_t piece;    // the first among those of all tensors
+  uint32_t by_pieces;  // floor(2^32 / pieces) + 1, 0 for one
+};
+
+constexpr int kMoveTensors = 60;     // per launch: the argument block stays below 4 KiB
+constexpr int kMovePieces = 512;     // of a row in all tensors, up to which they are dealt out together
+constexpr int kWidePieces = 256;     // of longer rows, per workgroup
+constexpr int kMoveRows = 256;       // per workgroup at most
+
+struct MoveArgs {
+  MoveRecord t[kMoveTensors];
+  uint32_t begin[kMoveTensors];  // first workgroup of each tensor in the second launch
+  uint8_t *m8, *r8, *fields;
+  uint32_t* bits;     // rows that change
+  int64_t state_size;
+  const void* index;
+  uint32_t rows;
+  int32_t n;
+  uint32_t groups;
+  int32_t tile;       // rows per workgroup of the first launch, a multiple of 64
+  uint32_t pieces;    // of a row in all tensors, 0 where they are too many to be dealt out together
+};
+static_assert(sizeof(MoveArgs) <= 4096, "kernel arguments");
+
+// Piece c of what `row` gets from row s (nothing for s < 0).
+__device__ inline void gather_piece(const MoveArgs& A, const MoveRecord& t, int64_t row, int32_t s, uint32_t c) {
+  const uint32_t len = t.row_len;
+  const uint64_t from = (uint64_t)t.at * kMomBlock;
+  if (t.plane) {
+    const uint64_t to = (uint64_t)row * len + c * 16;
+    vec4u wm{}, wr{};
+    uint16_t f = 0;
+    if (s >= 0) {
+      const uint64_t at = from + (uint64_t)s * len + c * 16;
+      wm = *reinterpret_cast<const vec4u*>(A.m8 + at);
+      wr = *reinterpret_cast<const vec4u*>(A.r8 + at);
+      f = *(const uint16_t*)(A.fields + 2 * (at >> 8));
     }
-    sources<true, kWide>(A, row, in, s);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (!in[j] || s[j] == row[j]) continue;
-      const int64_t e = (int64_t)row[j] * len - base;
-      const int from = e > 0 ? (int)(e / kMomBlock) : 0, to = (int)(min(e + len, end - base) - 1) / kMomBlock;
-      const uint64_t bits = ((uint64_t)2 << to) - ((uint64_t)1 << from);
-      lo |= (uint32_t)bits;
-      hi |= (uint32_t)(bits >> 32);
-    }
-  }
-  if (lo | hi) {  // once for each lane's part: lanes beside each other mostly have the same
-    const uint32_t first_lo = __builtin_amdgcn_readfirstlane(lo), first_hi = __builtin_amdgcn_readfirstlane(hi);
-    const bool other = lo != first_lo || hi != first_hi;
-    if (other || (threadIdx.x & 63) == __builtin_ctzll(__ballot(!other))) {
-      if (lo) atomicOr(&changed[0], lo);
-      if (hi) atomicOr(&changed[1], hi);
-    }
-  }
-  __syncthreads();
-  const uint64_t bits = (uint64_t)changed[1] << 32 | changed[0];
-  if (threadIdx.x == 0) A.changed[b] = bits;
-  if (bits == 0) return;
-  if (threadIdx.x < kMoveGroup && (bits >> threadIdx.x & 1u))
-    list[__popcll(bits & (((uint64_t)1 << threadIdx.x) - 1u))] = (uint8_t)threadIdx.x;
-  __syncthreads();
-  const int n = __popcll(bits);
-  if (len % 16 == 0) {
-    for (int i = threadIdx.x >> 4; (i & ~3) < n; i += 16 * kEvenAhead) {
-      uint32_t block[kEvenAhead];
-      bool make[kEvenAhead];
-#pragma unroll
-      for (int g = 0; g < kEvenAhead; ++g) {
-        make[g] = i + 16 * g < n;
-        block[g] = first + list[min(i + 16 * g, n - 1)];
-      }
-      make_even<true, kWide>(A, t, block, make);
-    }
+    *reinterpret_cast<vec4u*>(t.stage + to) = wm;
+    *reinterpret_cast<vec4u*>(t.stage + t.plane + to) = wr;
+    *(uint16_t*)(t.stage + 2 * t.plane + (to >> 4) * 2) = f;
     return;
   }
-  for (int i = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * kMomentAhead; i < n; i += 4 * kMomentAhead) {
-    uint32_t block[kMomentAhead];
+  typedef uint32_t any16 __attribute__((ext_vector_type(4), aligned(4)));
+  const uint32_t here = min(len - c * 4, 4u);
+  uint32_t* to = reinterpret_cast<uint32_t*>(t.stage) + (uint64_t)row * len + c * 4;
+  uint32_t w[4] = {0, 0, 0, 0};
+  if (s >= 0) {
+    const uint64_t at = from + (uint64_t)s * len + c * 4, size = (uint64_t)A.state_size;
+    const uint32_t wm = four_at(A.m8, at, size), wr = four_at(A.r8, at, size);
+    // the elements lie in one block or in two
+    const uint32_t f0 = *(const uint16_t*)(A.fields + 2 * (at >> 8)), f1 = *(const uint16_t*)(A.fields + 2 * ((at + here - 1) >> 8));
 #pragma unroll
-    for (int g = 0; g < kMomentAhead; ++g) block[g] = first + __builtin_amdgcn_readfirstlane(list[min(i + g, n - 1)]);
-    make_four<true, kWide>(A, t, block, min(n - i, kMomentAhead));
+    for (int j = 0; j < 4; ++j)
+      w[j] = ((wm >> (8 * j)) & 255u) | ((wr >> (8 * j)) & 255u) << 8 | (((at + j) >> 8) == (at >> 8) ? f0 : f1) << 16;
+  }
+  if (here == 4) {
+    *reinterpret_cast<any16*>(to) = any16{w[0], w[1], w[2], w[3]};
+  } else {
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+      if ((uint32_t)j < here) to[j] = w[j];
   }
 }
 
-// The changed blocks from the copy into their places, 16 bytes a lane and array.
-__global__ __launch_bounds__(256) void moment_back_kernel(MomentArgs A) {
-  typedef uint32_t vec __attribute__((ext_vector_type(4)));
+// The first launch: a workgroup looks at up to 256 rows, marks those that change and gathers what they get.
+template <bool kWide>
+__global__ __launch_bounds__(256) void moment_gather_kernel(MoveArgs A) {
+  __shared__ int32_t to[kMoveRows], of[kMoveRows];
+  __shared__ int32_t moved;
+  __shared__ uint8_t tensor[kMovePieces];
+  __shared__ MoveRecord rec[kMoveTensors];
+  if (threadIdx.x == 0) moved = 0;
+  __syncthreads();
+  const int lane = threadIdx.x & 63;
+  const int64_t base = (int64_t)blockIdx.x * A.tile, i = base + threadIdx.x;
+  const bool in = (int)threadIdx.x < A.tile && i < (int64_t)A.rows;
+  bool change = false;
+  int32_t s = -1;
+  if (in) {
+    s = entry<kWide>(A, i);
+    // a row stays whose source does not, or is none
+    change = s == -1 || (s >= 0 && s != i && entry<kWide>(A, s) == s);
+  }
+  const uint64_t move = __ballot(change);
+  if (lane == 0 && in && blockIdx.y == 0 && blockIdx.z == 0) {
+    A.bits[i >> 5] = (uint32_t)move;
+    A.bits[(i >> 5) + 1] = (uint32_t)(move >> 32);
+  }
+  int32_t at = 0;
+  if (lane == 0 && move) at = atomicAdd(&moved, __popcll(move));
+  at = __builtin_amdgcn_readfirstlane(at);
+  if (change) {
+    const int below = __builtin_amdgcn_mbcnt_hi((uint32_t)(move >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)move, 0));
+    to[at + below] = threadIdx.x;
+    of[at + below] = s;
+  }
+  __syncthreads();
+  const uint32_t m = moved;
+  if (m == 0) return;
+  if (A.pieces == 0) {  // long rows: kWidePieces of one tensor's
+    const MoveRecord& t = A.t[blockIdx.y];
+    const uint32_t first = blockIdx.z * kWidePieces;
+    if (first >= t.pieces) return;
+    const uint32_t pieces = min(t.pieces - first, (uint32_t)kWidePieces), by = pieces > 1 ? 0xffffffffu / pieces + 1 : 0;
+    for (uint32_t e = threadIdx.x; e < m * pieces; e += 256) {
+      const uint32_t q = by ? __umulhi(e, by) : e;
+      gather_piece(A, t, base + to[q], of[q], first + e - q * pieces);
+    }
+    return;
+  }
+  // the records and every piece's tensor at hand
+  for (int j = threadIdx.x; j < A.n * (int)(sizeof(MoveRecord) / 8); j += 256)
+    reinterpret_cast<uint64_t*>(rec)[j] = reinterpret_cast<const uint64_t*>(A.t)[j];
+  for (int k = threadIdx.x >> 6; k < A.n; k += 4)
+    for (uint32_t c = lane; c < A.t[k].pieces; c += 64) tensor[A.t[k].piece + c] = (uint8_t)k;
+  __syncthreads();
+  const uint32_t by_m = m > 1 ? 0xffffffffu / m + 1 : 0;
+  for (uint32_t e = threadIdx.x; e < m * A.pieces; e += 256) {
+    // tensor after tensor, row after row
+    const MoveRecord& t = rec[tensor[by_m ? __umulhi(e, by_m) : e]];
+    const uint32_t r = e - m * t.piece, q = t.by_pieces ? __umulhi(r, t.by_pieces) : r;
+    gather_piece(A, t, base + to[q], of[q], r - q * t.pieces);
+  }
+}
+
+__device__ inline bool changes(const MoveArgs& A, uint32_t row) { return A.bits[row >> 5] >> (row & 31u) & 1u; }
+
+// Whether a row with elements in a block changes, from every kStep-th of their words, this lane's from `from` on.
+template <int kStep>
+__device__ inline bool block_changes(const MoveArgs& A, const MoveRecord& t, uint32_t block, uint32_t from) {
+  const int64_t base = (int64_t)block * kMomBlock;
+  if (base >= t.count) return false;
+  uint32_t at0, at1;
+  const uint32_t row0 = (uint32_t)first_row(t, base, at0);
+  const uint32_t row1 = (uint32_t)first_row(t, min(base + kMomBlock, t.count) - 1, at1);
+  uint32_t any = 0;
+  for (uint32_t w = (row0 >> 5) + from; w <= row1 >> 5; w += kStep) {
+    uint32_t x = A.bits[w];
+    if (w == row0 >> 5) x &= ~0u << (row0 & 31u);
+    if (w == row1 >> 5) x &= ~0u >> (31u - (row1 & 31u));
+    any |= x;
+  }
+  return any != 0;
+}
+
+// The second launch: blocks with a changed row, in place; 64 a workgroup are looked over.
+__device__ inline void remake_even(const MoveArgs& A, const MoveRecord& t, uint32_t first, uint8_t* list) {
+  const int lane = threadIdx.x & 15, block = threadIdx.x & 63;
+  const uint64_t bits = __ballot(block_changes<1>(A, t, first + block, 0));  // the same in every wave
+  if (bits == 0) return;
+  if (threadIdx.x < kRemakeGroup && (bits >> block & 1u))
+    list[__popcll(bits & (((uint64_t)1 << block) - 1u))] = (uint8_t)block;
+  __syncthreads();
+  const int n = __popcll(bits);
+  for (int i = threadIdx.x >> 4; (i & ~3) < n; i += 16 * kEvenAhead) {
+    vec4u wm[kEvenAhead], wr[kEvenAhead];
+    uint32_t f[kEvenAhead];
+    uint64_t at[kEvenAhead];
+#pragma unroll
+    for (int g = 0; g < kEvenAhead; ++g) {
+      wm[g] = wr[g] = vec4u{};
+      f[g] = 0;
+      if (i + 16 * g >= n) continue;
+      const int64_t base = (int64_t)(first + list[i + 16 * g]) * kMomBlock;
+      uint32_t at0;
+      const uint32_t row = (uint32_t)first_row(t, base, at0) + row_of(t, at0 + lane * 16);
+      at[g] = (uint64_t)t.at * kMomBlock + base + lane * 16;
+      const uint8_t *m = A.m8 + at[g], *r = A.r8 + at[g], *e = A.fields + 2 * (at[g] >> 8);
+      if (base + lane * 16 < t.count && changes(A, row)) {
+        m = t.stage + base + lane * 16;
+        r = m + t.plane;
+        e = t.stage + 2 * t.plane + ((base >> 4) + lane) * 2;
+      }
+      wm[g] = *reinterpret_cast<const vec4u*>(m);
+      wr[g] = *reinterpret_cast<const vec4u*>(r);
+      f[g] = *(const uint16_t*)e;
+    }
+#pragma unroll
+    for (int g = 0; g < kEvenAhead; ++g) {
+      uint32_t fields;
+      recode(wm[g], wr[g], f[g], fields);
+      if (i + 16 * g >= n) continue;
+      *reinterpret_cast<vec4u*>(A.m8 + at[g]) = wm[g];
+      *reinterpret_cast<vec4u*>(A.r8 + at[g]) = wr[g];
+      if (lane == 0) *(uint16_t*)(A.fields + 2 * (at[g] >> 8)) = (uint16_t)fields;
+    }
+  }
+}
+
+// Four blocks a wave are looked over, sixteen lanes each; those that change are made kOddAhead at a time.
+__device__ inline void remake_odd(const MoveArgs& A, const MoveRecord& t, uint32_t first) {
+  const uint32_t lane = threadIdx.x & 63, l = lane * 4;
+  const uint32_t* stage = reinterpret_cast<const uint32_t*>(t.stage);
+  constexpr int kLanes = 16;  // a block
+  uint64_t left = __ballot(block_changes<kLanes>(A, t, first + lane / kLanes, lane % kLanes));
+#pragma unroll
+  for (int o = 1; o < kLanes; o <<= 1) left |= left >> o;
+  left &= 0x0001000100010001u;
+  while (left) {
+    int some = 0;
+    uint32_t block[kOddAhead];
+#pragma unroll
+    for (int g = 0; g < kOddAhead; ++g) {
+      block[g] = first;
+      if (left == 0) continue;
+      block[g] = first + __builtin_ctzll(left) / kLanes;
+      left &= left - 1;
+      some = g + 1;
+    }
+    uint32_t wm[kOddAhead], wr[kOddAhead], f[kOddAhead], change[kOddAhead];
+    vec4u got[kOddAhead];
+#pragma unroll
+    for (int g = 0; g < kOddAhead; ++g) {
+      change[g] = 0;
+      if (g >= some) continue;
+      const int64_t base = (int64_t)block[g] * kMomBlock;
+      const uint64_t at = (uint64_t)t.at * kMomBlock + base + l;
+      wm[g] = *reinterpret_cast<const uint32_t*>(A.m8 + at);
+      wr[g] = *reinterpret_cast<const uint32_t*>(A.r8 + at);
+      f[g] = *(const uint16_t*)(A.fields + 2 * (at >> 8));
+      // the rows of four elements are four at most: their bits lie in two words
+      uint32_t at0;
+      const uint32_t row0 = (uint32_t)first_row(t, base, at0), q = row_of(t, at0 + l), off = at0 + l - q * t.row_len;
+      uint32_t row[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        row[j] = row0 + q + (t.row_len >= 3 ? (off + j >= t.row_len ? 1u : 0u) : (off + j) >> (t.row_len - 1));
+      const int64_t here = t.count - base - l;  // elements from the lane's first on
+      if (here <= 0) continue;
+      const uint32_t last = here >= 4 ? row[3] : here == 3 ? row[2] : here == 2 ? row[1] : row[0];
+      const uint32_t w0 = A.bits[row[0] >> 5], w1 = A.bits[last >> 5];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < here && (row[j] >> 5 == row[0] >> 5 ? w0 : w1) >> (row[j] & 31u) & 1u) change[g] |= 1u << j;
+      if (change[g]) got[g] = *reinterpret_cast<const vec4u*>(stage + base + l);
+    }
+#pragma unroll
+    for (int g = 0; g < kOddAhead; ++g) {
+      if (g >= some) continue;
+      const uint64_t at = ((uint64_t)t.at + block[g]) * kMomBlock + l;
+      int fm[4], fr[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t e = f[g];
+        if (change[g] >> j & 1u) {
+          const uint32_t w = got[g][j], keep = ~(255u << (8 * j));
+          wm[g] = (wm[g] & keep) | (w & 255u) << (8 * j);
+          wr[g] = (wr[g] & keep) | (w >> 8 & 255u) << (8 * j);
+          e = w >> 16;
+        }
+        fm[j] = (int)(e & 255u);
+        fr[j] = (int)(e >> 8);
+      }
+      float m[4], r[4];
+      decode_m4(wm[g], fm, m);
+      decode_r4(wr[g], fr, r);
+      const uint32_t none[4] = {0, 0, 0, 0};
+      uint32_t cm, cr, fields;
+      encode_block<false>(m, r, none, cm, cr, fields);
+      *reinterpret_cast<uint32_t*>(A.m8 + at) = cm;
+      *reinterpret_cast<uint32_t*>(A.r8 + at) = cr;
+      if (l == 0) *(uint16_t*)(A.fields + 2 * (at >> 8)) = (uint16_t)fields;
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void moment_remake_even_kernel(MoveArgs A) {
+  __shared__ uint8_t list[kRemakeGroup];
   const uint32_t b = blockIdx.x;
   if (b >= A.groups) return;
-  const uint64_t bits = A.changed[b];
-  if (bits == 0) return;
-  const int k = tensor_of(A, b), lane = threadIdx.x & 15;
-  const uint64_t first = (uint64_t)A.t[k].dst_at + (b - A.begin[k]) * A.t[k].group;
-#pragma unroll
-  for (int g = 0; g < kMoveGroup / 16; ++g) {
-    const uint32_t block = g * 16 + (threadIdx.x >> 4);
-    if (!(bits >> block & 1u)) continue;
-    const uint64_t i = first + block, at = i * kMomBlock + lane * 16;
-    *reinterpret_cast<vec*>(const_cast<uint8_t*>(A.m8) + at) = *reinterpret_cast<const vec*>(A.to_m8 + at);
-    *reinterpret_cast<vec*>(const_cast<uint8_t*>(A.r8) + at) = *reinterpret_cast<const vec*>(A.to_r8 + at);
-    if (lane == 0) *(uint16_t*)(const_cast<uint8_t*>(A.fields) + 2 * i) = *(const uint16_t*)(A.to_fields + 2 * i);
-  }
+  const int k = tensor_of(A, b);
+  remake_even(A, A.t[k], (b - A.begin[k]) * kRemakeGroup, list);
+}
+
+__global__ __launch_bounds__(256, 8) void moment_remake_odd_kernel(MoveArgs A) {
+  const uint32_t b = blockIdx.x;
+  if (b >= A.groups) return;
+  const int k = tensor_of(A, b);
+  remake_odd(A, A.t[k], __builtin_amdgcn_readfirstlane((b - A.begin[k]) * kOddGroup + (threadIdx.x >> 6) * 4));
 }
 
 bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
@@ -535,48 +735,14 @@ int check_side(const char* what, int num, const int64_t* row_lens, int64_t rows,
   return GS_OK;
 }
 
-enum { kTake, kMove, kBack };
+int64_t padded(int64_t bytes) { return (bytes + 255) & ~(int64_t)255; }
 
-int launch(int what, hipStream_t stream, int num, const int64_t* row_lens, const int64_t* offsets, const int64_t* out_offsets,
-           int64_t count, MomentArgs& A) {
-  uint64_t* const changed = A.changed;
-  int64_t done = 0;  // workgroups of the launches before
-  for (int i = 0; i < num;) {
-    int k = 0;
-    int64_t groups = 0;
-    for (; i < num && k < kMomentTensors; ++i) {
-      const int64_t elements = row_lens[i] * count, blocks = (elements + kMomBlock - 1) / kMomBlock;
-      if (blocks == 0) continue;
-      const int64_t per = what != kTake ? (row_lens[i] < 16 ? 16 : kMoveGroup) : row_lens[i] % 16 ? kTakeGroup : 16 * kEvenAhead, more = (blocks + per - 1) / per;
-      GS_REQUIRE(more <= kMaxGroups, "gs_moments: tensor %d is too large", i);
-      if (groups + more > kMaxGroups) break;
-      MomentRecord& t = A.t[k];
-      t.count = elements;
-      t.row_len = (uint32_t)row_lens[i];
-      t.magic = row_magic(row_lens[i]);
-      t.src_at = (uint32_t)(offsets[i] / kMomBlock);
-      t.dst_at = (uint32_t)(out_offsets[i] / kMomBlock);
-      t.blocks = (uint32_t)blocks;
-      t.group = (uint32_t)per;
-      A.begin[k++] = (uint32_t)groups;
-      groups += more;
-    }
-    if (k == 0) continue;
-    A.n = k;
-    A.groups = (uint32_t)groups;
-    A.changed = changed + done;
-    done += groups;
-    auto* kernel = what == kBack   ? moment_back_kernel
-                   : what == kMove ? (A.wide ? moment_move_kernel<true> : moment_move_kernel<false>)
-                                   : (A.wide ? moment_take_kernel<true> : moment_take_kernel<false>);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), 0, stream, A);
-    GS_LAUNCH_CHECK("moment_rows_kernel");
-  }
-  A.changed = changed;
-  return GS_OK;
+// A move's workspace: the bits of the rows, and of each tensor what changed rows get.
+int64_t bits_bytes(int64_t rows) { return padded((rows + 63) / 64 * 8); }
+int64_t stage_bytes(int64_t row_len, int64_t rows) {
+  const int64_t elements = row_len * rows;
+  return row_len % 16 ? padded(elements * 4) : 2 * padded(elements) + padded(elements / 8);
 }
-
-size_t padded(int64_t bytes) { return ((size_t)bytes + 255) & ~(size_t)255; }
 
 }  // namespace
 }  // namespace gs
@@ -615,15 +781,45 @@ extern "C" int gs_moments_take(void* stream, int num, const int64_t* row_lens, i
   A.to_fields = out_fields;
   A.index = index;
   A.rows = (uint32_t)rows;
-  A.wide = index_bits == 64;
-  return launch(kTake, (hipStream_t)stream, num, row_lens, offsets, out_offsets, count, A);
+  bool even = false;
+  for (int i = 0; i < num; ++i) even |= row_lens[i] > 0 && row_lens[i] % 16 == 0;
+  auto* kernel = even ? (index_bits == 64 ? moment_take_kernel<true> : moment_take_kernel<false>)
+                      : (index_bits == 64 ? moment_take_odd_kernel<true> : moment_take_odd_kernel<false>);
+  for (int i = 0; i < num;) {
+    int64_t groups = 0;
+    A.n = 0;
+    for (; i < num && A.n < kMomentTensors; ++i) {
+      const int64_t elements = row_lens[i] * count, blocks = (elements + kMomBlock - 1) / kMomBlock;
+      if (blocks == 0) continue;
+      const int64_t per = row_lens[i] % 16 ? kOddGroup : kEvenGroup, more = (blocks + per - 1) / per;
+      GS_REQUIRE(more <= kMaxGroups, "%s: tensor %d is too large", what, i);
+      if (groups + more > kMaxGroups) break;
+      MomentRecord& t = A.t[A.n];
+      t.count = elements;
+      t.row_len = (uint32_t)row_lens[i];
+      t.magic = row_magic(row_lens[i]);
+      t.src_at = (uint32_t)(offsets[i] / kMomBlock);
+      t.dst_at = (uint32_t)(out_offsets[i] / kMomBlock);
+      t.blocks = (uint32_t)blocks;
+      A.begin[A.n++] = (uint32_t)groups;
+      groups += more;
+    }
+    if (A.n == 0) continue;
+    A.groups = (uint32_t)groups;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, A);
+    GS_LAUNCH_CHECK("moment_take_kernel");
+  }
+  return GS_OK;
 }
 
-extern "C" size_t gs_moments_move_workspace_size(int64_t state_size) {
-  if (state_size < 0 || state_size % kMomBlock) return 0;
-  const int64_t blocks = state_size / kMomBlock;
-  // codes, exponents, and which blocks changed: eight bytes for each workgroup, at most one a block
-  return (size_t)state_size * 2 + padded(blocks * 2) + padded(blocks * 8);
+extern "C" size_t gs_moments_move_workspace_size(int num, const int64_t* row_lens, int64_t rows) {
+  if (num < 0 || (num > 0 && !row_lens) || rows < 0 || rows >= ((int64_t)1 << 31)) return 0;
+  int64_t bytes = bits_bytes(rows);
+  for (int i = 0; i < num; ++i) {
+    if (row_lens[i] < 0 || row_lens[i] >= kMaxRowLen) return 0;
+    bytes += stage_bytes(row_lens[i], rows);
+  }
+  return (size_t)bytes;
 }
 
 extern "C" int gs_moments_move(void* stream, int num, const int64_t* row_lens, int64_t rows, const int64_t* offsets,
@@ -640,25 +836,74 @@ extern "C" int gs_moments_move(void* stream, int num, const int64_t* row_lens, i
   GS_REQUIRE(state_size == 0 || (mu8 && nu8 && fields && workspace), "%s: NULL state", what);
   GS_REQUIRE(aligned(mu8, 16) && aligned(nu8, 16) && aligned(fields, 2) && aligned(workspace, 16),
              "%s: the state's arrays and the workspace must be 16-byte aligned", what);
-  const size_t need = gs_moments_move_workspace_size(state_size);
-  GS_REQUIRE(workspace_bytes >= need, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
   const int rc = check_side(what, num, row_lens, rows, offsets, state_size);
   if (rc != GS_OK) return rc;
-  const int64_t blocks = state_size / kMomBlock;
-  uint8_t* ws = (uint8_t*)workspace;
-  MomentArgs A{};
+  const size_t need = gs_moments_move_workspace_size(num, row_lens, rows);
+  GS_REQUIRE(workspace_bytes >= need, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
+  if (rows == 0 || state_size == 0) return GS_OK;
+  uint8_t* const ws = (uint8_t*)workspace;
+  MoveArgs A{};
   A.m8 = mu8;
   A.r8 = nu8;
   A.fields = fields;
-  A.to_m8 = ws;
-  A.to_r8 = ws + state_size;
-  A.to_fields = ws + 2 * state_size;
-  A.changed = (uint64_t*)(ws + 2 * state_size + padded(blocks * 2));
+  A.bits = (uint32_t*)ws;
   A.state_size = state_size;
   A.index = index;
   A.rows = (uint32_t)rows;
-  A.wide = index_bits == 64;
-  const int done = launch(kMove, (hipStream_t)stream, num, row_lens, offsets, offsets, rows, A);
-  if (done != GS_OK) return done;
-  return launch(kBack, (hipStream_t)stream, num, row_lens, offsets, offsets, rows, A);
+  // everything is gathered before anything is made anew
+  enum { kGather, kEven, kOdd };
+  for (const int pass : {kGather, kEven, kOdd}) {
+    uint8_t* stage = ws + bits_bytes(rows);
+    const int64_t per = pass == kEven ? kRemakeGroup : kOddGroup;
+    for (int i = 0; i < num;) {
+      int64_t groups = 0, pieces = 0, most = 0;
+      A.n = 0;
+      for (; i < num && A.n < kMoveTensors; ++i) {
+        const int64_t elements = row_lens[i] * rows, blocks = (elements + kMomBlock - 1) / kMomBlock;
+        const int64_t more = (blocks + per - 1) / per;
+        const bool even = row_lens[i] % 16 == 0;
+        if (pass == kGather || even == (pass == kEven)) {
+          GS_REQUIRE(more <= kMaxGroups, "%s: tensor %d is too large", what, i);
+          if (pass != kGather && groups + more > kMaxGroups) break;
+          if (blocks) {
+            MoveRecord& t = A.t[A.n];
+            t.count = elements;
+            t.magic = row_magic(row_lens[i]);
+            t.stage = stage;
+            t.plane = even ? padded(elements) : 0;
+            t.at = (uint32_t)(offsets[i] / kMomBlock);
+            t.row_len = (uint32_t)row_lens[i];
+            t.blocks = (uint32_t)blocks;
+            t.pieces = (uint32_t)(even ? row_lens[i] / 16 : (row_lens[i] + 3) / 4);
+            t.piece = (uint32_t)pieces;
+            t.by_pieces = t.pieces > 1 ? (uint32_t)((((uint64_t)1 << 32) / t.pieces) + 1) : 0;
+            pieces += t.pieces;
+            most = std::max<int64_t>(most, t.pieces);
+            A.begin[A.n++] = (uint32_t)groups;
+            groups += more;
+          }
+        }
+        stage += stage_bytes(row_lens[i], rows);
+      }
+      if (A.n == 0) continue;
+      A.groups = (uint32_t)groups;
+      dim3 grid((unsigned)groups);
+      if (pass == kGather) {
+        A.pieces = pieces <= kMovePieces ? (uint32_t)pieces : 0;
+        // few rows a workgroup where there are few workgroups, as the rows that change may lie together (2M Gaussians, 8 % of
+        // them at random: 188 us by 64, 167 by 128, 158 by 256)
+        A.tile = !A.pieces || rows <= ((int64_t)1 << 18) ? 64 : rows <= ((int64_t)1 << 19) ? 128 : kMoveRows;
+        while (div_up(rows, A.tile) > kMaxGroups) A.tile *= 2;
+        grid = dim3((unsigned)div_up(rows, A.tile), A.pieces ? 1u : (unsigned)A.n,
+                    A.pieces ? 1u : (unsigned)div_up(most, kWidePieces));
+        GS_REQUIRE(grid.z < 65536, "%s: rows are too long", what);
+      }
+      auto* kernel = pass == kEven  ? moment_remake_even_kernel
+                     : pass == kOdd ? moment_remake_odd_kernel
+                     : index_bits == 64 ? moment_gather_kernel<true> : moment_gather_kernel<false>;
+      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, A);
+      GS_LAUNCH_CHECK("moment_move_kernel");
+    }
+  }
+  return GS_OK;
 }

@@ -120,7 +120,7 @@ _SIGS = {
     "gs_take_rows": [_P, _I, _P, _P, _P, _I64, _P, _P, _P, _P, _I, _I64],
     "gs_move_rows": [_P, _I, _P, _P, _P, _I64, _P, _P, _I, _P],
     "gs_moments_take": [_P, _I, _P, _I64, _P, _I64, _P, _P, _P, _P, _I, _I64, _P, _I64, _P, _P, _P],
-    "gs_moments_move_workspace_size": [_I64],
+    "gs_moments_move_workspace_size": [_I, _P, _I64],
     "gs_moments_move": [_P, _I, _P, _I64, _P, _I64, _P, _P, _P, _P, _I, _P, _SZ],
     "gs_best_rows_workspace_size": [_I64],
     "gs_best_rows": [_P, _I64, _P, _I, _P, _I64, _P, _SZ, _P],

@@ -354,7 +354,7 @@ class AdamWState:
                 _lib.call("gs_move_rows", stream, each * k, self._addresses(flats), row_bytes * each, row_bytes * each,
                           rows, None, index.data_ptr(), bits, None)
             if self.bits == 8:
-                nbytes = _lib.lib().gs_moments_move_workspace_size(self.size)
+                nbytes = _lib.lib().gs_moments_move_workspace_size(k, lens_bytes, rows)
                 ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
                 _lib.call("gs_moments_move", stream, k, lens_bytes, rows, self._offsets, self.size,
                           self.mu_flat.data_ptr(), self.nu_flat.data_ptr(), self.fields.data_ptr(), index.data_ptr(), bits,

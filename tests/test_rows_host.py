@@ -80,7 +80,10 @@ def test_moments_take_entry_refuses():
 
 def test_moments_move_entry_refuses():
     size = _lib.lib().gs_moments_move_workspace_size
-    assert size(0) == 0 and size(-256) == 0 and size(100) == 0 and size(1024) >= 2 * 1024 + 4 * 3
+    assert size(0, None, 0) == 0 and size(-1, None, 5) == 0 and size(1, None, 5) == 0 and size(1, i64(3), -1) == 0
+    assert size(1, i64(1 << 24), 5) == 0 and size(1, i64(-1), 5) == 0 and size(1, i64(3), 1 << 31) == 0
+    # a bit a row, 4 B an element, or with rows of a multiple of sixteen 2 B and 2 for each sixteen
+    assert size(2, i64(3, 48), 1000) >= 125 + 12 * 1000 + (2 * 48 + 6) * 1000
 
     def move(num=1, lens=i64(3), rows=100, at=i64(0), state=512, m=P, index=P, bits=32, ws=P, nbytes=1 << 20):
         return refused("gs_moments_move", None, num, lens, rows, at, state, m, P, P, index, bits, ws, nbytes)
@@ -92,7 +95,7 @@ def test_moments_move_entry_refuses():
     assert "state of" in move(state=511)
     assert "NULL state" in move(m=None) and "NULL state" in move(ws=None)
     assert "16-byte aligned" in move(ws=P + 8)
-    assert "workspace of" in move(nbytes=size(512) - 1)
+    assert "workspace of" in move(nbytes=size(1, i64(3), 100) - 1)
     assert "outside the state" in move(rows=200)
 
 
