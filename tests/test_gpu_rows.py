@@ -349,6 +349,39 @@ def test_moments_of_all_sizes_side_by_side(cuda, row, kind):
     check(state.move_rows_(index.to(cuda)), index)
 
 
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("n, shapes", [
+    (40, [(8208,), (20000,), (3,), (8192,)]),           # long rows, dealt out piece by piece
+    (130, [(1 + i % 19,) for i in range(150)]),         # more tensors than a launch holds
+    (600_001, [(1,), (2,), (3,), (16,)]),               # more than 512 rows a CU
+    (262_145, [(5,), (32,), (0,)])])
+def test_moments_of_long_rows_many_tensors_and_many_rows(cuda, n, shapes, dtype):
+    """Taken and moved against the way by 32 bits."""
+    gen = torch.Generator(device=cuda).manual_seed(n)
+    mu, nu = [], []
+    for s in shapes:
+        size = torch.exp(torch.randn(n, 1, generator=gen, device=cuda) * 2.0 - 9.0)
+        mu.append(torch.randn(n, *s, generator=gen, device=cuda) * size)
+        nu.append((torch.rand(n, *s, generator=gen, device=cuda) * size) ** 2)
+    opt = AdamW(1e-3, moment_bits=8)
+    state = opt.restore([torch.zeros_like(x) for x in mu], mu, nu, 1)
+    was = state.moments()
+
+    def check(got, index):
+        index = index.to(cuda).long()
+        there = ((index >= 0) & (index < n))[:, None]
+        rows = [[torch.where(there, x[index.clamp(0, n - 1)], 0.0) for x in xs] for xs in was]
+        want = opt.restore([torch.zeros_like(x) for x in rows[0]], *rows, 1)
+        # (the values: blocks that a move leaves alone may hold them under a larger exponent than a new encoding)
+        for xs, ys in zip(got.moments(), want.moments()):
+            assert all([torch.equal(a, b) for a, b in zip(xs, ys)])
+
+    index = an_index(n, n + 77, 3, dtype)
+    check(state.take_rows(index.to(cuda)), index)
+    index = a_move(n, 5, dtype, moved=0.2, freed=0.05)
+    check(state.move_rows_(index.to(cuda)), index)
+
+
 def test_masters_follow(cuda):
     for moment_bits in (32, 8):
         p = [torch.randn(200, 3, device=cuda).bfloat16(), torch.randn(200, device=cuda).half()]
