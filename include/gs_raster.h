@@ -591,8 +591,9 @@ int gs_moments_decode(void* stream, int64_t state_size, const uint8_t* mu8, cons
  * outside [0, rows) the row fills[k] (device pointers, fills and any of them may be NULL: zeros).
  * Rows are bytes: row_bytes[k] of them one after another, strides[k] from row to row of tensors[k];
  * out[k] is 16-byte aligned, its count rows lie one behind the other, and out_bytes[k] >= count *
- * row_bytes[k] (NULL: equal) are written, zeros behind the rows.  index: device, count entries of
- * index_bits 32 or 64.  Outputs overlap nothing else. */
+ * row_bytes[k] (NULL: equal) are written, zeros behind the rows: at most 2^24 - 1 times 8192 bytes, or
+ * 512 rows where they are shorter than 16 bytes.  index: device, count entries of index_bits 32 or 64.
+ * Outputs overlap nothing else. */
 int gs_take_rows(void* stream, int num, const void* const* tensors, const int64_t* row_bytes,
                  const int64_t* strides, int64_t rows, void* const* out, const int64_t* out_bytes,
                  const void* const* fills, const void* index, int index_bits, int64_t count);

@@ -337,6 +337,9 @@ __global__ __launch_bounds__(256) void move_rows_kernel(MoveArgs M, int32_t* lef
   }
 }
 
+// Bytes of an output that a workgroup writes.
+int64_t take_bytes(int64_t row) { return row < 16 ? kTakeRows * row : kTakeBytes; }
+
 uint32_t reciprocal(uint32_t d) { return d > 1 ? (uint32_t)((((uint64_t)1 << 32) / d) + 1) : 0; }
 
 }  // namespace
@@ -357,8 +360,8 @@ extern "C" int gs_take_rows(void* stream, int num, const void* const* tensors, c
   for (int i = 0; i < num; ++i) {
     GS_REQUIRE(row_bytes[i] >= 0 && row_bytes[i] < kMaxRowBytes, "gs_take_rows: rows of %lld bytes", (long long)row_bytes[i]);
     const int64_t need = row_bytes[i] * count, all = out_bytes ? out_bytes[i] : need;
-    GS_REQUIRE(all >= need && all <= kMaxGroups * kTakeBytes && (all == 0 || row_bytes[i] > 0), "gs_take_rows: output %d of %lld bytes for %lld", i,
-               (long long)all, (long long)need);
+    GS_REQUIRE(all >= need && all <= kMaxGroups * take_bytes(row_bytes[i]) && (all == 0 || row_bytes[i] > 0),
+               "gs_take_rows: output %d of %lld bytes for %lld", i, (long long)all, (long long)need);
     GS_REQUIRE(all == 0 || out[i], "gs_take_rows: NULL output %d", i);
     GS_REQUIRE(need == 0 || rows == 0 || tensors[i], "gs_take_rows: NULL tensor %d", i);
     GS_REQUIRE((reinterpret_cast<uintptr_t>(out[i]) & 15) == 0, "gs_take_rows: output %d must be 16-byte aligned", i);
@@ -377,7 +380,7 @@ extern "C" int gs_take_rows(void* stream, int num, const void* const* tensors, c
     for (; i < num && k < kRowTensors; ++i) {
       const int64_t all = out_bytes ? out_bytes[i] : row_bytes[i] * count;
       if (all == 0) continue;
-      const int64_t per = row_bytes[i] < 16 ? kTakeRows * row_bytes[i] : kTakeBytes, more = (all + per - 1) / per;
+      const int64_t per = take_bytes(row_bytes[i]), more = (all + per - 1) / per;
       if (groups + more > kMaxGroups) break;
       RowRecord& t = A.t[k];
       t.src = (const char*)tensors[i];
