@@ -342,25 +342,36 @@ class AdamWState:
         is negative, as ``rows.move_rows_`` moves the parameters.  Returns the state."""
         dev = self.mu_flat.device
         index = row_index(index, dev, "AdamWState.move_rows_")
-        rows, lens, lens_bytes, row_bytes, _ = self._rows("move_rows_")
+        rows = self._rows("move_rows_")[0]
         if index.numel() != rows:
             raise ValueError(f"AdamWState.move_rows_: {index.numel()} indices for {rows} rows")
-        k = len(lens)
         with _lib.on(dev):
-            stream, bits = _lib.stream_handle(dev), 8 * index.element_size()
-            flats = self._flats()
-            if flats:
-                each = len(flats)
-                _lib.call("gs_move_rows", stream, each * k, self._addresses(flats), row_bytes * each, row_bytes * each,
-                          rows, None, index.data_ptr(), bits, None)
-            if self.bits == 8:
-                nbytes = _lib.lib().gs_moments_move_workspace_size(k, lens_bytes, rows)
-                ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-                _lib.call("gs_moments_move", stream, k, lens_bytes, rows, self._offsets, self.size,
-                          self.mu_flat.data_ptr(), self.nu_flat.data_ptr(), self.fields.data_ptr(), index.data_ptr(), bits,
-                          ws.data_ptr(), nbytes)
-        _lib.tensors().written([], [], [self.mu_flat, self.nu_flat, self.fields, self.master_flat])
+            self._move(index, self._move_workspace())
         return self
+
+    def _move_workspace(self) -> Optional[torch.Tensor]:
+        """What ``_move`` needs beside the state, so that it is there before anything is written."""
+        if self.bits != 8:
+            return None
+        rows, lens, lens_bytes, _, _ = self._rows("move_rows_")
+        nbytes = _lib.lib().gs_moments_move_workspace_size(len(lens), lens_bytes, rows)
+        return torch.empty((nbytes,), dtype=torch.uint8, device=self.mu_flat.device)
+
+    def _move(self, index: torch.Tensor, ws: Optional[torch.Tensor]) -> None:
+        """``move_rows_`` by an index that was looked over, on the current device: allocates nothing there."""
+        dev = self.mu_flat.device
+        rows, lens, lens_bytes, row_bytes, _ = self._rows("move_rows_")
+        k, stream, bits = len(lens), _lib.stream_handle(dev), 8 * index.element_size()
+        flats = self._flats()
+        if flats:
+            each = len(flats)
+            _lib.call("gs_move_rows", stream, each * k, self._addresses(flats), row_bytes * each, row_bytes * each,
+                      rows, None, index.data_ptr(), bits, None)
+        if self.bits == 8:
+            _lib.call("gs_moments_move", stream, k, lens_bytes, rows, self._offsets, self.size,
+                      self.mu_flat.data_ptr(), self.nu_flat.data_ptr(), self.fields.data_ptr(), index.data_ptr(), bits,
+                      ws.data_ptr(), ws.numel())
+        _lib.tensors().written([], [], [self.mu_flat, self.nu_flat, self.fields, self.master_flat])
 
     def state_dict(self) -> dict:
         """The state as a dict of tensors (the state's own) and plain values, for a checkpoint."""

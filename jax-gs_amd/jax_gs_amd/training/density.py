@@ -93,6 +93,9 @@ def densify_and_prune(state: DensityState, generator: Optional[torch.Generator] 
     nbytes = _lib.lib().gs_densify_workspace_size(M)
     ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
     counts = torch.empty((5,), dtype=torch.int32, device=dev)
+    # everything is allocated before the first array changes: a call that runs out of memory leaves the state whole
+    moved_from = torch.empty((M,), dtype=torch.int32, device=dev) if after or sources else None
+    room = opt._move_workspace() if after else None
     P = ctypes.c_void_p * max(len(moments), 1)
     mptr = P(*[m.data_ptr() for m in moments]) if moments else None
     _lib.call("gs_densify_and_prune", _lib.stream_handle(dev), M, g.sh_coeffs.shape[1], _lib.ptr(g.means),
@@ -100,13 +103,13 @@ def densify_and_prune(state: DensityState, generator: Optional[torch.Generator] 
               len(moments), mptr, _lib.ptr(state.active_mask), _lib.ptr(state.grad_accum), _lib.ptr(state.denom),
               _lib.ptr(state.max_radii), _lib.ptr(noise), int(bool(densify_enabled)), float(grad_threshold),
               float(min_opacity), float(extent), float(max_screen_size), _lib.ptr(ws), nbytes, _lib.ptr(counts))
-    state.last_counts, state.last_sources = counts, None
-    if after or sources:
-        state.last_sources = torch.empty((M,), dtype=torch.int32, device=dev)
+    state.last_counts, state.last_sources = counts, moved_from
+    if moved_from is not None:
         _lib.call("gs_densify_sources", _lib.stream_handle(dev), M, _lib.ptr(ws), nbytes, _lib.ptr(counts),
-                  _lib.ptr(state.last_sources))
+                  _lib.ptr(moved_from))
     if after:
-        opt.move_rows_(state.last_sources)
+        with _lib.on(dev):
+            opt._move(moved_from, room)
     return state
 
 
