@@ -182,6 +182,9 @@ PyObject* do_pair(PyObject* params, PyObject* grads, PyObject* shapes, int64_t d
 void no_graph(const at::Tensor& t, const char* what) {
   if (t.requires_grad() && c10::GradMode::is_enabled())
     refuse(PyExc_RuntimeError, std::string(what) + " is not differentiated: call it under torch.no_grad()");
+  // torch.no_grad() does not stop the forward mode: a tangent would stay as it was, or be lost
+  if (t._fw_grad(0).defined())
+    refuse(PyExc_RuntimeError, std::string(what) + " is not differentiated: a tensor carries a tangent");
 }
 
 // The memory of a tensor's rows: rows * row bytes, `stride` from one to the next.
