@@ -284,26 +284,30 @@ class AdamWState:
             _lib.call("gs_moments_decode", _lib.stream_handle(dev), self.size, *map(_address, (
                 mu, nu, fields, self.mu_flat, self.nu_flat)))
 
-    def _rows(self, what: str):
+    def _rows(self, what: str, only: Optional[list] = None):
         """(rows, elements per row of each tensor, the same as int64, bytes per row in 32 bits, a row's shapes) of a
-        state whose tensors have the same rows."""
-        if self._row_layout is None:
-            rows = self.shapes[0][0] if len(self.shapes[0]) else None
-            if any([not len(s) or s[0] != rows for s in self.shapes]):
-                raise ValueError(f"AdamWState.{what}: the state's tensors do not have the same rows")
-            lens = [s[1:].numel() for s in self.shapes]
-            self._row_layout = (rows, lens, array("q", lens).tobytes(), array("q", [4 * n for n in lens]).tobytes(),
-                                [tuple(s[1:]) for s in self.shapes])
-        return self._row_layout
+        state whose tensors have the same rows; of the tensors with the numbers `only`, if given."""
+        if only is None and self._row_layout is not None:
+            return self._row_layout
+        shapes = self.shapes if only is None else [self.shapes[i] for i in only]
+        rows = shapes[0][0] if len(shapes[0]) else None
+        if any([not len(s) or s[0] != rows for s in shapes]):
+            raise ValueError(f"AdamWState.{what}: the state's tensors do not have the same rows")
+        lens = [s[1:].numel() for s in shapes]
+        layout = (rows, lens, array("q", lens).tobytes(), array("q", [4 * n for n in lens]).tobytes(),
+                  [tuple(s[1:]) for s in shapes])
+        if only is None:
+            self._row_layout = layout
+        return layout
 
     def _flats(self) -> list:
         """The float32 arrays."""
         flats = [self.mu_flat, self.nu_flat] if self.bits == 32 else []
         return flats if self.master_flat is None else flats + [self.master_flat]
 
-    def _addresses(self, flats) -> bytes:
-        """Of every tensor in each of the float32 arrays."""
-        offsets = self.offsets
+    def _addresses(self, flats, only: Optional[list] = None) -> bytes:
+        """Of every tensor (of `only`) in each of the float32 arrays."""
+        offsets = self.offsets if only is None else [self.offsets[i] for i in only]
         return array("q", [at + 4 * o for at in [x.data_ptr() for x in flats] for o in offsets]).tobytes()
 
     def take_rows(self, index) -> "AdamWState":
@@ -349,26 +353,28 @@ class AdamWState:
             self._move(index, self._move_workspace())
         return self
 
-    def _move_workspace(self) -> Optional[torch.Tensor]:
+    def _move_workspace(self, only: Optional[list] = None) -> Optional[torch.Tensor]:
         """What ``_move`` needs beside the state, so that it is there before anything is written."""
         if self.bits != 8:
             return None
-        rows, lens, lens_bytes, _, _ = self._rows("move_rows_")
+        rows, lens, lens_bytes, _, _ = self._rows("move_rows_", only)
         nbytes = _lib.lib().gs_moments_move_workspace_size(len(lens), lens_bytes, rows)
         return torch.empty((nbytes,), dtype=torch.uint8, device=self.mu_flat.device)
 
-    def _move(self, index: torch.Tensor, ws: Optional[torch.Tensor]) -> None:
-        """``move_rows_`` by an index that was looked over, on the current device: allocates nothing there."""
+    def _move(self, index: torch.Tensor, ws: Optional[torch.Tensor], only: Optional[list] = None) -> None:
+        """``move_rows_`` by an index that was looked over, on the current device: allocates nothing there.  `only`:
+        the numbers of the tensors that it is for, ascending, if not all."""
         dev = self.mu_flat.device
-        rows, lens, lens_bytes, row_bytes, _ = self._rows("move_rows_")
+        rows, lens, lens_bytes, row_bytes, _ = self._rows("move_rows_", only)
         k, stream, bits = len(lens), _lib.stream_handle(dev), 8 * index.element_size()
         flats = self._flats()
         if flats:
             each = len(flats)
-            _lib.call("gs_move_rows", stream, each * k, self._addresses(flats), row_bytes * each, row_bytes * each,
+            _lib.call("gs_move_rows", stream, each * k, self._addresses(flats, only), row_bytes * each, row_bytes * each,
                       rows, None, index.data_ptr(), bits, None)
         if self.bits == 8:
-            _lib.call("gs_moments_move", stream, k, lens_bytes, rows, self._offsets, self.size,
+            offsets = self._offsets if only is None else array("q", [self.offsets[i] for i in only]).tobytes()
+            _lib.call("gs_moments_move", stream, k, lens_bytes, rows, offsets, self.size,
                       self.mu_flat.data_ptr(), self.nu_flat.data_ptr(), self.fields.data_ptr(), index.data_ptr(), bits,
                       ws.data_ptr(), ws.numel())
         _lib.tensors().written([], [], [self.mu_flat, self.nu_flat, self.fields, self.master_flat])

@@ -69,7 +69,8 @@ def densify_and_prune(state: DensityState, generator: Optional[torch.Generator] 
     overrides the draws from ``generator``.  state.last_counts (int32 [5] on the device):
     clones, splits, pruned, available slots, densified.  With ``sources``,
     state.last_sources (int32 [M]) is the index by which ``rows.move_rows_`` moves what
-    else a program keeps for each Gaussian: the slot that each slot's rows came from."""
+    else a program keeps for each Gaussian: the slot that each slot's rows came from.
+    Of an optimizer's state the moments of the five arrays move, whatever else it is of."""
     g = state.gaussians
     M = g.means.shape[0]
     dev = g.means.device
@@ -80,10 +81,16 @@ def densify_and_prune(state: DensityState, generator: Optional[torch.Generator] 
         raise ValueError(f"densify_and_prune: noise must be [{M}, 3]")
     moments = []
     opt = state.opt_state
-    # 8-bit moments follow the other arrays by the index of sources
-    after = opt is not None and getattr(opt, "bits", 32) == 8
-    if after and (opt._rows("move_rows_")[0] != M or opt.mu_flat.device != dev):
-        raise ValueError(f"densify_and_prune: the optimizer's state must have the capacity rows, on {dev}")
+    # 8-bit moments follow the other arrays by the index of sources; those of other tensors in the state stay
+    after, only = opt is not None and getattr(opt, "bits", 32) == 8, None
+    if after:
+        if opt.keys is not None:
+            missing = [f for f in FIELDS if f not in opt.keys]
+            if missing:
+                raise ValueError(f"densify_and_prune: the optimizer's state has no moments of {missing}")
+            only = sorted(opt.keys.index(f) for f in FIELDS)
+        if opt._rows("move_rows_", only)[0] != M or opt.mu_flat.device != dev:
+            raise ValueError(f"densify_and_prune: the optimizer's state must have the capacity rows, on {dev}")
     if opt is not None and not after:
         mu, nu = opt.mu, opt.nu
         moments = [mu[f] for f in FIELDS] + [nu[f] for f in FIELDS]
@@ -95,7 +102,7 @@ def densify_and_prune(state: DensityState, generator: Optional[torch.Generator] 
     counts = torch.empty((5,), dtype=torch.int32, device=dev)
     # everything is allocated before the first array changes: a call that runs out of memory leaves the state whole
     moved_from = torch.empty((M,), dtype=torch.int32, device=dev) if after or sources else None
-    room = opt._move_workspace() if after else None
+    room = opt._move_workspace(only) if after else None
     P = ctypes.c_void_p * max(len(moments), 1)
     mptr = P(*[m.data_ptr() for m in moments]) if moments else None
     _lib.call("gs_densify_and_prune", _lib.stream_handle(dev), M, g.sh_coeffs.shape[1], _lib.ptr(g.means),
@@ -109,7 +116,7 @@ def densify_and_prune(state: DensityState, generator: Optional[torch.Generator] 
                   _lib.ptr(moved_from))
     if after:
         with _lib.on(dev):
-            opt._move(moved_from, room)
+            opt._move(moved_from, room, only)
     return state
 
 
