@@ -71,6 +71,14 @@ def _tensors(x, keys=None) -> list:
     return list(x)
 
 
+def _fills(fill, keys, count: int, what: str) -> list:
+    """The rows (or None) that new rows of `count` tensors get."""
+    fills = _tensors(fill, keys)
+    if len(fills) != count:
+        raise ValueError(f"{what}: {len(fills)} fills for {count} tensors")
+    return fills
+
+
 def _like(keys, values):
     return list(values) if keys is None else dict(zip(keys, values))
 
@@ -310,13 +318,37 @@ class AdamWState:
         offsets = self.offsets if only is None else [self.offsets[i] for i in only]
         return array("q", [at + 4 * o for at in [x.data_ptr() for x in flats] for o in offsets]).tobytes()
 
-    def take_rows(self, index) -> "AdamWState":
+    def _master_fills(self, fill, row_shapes: list, what: str) -> Optional[list]:
+        """The masters' new rows, copies in float32 of the parameters' `fill`; None without masters or fills."""
+        if fill is None:
+            return None
+        dev, rows = self.mu_flat.device, []
+        for i, (f, s) in enumerate(zip(_fills(fill, self.keys, len(row_shapes), what), row_shapes)):
+            if f is not None:
+                if not isinstance(f, torch.Tensor) or not f.is_floating_point() or f.device != dev or tuple(f.shape) != s:
+                    raise ValueError(f"{what}: fill {i} must be one row of its tensor, of shape {s} on {dev}")
+                if self.master_flat is not None:
+                    f = torch.empty(s, dtype=torch.float32, device=dev).copy_(f.detach())
+            rows.append(f)
+        return None if self.master_flat is None else rows
+
+    @staticmethod
+    def _fill_addresses(fills: Optional[list], each: int) -> Optional[bytes]:
+        """Of the masters' new rows, behind none for the moments: the masters are the last of `each` float32 arrays."""
+        if fills is None:
+            return None
+        rows = [0 if f is None else f.data_ptr() for f in fills]
+        return array("q", [0] * (len(rows) * (each - 1)) + rows).tobytes()
+
+    def take_rows(self, index, fill=None) -> "AdamWState":
         """A state of its own for tensors whose row i is these tensors' row ``index[i]`` (``rows.take_rows``
-        of the parameters): moments and masters of those rows, zeros where ``index`` is no row's.  8-bit
+        of the parameters): moments and masters of those rows.  Where ``index`` is no row's the moments are
+        zero and the masters hold ``fill``, which is that of the parameters (zeros without it).  8-bit
         moments are rounded to nearest where a new neighbour raises the exponent of their block."""
         dev = self.mu_flat.device
         index = row_index(index, dev, "AdamWState.take_rows")
         rows, lens, lens_bytes, row_bytes, row_shapes = self._rows("take_rows")
+        fills = self._master_fills(fill, row_shapes, "AdamWState.take_rows")
         count, k = index.numel(), len(lens)
         to = AdamWState.__new__(AdamWState)
         to.__dict__.update(self.__dict__)  # the powers are never written in place
@@ -334,23 +366,26 @@ class AdamWState:
                 each = len(flats)
                 padded = array("q", [4 * (b - a) for a, b in zip(to.offsets, to.offsets[1:] + [to.size])]).tobytes()
                 _lib.call("gs_take_rows", stream, each * k, self._addresses(flats), row_bytes * each, row_bytes * each,
-                          rows, to._addresses(to._flats()), padded * each, None, *of)
+                          rows, to._addresses(to._flats()), padded * each,
+                          self._fill_addresses(fills, each), *of)
             if self.bits == 8:
                 _lib.call("gs_moments_take", stream, k, lens_bytes, rows, self._offsets, self.size,
                           self.mu_flat.data_ptr(), self.nu_flat.data_ptr(), self.fields.data_ptr(), *of, to._offsets,
                           to.size, to.mu_flat.data_ptr(), to.nu_flat.data_ptr(), to.fields.data_ptr())
         return to
 
-    def move_rows_(self, index) -> "AdamWState":
-        """In place, the moments and masters of row i become those of row ``index[i]``, or zero where ``index``
-        is negative, as ``rows.move_rows_`` moves the parameters.  Returns the state."""
+    def move_rows_(self, index, fill=None) -> "AdamWState":
+        """In place, the moments and masters of row i become those of row ``index[i]``, as ``rows.move_rows_``
+        moves the parameters.  Where ``index`` is negative the moments become zero and the masters ``fill``, which is
+        that of the parameters (zero without it).  Returns the state."""
         dev = self.mu_flat.device
         index = row_index(index, dev, "AdamWState.move_rows_")
-        rows = self._rows("move_rows_")[0]
+        rows, _, _, _, row_shapes = self._rows("move_rows_")
         if index.numel() != rows:
             raise ValueError(f"AdamWState.move_rows_: {index.numel()} indices for {rows} rows")
+        fills = self._master_fills(fill, row_shapes, "AdamWState.move_rows_")
         with _lib.on(dev):
-            self._move(index, self._move_workspace())
+            self._move(index, self._move_workspace(), fills=fills)
         return self
 
     def _move_workspace(self, only: Optional[list] = None) -> Optional[torch.Tensor]:
@@ -361,7 +396,8 @@ class AdamWState:
         nbytes = _lib.lib().gs_moments_move_workspace_size(len(lens), lens_bytes, rows)
         return torch.empty((nbytes,), dtype=torch.uint8, device=self.mu_flat.device)
 
-    def _move(self, index: torch.Tensor, ws: Optional[torch.Tensor], only: Optional[list] = None) -> None:
+    def _move(self, index: torch.Tensor, ws: Optional[torch.Tensor], only: Optional[list] = None,
+              fills: Optional[list] = None) -> None:
         """``move_rows_`` by an index that was looked over, on the current device: allocates nothing there.  `only`:
         the numbers of the tensors that it is for, ascending, if not all."""
         dev = self.mu_flat.device
@@ -371,7 +407,7 @@ class AdamWState:
         if flats:
             each = len(flats)
             _lib.call("gs_move_rows", stream, each * k, self._addresses(flats, only), row_bytes * each, row_bytes * each,
-                      rows, None, index.data_ptr(), bits, None)
+                      rows, self._fill_addresses(fills, each), index.data_ptr(), bits, None)
         if self.bits == 8:
             offsets = self._offsets if only is None else array("q", [self.offsets[i] for i in only]).tobytes()
             _lib.call("gs_moments_move", stream, k, lens_bytes, rows, offsets, self.size,

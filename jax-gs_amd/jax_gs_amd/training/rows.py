@@ -22,14 +22,7 @@ import torch
 from .. import _lib
 from ..core.gaussians import Gaussians
 from ..renderer._buffers import as_bytes
-from .adamw import _device, _keys, _tensors, row_index
-
-
-def _fills(fill, keys, count: int, what: str):
-    fills = _tensors(fill, keys)
-    if len(fills) != count:
-        raise ValueError(f"{what}: {len(fills)} fills for {count} tensors")
-    return fills
+from .adamw import _device, _fills, _keys, _tensors, row_index
 
 
 def _like(tensors, new: list):
