@@ -200,9 +200,10 @@ class AdamWState:
     number of steps asked for; ``powers`` (device float64) belongs to the updates made, which
     are fewer if a scale was not finite."""
 
+    _row_layout = None  # _rows; of the class, as states that were saved whole may not have one
+
     def __init__(self, keys, shapes, bits: int):
         self.keys, self.shapes, self.bits = keys, [torch.Size(s) for s in shapes], bits
-        self._row_layout = None  # _rows
         self._lay_out([s.numel() for s in self.shapes])
         self.mu_flat = self.nu_flat = self.fields = self.master_flat = self.powers = None
         self._powers_stream: Optional[int] = None  # that the powers were allocated on
