@@ -157,6 +157,7 @@ def _train_step_fused(state, target_image, camera, optimizer, sh_degree, fast_tp
                   optimizer.eps, _lib.ptr(state.active_mask), _lib.ptr(valid), _lib.ptr(pre["radii"]), focal,
                   pixel_scale, _lib.ptr(state.grad_accum), _lib.ptr(state.denom), _lib.ptr(state.max_radii))
         ost.count += 1
+        ost.norms = None  # no gradients were clipped
         metrics = {"l1": l1, "ssim": terms[4]}
         metrics.update(_stats_metrics(b["stats"]))
     return state, total, metrics
