@@ -92,7 +92,8 @@ class Adam:
         if self.max_grad_norm is not None:
             from .adamw import clip_grads_
 
-            state.norms = clip_grads_([a[1] for a in arrays], self.max_grad_norm, active_mask=act)
+            state.norms = clip_grads_([a[1] for a in arrays], self.max_grad_norm,
+                                      active_mask=None if act is None else act.reshape(-1))
         k = len(arrays)
         P = ctypes.c_void_p * k
         _lib.call("gs_adam_step", _lib.stream_handle(dev), k, P(*[a[0].data_ptr() for a in arrays]),

@@ -26,3 +26,20 @@ def test_norms_are_those_of_the_last_step(cuda):
         _, _, metrics = train_step(state, tgt, cam.W2C, static, plain, sh_degree=3, fused=fused)
         assert "grad_norm" not in metrics and state.opt_state.norms is None
     assert state.opt_state.count == 4
+
+
+def test_a_mask_of_one_column(cuda):
+    """Adam takes any mask with an entry for each Gaussian, with clipping too."""
+    n = 300
+    gen = torch.Generator(device=cuda).manual_seed(1)
+    some = lambda: Gaussians(*[torch.randn(n, *s, generator=gen, device=cuda) for s in ((3,), (3,), (4,), (1,), (16, 3))])
+    params, grads = some(), some()
+    mask = torch.rand(n, generator=gen, device=cuda) < 0.5
+    runs = []
+    for m in (mask, mask[:, None], mask.view(1, n, 1).to(torch.int32)):
+        p, g = [Gaussians(*[getattr(x, f).clone() for f in FIELDS]) for x in (params, grads)]
+        opt = Adam(RATES, max_grad_norm=0.5)
+        state = opt.step(p, g, opt.init(p), active_mask=m)
+        runs.append([state.norms.total, *[getattr(x, f) for x in (p, g) for f in FIELDS]])
+    for run in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(runs[0], run))
