@@ -84,7 +84,7 @@ def densify_and_prune(state: DensityState, generator: Optional[torch.Generator] 
     # 8-bit moments follow the other arrays by the index of sources; those of other tensors in the state stay
     after, only = opt is not None and getattr(opt, "bits", 32) == 8, None
     if after:
-        if opt.keys is not None:
+        if opt.keys is not None and opt.keys != list(FIELDS):
             missing = [f for f in FIELDS if f not in opt.keys]
             if missing:
                 raise ValueError(f"densify_and_prune: the optimizer's state has no moments of {missing}")
