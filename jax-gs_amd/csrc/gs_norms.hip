@@ -337,8 +337,10 @@ __device__ inline double sum_of(const double* __restrict__ partial, int n, doubl
   return (w[0] + w[1]) + (w[2] + w[3]);
 }
 
-// Every workgroup adds all partial sums for itself: up to 16 KiB out of L2, which takes less than a launch that does
-// it once for all.
+// Every workgroup adds all partial sums for itself, up to 2 * kNormRuns of them (32 KiB out of L2), which takes less than a
+// launch that does it once for all: one tensor of 16M elements (2048 sums) 17.6 us, 19.8 with the launch; beside it 1000
+// tensors of 1000 elements 75 and 81, 3000 of them (4024 sums) 203 and 205.  Beyond, the launch is faster: 6000 such
+// tensors alone 394 and 379.
 template <bool kStream>
 __global__ __launch_bounds__(256) void grad_scale_kernel(ScaleArgs S) {
   const NormArgs& A = S.a;
