@@ -394,7 +394,9 @@ __device__ inline void take_odd(const MomentArgs& A, const MomentRecord& t, uint
 }
 
 // Where there are rows of a multiple of sixteen elements, which want registers (of 48: 65 us at five waves a SIMD, 133 at
-// eight), all tensors go together, where there are none at eight waves (rows of 45: 114 us, 133 at five).
+// eight), all tensors go together, at five waves; where there are none at seven (1.4M of 2M rows of 45: 106 us by an int32
+// index, 107 by an int64 one; the same at eight waves, which keep two or seven registers in scratch; 115 on another card,
+// on which rows of 16 beside them take 137 together and 21 alone).
 template <bool kWide>
 __global__ __launch_bounds__(256) void moment_take_kernel(MomentArgs A) {
   const uint32_t b = blockIdx.x;
@@ -416,7 +418,7 @@ __global__ __launch_bounds__(256) void moment_take_kernel(MomentArgs A) {
 }
 
 template <bool kWide>
-__global__ __launch_bounds__(256, 8) void moment_take_odd_kernel(MomentArgs A) {
+__global__ __launch_bounds__(256, 7) void moment_take_odd_kernel(MomentArgs A) {
   const uint32_t b = blockIdx.x;
   if (b >= A.groups) return;
   const int k = tensor_of(A, b);
