@@ -35,7 +35,7 @@ def _like(tensors, new: list):
 
 
 def take_rows(tensors, index: torch.Tensor, fill=None):
-    """New tensors, in the form of the given ones, whose row i is row ``index[i]``: an index that comes
+    """New tensors, in the form of the given ones (a list for a tuple), whose row i is row ``index[i]``: an index that comes
     twice forks a row, one that does not come drops it.  Where ``index`` is negative or not a
     row's, the row holds ``fill`` (for each tensor one row or None; zeros without it)."""
     ts = _tensors(tensors)
